@@ -66,7 +66,7 @@
 extern "C" {
 #endif
 
-#define TRINIX_ATTN_ABI_VERSION 6
+#define TRINIX_ATTN_ABI_VERSION 7
 
 typedef enum trinix_status {
   TRINIX_OK = 0,
@@ -445,6 +445,79 @@ int trinix_dropout_keep_map_bytes(int64_t batch, int64_t nheads_q, int64_t seqle
 
 /* TRINIX_ATTN_ABI_VERSION of the built library. */
 int trinix_abi_version(void);
+
+/* ---- attention over packed sequences (ABI version 7) -----------------------
+ * No counterpart in the reference, whose attention takes (batch, seq, head,
+ * head_dim) tensors of one length (attention_kernel.py:497-517).
+ *
+ * n_seqs sequences of different lengths lie one behind the other in the rows of
+ * q (total_q, Hq, D) and of k and v (total_k, Hkv, D): sequence s holds query
+ * rows cu_q[s] .. cu_q[s + 1] - 1 and keys cu_k[s] .. cu_k[s + 1] - 1
+ * (int32, n_seqs + 1 entries each, device memory; entry 0 is taken as 0).  With
+ * Lq and Lk of them and off = Lk - Lq, the queries are the sequence's last
+ * positions (a whole prompt: off = 0; a chunk behind its cache: off > 0):
+ *   s[i,j] = scale * <q_i, k_j> - slope[h] * |i + off - j|   (if alibi_slopes)
+ *   s[i,j] = -inf unless  j <= i + off            (if causal),
+ *                         -wl <= j - i - off <= wr (if has_window)
+ *   out_i = softmax_j(s[i,:]) @ v,  lse_i = log(sum_j exp(s[i,j]))
+ * A row that sees no key has out 0 and lse -inf, and takes no part in any
+ * gradient.  Rows behind the last sequence are such rows; keys behind it get
+ * gradients of 0.
+ *
+ * The plan is a table of work items built on the GPU from cu_q and cu_k
+ * (nothing is read back); boundaries are clamped into the tensors and made
+ * non-decreasing, so that no content of the arrays reads or writes outside.
+ * trinix_packed_plan_bytes: its size (host only; TRINIX_ERR_BAD_SHAPE unless
+ * 1 <= n_seqs < 2^24 and 0 <= total_q, total_k < 2^30).
+ * trinix_packed_plan: writes it on `stream`; plan 16-byte aligned.  A plan
+ * serves any number of calls with the same n_seqs, total_q and total_k. */
+int trinix_packed_plan_bytes(int64_t n_seqs, int64_t total_q, int64_t total_k,
+                             int64_t* bytes);
+int trinix_packed_plan(const int32_t* cu_q, const int32_t* cu_k, int64_t n_seqs,
+                       int64_t total_q, int64_t total_k, int32_t* plan,
+                       int64_t plan_bytes, void* stream);
+
+typedef struct trinix_packed_args {
+  const void* q;        /* (total_q, Hq, D)  */
+  const void* k;        /* (total_k, Hkv, D) */
+  const void* v;        /* (total_k, Hkv, D) */
+  void* out;            /* (total_q, Hq, D): written forward, read backward */
+  void* out_lo;         /* 16-bit types: what out lost by its rounding, laid
+                         * out like out (bf16; fp16 times 2^11), for a backward;
+                         * written forward if not NULL, read backward */
+  float* lse;           /* (Hq, total_q) contiguous; forward: or NULL */
+  int64_t q_stride[3];  /* elements: row, head, d (1) */
+  int64_t k_stride[3];
+  int64_t v_stride[3];
+  int64_t out_stride[3];
+  /* backward only */
+  const void* dout;     /* (total_q, Hq, D)  */
+  float* delta;         /* (Hq, total_q) scratch */
+  void* dq;             /* (total_q, Hq, D)  */
+  void* dk;             /* (total_k, Hkv, D) */
+  void* dv;
+  int64_t dout_stride[3];
+  int64_t dq_stride[3];
+  int64_t dk_stride[3];
+  int64_t dv_stride[3];
+  const int32_t* plan;  /* from trinix_packed_plan */
+  int64_t plan_bytes;
+  int64_t n_seqs, total_q, total_k;
+  int64_t nheads_q, nheads_kv, head_dim; /* head_dim 64, 128 or 256 */
+  int32_t dtype;        /* TRINIX_F32, TRINIX_F16 or TRINIX_BF16 */
+  float softmax_scale;
+  int32_t causal;
+  int32_t has_window;
+  int64_t window_left, window_right;
+  const float* alibi_slopes; /* (Hq) fp32, or NULL */
+  int64_t alibi_stride;
+} trinix_packed_args;
+
+/* Forward and backward on `stream`; 16-bit rows 16-byte aligned.  The backward
+ * takes the forward's out, out_lo and lse.  No atomics: the same call gives the
+ * same bits. */
+int trinix_packed_fwd(const trinix_packed_args* args, void* stream);
+int trinix_packed_bwd(const trinix_packed_args* args, void* stream);
 
 #ifdef __cplusplus
 }

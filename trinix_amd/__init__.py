@@ -12,6 +12,8 @@ from .layers.attention import (
     FastMultiHeadAttention,
     FastMultiHeadSelfAttention,
     FastMultiQueryAttention,
+    PackedSequences,
+    packed_attn_func,
     triton_attn_func,
 )
 from .layers.embeddings import FastALiBiPositionEmbedding, FastRoPEPositionEmbedding
@@ -22,6 +24,8 @@ __all__ = [
     "TritonRoPEKernel",
     "calculate_attention_block_sizes",
     "triton_attn_func",
+    "PackedSequences",
+    "packed_attn_func",
     "FastBaseAttention",
     "FastGroupedQueryAttention",
     "FastMultiHeadAttention",

@@ -40,10 +40,11 @@ TRINIX_NORM_LAYER = 1
 BLOCKMAP_ROWS = 32
 BLOCKMAP_COLS = 64
 
-ABI_VERSION = 6
+ABI_VERSION = 7
 
 Int64x4 = c_int64 * 4
 Int64x2 = c_int64 * 2
+Int64x3 = c_int64 * 3
 
 
 class AttnFwdArgs(ctypes.Structure):
@@ -141,6 +142,48 @@ class AttnBwdArgs(ctypes.Structure):
     ]
 
 
+class PackedArgs(ctypes.Structure):
+    """Mirror of ``trinix_packed_args`` (field order and types identical)."""
+
+    _fields_ = [
+        ("q", c_void_p),
+        ("k", c_void_p),
+        ("v", c_void_p),
+        ("out", c_void_p),
+        ("out_lo", c_void_p),
+        ("lse", c_void_p),
+        ("q_stride", Int64x3),
+        ("k_stride", Int64x3),
+        ("v_stride", Int64x3),
+        ("out_stride", Int64x3),
+        ("dout", c_void_p),
+        ("delta", c_void_p),
+        ("dq", c_void_p),
+        ("dk", c_void_p),
+        ("dv", c_void_p),
+        ("dout_stride", Int64x3),
+        ("dq_stride", Int64x3),
+        ("dk_stride", Int64x3),
+        ("dv_stride", Int64x3),
+        ("plan", c_void_p),
+        ("plan_bytes", c_int64),
+        ("n_seqs", c_int64),
+        ("total_q", c_int64),
+        ("total_k", c_int64),
+        ("nheads_q", c_int64),
+        ("nheads_kv", c_int64),
+        ("head_dim", c_int64),
+        ("dtype", c_int32),
+        ("softmax_scale", c_float),
+        ("causal", c_int32),
+        ("has_window", c_int32),
+        ("window_left", c_int64),
+        ("window_right", c_int64),
+        ("alibi_slopes", c_void_p),
+        ("alibi_stride", c_int64),
+    ]
+
+
 class TileCfg(ctypes.Structure):
     """Mirror of ``trinix_tile_cfg``."""
 
@@ -192,6 +235,10 @@ SIGNATURES = {
          c_void_p, c_void_p, c_int64, c_void_p],
     ),
     "trinix_alibi_bias": (c_int32, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p]),
+    "trinix_packed_plan_bytes": (c_int32, [c_int64, c_int64, c_int64, POINTER(c_int64)]),
+    "trinix_packed_plan": (c_int32, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p]),
+    "trinix_packed_fwd": (c_int32, [POINTER(PackedArgs), c_void_p]),
+    "trinix_packed_bwd": (c_int32, [POINTER(PackedArgs), c_void_p]),
     "trinix_attn_tile_config": (c_int32, [c_int64, c_int32, POINTER(TileCfg)]),
     "trinix_dropout_state_advance": (c_int32, [c_void_p, c_void_p, c_uint64, c_void_p]),
     "trinix_dropout_keep_map_bytes": (c_int32, [c_int64, c_int64, c_int64, c_int64, c_void_p]),

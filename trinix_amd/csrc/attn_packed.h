@@ -1,0 +1,87 @@
+// Attention over packed sequences: parameters, the work item of a workgroup and
+// the pieces that its kernels share (semantics: trinix_attn.h, trinix_packed_args).
+#pragma once
+#include "attn_params.h"
+#include "lds_tile.h"
+#include "packed_map.h"
+
+namespace trinix {
+
+struct PackedParams {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* o;
+  void* o_lo;  // what o lost by rounding (16-bit), or null
+  float* lse;
+  const void* dout;
+  float* delta;
+  void* dq;
+  void* dk;
+  void* dv;
+  int64_t q_ss, q_sh, k_ss, k_sh, v_ss, v_sh, o_ss, o_sh;
+  int64_t do_ss, do_sh, dq_ss, dq_sh, dk_ss, dk_sh, dv_ss, dv_sh;
+  int Tq, Hq, Hkv, G;
+  float scale, scale_log2;
+  int causal, has_window;
+  int64_t wl, wr;  // clamped to +-2^30
+  const float* alibi;
+  int64_t al_sh;
+  int rows16;             // fp32: q, k, v and dout take 16-byte copies
+  const int32_t* items;   // of the launch's list
+};
+
+// The block of rows or keys that a workgroup runs: its sequence (first row and
+// rows, first key and keys), block number (-1: none) and head, all wave-uniform.
+struct PackedBlock {
+  int q0, lq, k0, lk, blk, h, dlo, dhi;
+  __device__ PackedBlock(const PackedParams& p, int wg, int heads_kv, int G) {
+    typedef int i32x4 __attribute__((ext_vector_type(4)));
+    const PackedWork w = packed_work(wg, heads_kv, G);
+    const i32x4* it = (const i32x4*)(p.items + (int64_t)w.item * kPackedItemInts);
+    const i32x4 a = it[0];
+    q0 = __builtin_amdgcn_readfirstlane(a[0]);
+    lq = __builtin_amdgcn_readfirstlane(a[1]);
+    k0 = __builtin_amdgcn_readfirstlane(a[2]);
+    lk = __builtin_amdgcn_readfirstlane(a[3]);
+    blk = __builtin_amdgcn_readfirstlane(it[1][0]);
+    h = w.h;
+    packed_band(lq, lk, p.causal != 0, p.has_window != 0, p.wl, p.wr, dlo, dhi);
+  }
+  // keys that query row i sees, and rows that see key j (empty outside the sequence)
+  __device__ Span keys_of(int i) const {
+    return i < lq ? Span(max((int64_t)0, (int64_t)i + dlo), min((int64_t)lk - 1, (int64_t)i + dhi)) : Span(1, 0);
+  }
+  __device__ Span rows_of(int j) const {
+    return j < lk ? Span(max((int64_t)0, (int64_t)j - dhi), min((int64_t)lq - 1, (int64_t)j - dlo)) : Span(1, 0);
+  }
+  // Block of rows [ia, ia + ni) and keys [ja, ja + nj): does it hold allowed
+  // pairs; are all of its pairs allowed?
+  __device__ bool live(int ia, int ni, int ja, int nj) const {
+    if (ia >= lq || ja >= lk) return false;
+    const int ib = min(ia + ni, lq) - 1, jb = min(ja + nj, lk) - 1;
+    return ja - ib <= dhi && jb - ia >= dlo;
+  }
+  __device__ bool full(int ia, int ni, int ja, int nj) const {
+    return ia + ni <= lq && ja + nj <= lk && ja + nj - 1 - ia <= dhi && ja - (ia + ni - 1) >= dlo;
+  }
+};
+
+// fp16 keeps its output's rounding residue times 2^11 (half a step of the
+// largest fp16 number is 2^4; unscaled, the residue of 2^-10 would be denormal).
+template <class E>
+constexpr float kLoScale = std::is_same<E, F16>::value ? 2048.f : 1.f;
+
+// Launchers, one translation unit per type (attn_packed_*.hip).  rows: block
+// size of the item list that p.items points at.
+hipError_t launch_packed_fwd_bf16(const PackedParams& p, int D, int grid, hipStream_t st);
+hipError_t launch_packed_fwd_f16(const PackedParams& p, int D, int grid, hipStream_t st);
+hipError_t launch_packed_fwd_f32(const PackedParams& p, int D, int grid, hipStream_t st);
+hipError_t launch_packed_dkdv_bf16(const PackedParams& p, int D, int grid, hipStream_t st);
+hipError_t launch_packed_dkdv_f16(const PackedParams& p, int D, int grid, hipStream_t st);
+hipError_t launch_packed_dkdv_f32(const PackedParams& p, int D, int grid, hipStream_t st);
+hipError_t launch_packed_dq_bf16(const PackedParams& p, int D, int grid, hipStream_t st);
+hipError_t launch_packed_dq_f16(const PackedParams& p, int D, int grid, hipStream_t st);
+hipError_t launch_packed_dq_f32(const PackedParams& p, int D, int grid, hipStream_t st);
+
+}  // namespace trinix

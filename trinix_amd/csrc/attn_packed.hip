@@ -1,0 +1,146 @@
+// Entry points of attention over packed sequences, and the delta pass of its
+// backward.
+#include "attn_packed.h"
+#include "packed_host.h"
+
+namespace trinix {
+namespace {
+
+// delta[h, t] = sum_d dO[t, h, d] * O[t, h, d] in fp32, O with the part that its
+// rounding took off (o_lo): with O as rounded, delta is off by half a step of O,
+// which dZ = P (dP - delta) amplifies where a row's softmax is peaked (dQ and dK of
+// bf16 then err up to 1.9 times as much as from their own rounding).
+// VE elements (16 bytes) per lane, D / VE lanes per row.
+template <class E, int D, bool F32>
+__global__ __launch_bounds__(256) void packed_delta_kernel(const PackedParams p, int64_t rows) {
+  typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+  constexpr int VE = F32 ? 4 : 8, LPR = D / VE, RPB = 256 / LPR;
+  const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / LPR;  // t * Hq + h
+  const int c = threadIdx.x % LPR;
+  float acc = 0.f;
+  const int64_t t = row / p.Hq;
+  const int h = (int)(row % p.Hq);
+  if (row < rows) {
+    const int64_t oo = t * p.o_ss + h * p.o_sh + c * VE, od = t * p.do_ss + h * p.do_sh + c * VE;
+    if constexpr (F32) {
+      const f32x4_t o = *(const f32x4_any*)((const float*)p.o + oo), d = *(const f32x4_any*)((const float*)p.dout + od);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc += o[e] * d[e];
+    } else {
+      const u32x4_t o = *(const u32x4_t*)((const uint16_t*)p.o + oo), r = *(const u32x4_t*)((const uint16_t*)p.o_lo + oo);
+      const u32x4_t d = *(const u32x4_t*)((const uint16_t*)p.dout + od);
+      constexpr float f = 1.f / kLoScale<E>;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        acc += __builtin_fmaf(E::lo(r[e]), f, E::lo(o[e])) * E::lo(d[e]) +
+               __builtin_fmaf(E::hi(r[e]), f, E::hi(o[e])) * E::hi(d[e]);
+    }
+  }
+#pragma unroll
+  for (int m = LPR / 2; m >= 1; m /= 2) acc += __shfl_xor(acc, m);
+  if (c == 0 && row < rows) {
+    const int64_t at = (int64_t)h * p.Tq + t;
+    // a row that sees no key: P = 0 and delta = 0, whatever its dO holds
+    p.delta[at] = p.lse[at] == -INFINITY ? 0.f : acc;
+  }
+}
+
+template <class E, bool F32>
+hipError_t launch_delta(const PackedParams& p, int D, hipStream_t st) {
+  const int64_t rows = (int64_t)p.Tq * p.Hq;
+  const int rpb = 256 * (F32 ? 4 : 8) / D;
+  const dim3 grid((unsigned)((rows + rpb - 1) / rpb)), block(256);
+  switch (D) {
+    case 64: return launch_kernel(&packed_delta_kernel<E, 64, F32>, grid, block, 0, st, p, rows);
+    case 128: return launch_kernel(&packed_delta_kernel<E, 128, F32>, grid, block, 0, st, p, rows);
+    case 256: return launch_kernel(&packed_delta_kernel<E, 256, F32>, grid, block, 0, st, p, rows);
+  }
+  return hipErrorNotSupported;
+}
+
+bool rows16(const void* ptr, const int64_t st[3]) {
+  const int64_t st4[4] = {0, st[0], st[1], 1};
+  return rows_aligned16(ptr, st4);
+}
+
+PackedParams params(const trinix_packed_args* a) {
+  PackedParams p{};
+  p.q = a->q, p.k = a->k, p.v = a->v, p.o = a->out, p.o_lo = a->out_lo, p.lse = a->lse;
+  p.dout = a->dout, p.delta = a->delta, p.dq = a->dq, p.dk = a->dk, p.dv = a->dv;
+  p.q_ss = a->q_stride[0], p.q_sh = a->q_stride[1];
+  p.k_ss = a->k_stride[0], p.k_sh = a->k_stride[1];
+  p.v_ss = a->v_stride[0], p.v_sh = a->v_stride[1];
+  p.o_ss = a->out_stride[0], p.o_sh = a->out_stride[1];
+  p.do_ss = a->dout_stride[0], p.do_sh = a->dout_stride[1];
+  p.dq_ss = a->dq_stride[0], p.dq_sh = a->dq_stride[1];
+  p.dk_ss = a->dk_stride[0], p.dk_sh = a->dk_stride[1];
+  p.dv_ss = a->dv_stride[0], p.dv_sh = a->dv_stride[1];
+  p.Tq = (int)a->total_q;
+  p.Hq = (int)a->nheads_q;
+  p.Hkv = (int)a->nheads_kv;
+  p.G = p.Hq / p.Hkv;
+  p.scale = a->softmax_scale;
+  p.scale_log2 = a->softmax_scale * kLog2e;
+  p.causal = a->causal ? 1 : 0;
+  p.has_window = a->has_window ? 1 : 0;
+  p.wl = clamp_window(a->window_left);
+  p.wr = clamp_window(a->window_right);
+  p.alibi = a->alibi_slopes;
+  p.al_sh = a->alibi_stride;
+  return p;
+}
+
+// Points p at a list of the plan; returns its items.
+int64_t use_list(PackedParams& p, const trinix_packed_args* a, int list) {
+  p.items = a->plan + packed_list_offset(list, a->total_q, a->total_k, a->n_seqs);
+  return packed_list_cap(packed_list_is_keys(list) ? a->total_k : a->total_q, a->n_seqs, packed_list_block(list));
+}
+constexpr int kRows128 = 1, kKeys128 = 4;
+
+}  // namespace
+}  // namespace trinix
+
+using namespace trinix;
+
+extern "C" int trinix_packed_fwd(const trinix_packed_args* a, void* stream) {
+  const int rc = validate_packed(a, false);
+  if (rc != TRINIX_OK) return rc;
+  if (a->total_q == 0) return TRINIX_OK;
+  PackedParams p = params(a);
+  hipStream_t st = (hipStream_t)stream;
+  const int D = (int)a->head_dim, grid = (int)(use_list(p, a, kRows128) * p.Hq);
+  hipError_t e;
+  if (a->dtype == TRINIX_F32) {
+    p.rows16 = rows16(a->k, a->k_stride) && rows16(a->v, a->v_stride);
+    e = launch_packed_fwd_f32(p, D, grid, st);
+  } else {
+    e = a->dtype == TRINIX_BF16 ? launch_packed_fwd_bf16(p, D, grid, st) : launch_packed_fwd_f16(p, D, grid, st);
+  }
+  return e == hipSuccess ? TRINIX_OK : TRINIX_ERR_LAUNCH;
+}
+
+extern "C" int trinix_packed_bwd(const trinix_packed_args* a, void* stream) {
+  const int rc = validate_packed(a, true);
+  if (rc != TRINIX_OK) return rc;
+  PackedParams p = params(a);
+  hipStream_t st = (hipStream_t)stream;
+  const int D = (int)a->head_dim;
+  const bool f32 = a->dtype == TRINIX_F32, bf = a->dtype == TRINIX_BF16;
+  hipError_t e = hipSuccess;
+  if (f32) p.rows16 = rows16(a->q, a->q_stride) && rows16(a->dout, a->dout_stride);
+  if (a->total_q > 0) {
+    e = f32 ? launch_delta<BF16, true>(p, D, st) : bf ? launch_delta<BF16, false>(p, D, st) : launch_delta<F16, false>(p, D, st);
+    if (e != hipSuccess) return TRINIX_ERR_LAUNCH;
+  }
+  if (a->total_k > 0) {
+    const int grid = (int)(use_list(p, a, kKeys128) * p.Hkv);
+    e = f32 ? launch_packed_dkdv_f32(p, D, grid, st) : bf ? launch_packed_dkdv_bf16(p, D, grid, st) : launch_packed_dkdv_f16(p, D, grid, st);
+    if (e != hipSuccess) return TRINIX_ERR_LAUNCH;
+  }
+  if (a->total_q > 0) {
+    if (f32) p.rows16 = rows16(a->k, a->k_stride) && rows16(a->v, a->v_stride);
+    const int grid = (int)(use_list(p, a, kRows128) * p.Hq);
+    e = f32 ? launch_packed_dq_f32(p, D, grid, st) : bf ? launch_packed_dq_bf16(p, D, grid, st) : launch_packed_dq_f16(p, D, grid, st);
+  }
+  return e == hipSuccess ? TRINIX_OK : TRINIX_ERR_LAUNCH;
+}

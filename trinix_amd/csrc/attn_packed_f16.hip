@@ -1,0 +1,32 @@
+// Packed-sequence attention kernels, f16.
+#include "attn_packed_generic.h"
+
+namespace trinix {
+
+hipError_t launch_packed_fwd_f16(const PackedParams& p, int D, int grid, hipStream_t st) {
+  const dim3 g((unsigned)grid), b(256);
+  switch (D) {
+    case 64: return launch_kernel(&packed_fwd_generic<Ops16<F16, 64>, F16, 2>, g, b, 0, st, p);
+    case 128: return launch_kernel(&packed_fwd_generic<Ops16<F16, 128>, F16, 2>, g, b, 0, st, p);
+    case 256: return launch_kernel(&packed_fwd_generic<Ops16<F16, 256>, F16, 1>, g, b, 0, st, p);
+  }
+  return hipErrorNotSupported;
+}
+hipError_t launch_packed_dkdv_f16(const PackedParams& p, int D, int grid, hipStream_t st) {
+  switch (D) {
+    case 64: return launch_packed_dkdv_g<Ops16<F16, 64>, 2, 1>(p, grid, st);
+    case 128: return launch_packed_dkdv_g<Ops16<F16, 128>, 1, 1>(p, grid, st);
+    case 256: return launch_packed_dkdv_g<Ops16<F16, 256>, 1, 2>(p, grid, st);
+  }
+  return hipErrorNotSupported;
+}
+hipError_t launch_packed_dq_f16(const PackedParams& p, int D, int grid, hipStream_t st) {
+  switch (D) {
+    case 64: return launch_packed_dq_g<Ops16<F16, 64>, 2, 1>(p, grid, st);
+    case 128: return launch_packed_dq_g<Ops16<F16, 128>, 1, 1>(p, grid, st);
+    case 256: return launch_packed_dq_g<Ops16<F16, 256>, 1, 2>(p, grid, st);
+  }
+  return hipErrorNotSupported;
+}
+
+}  // namespace trinix

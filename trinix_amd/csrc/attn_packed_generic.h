@@ -1,0 +1,344 @@
+// Packed-sequence attention on the operand policies of attn_ops.h (fp32 on fp32
+// matrix products, 16-bit types with their coefficients in two terms):
+//   packed_fwd_generic    128 query rows of one sequence and head, 32 per wavefront,
+//                         over 32-key tiles: S^T = K Q^T, online softmax, O^T += V^T P^T;
+//   packed_dkdv_generic   128 keys of one sequence and KV head, 32 per wavefront, over
+//                         32-row tiles of Q and dO of every head of the group:
+//                         dV += P^T dO, dZ = P (dO V^T - delta), dK += dZ^T Q;
+//   packed_dq_generic     128 query rows as in the forward: dQ += dZ K.
+// Tiles go global -> LDS asynchronously into two slots, one barrier per tile.
+#pragma once
+#include <cfloat>
+
+#include "attn_ops.h"
+#include "attn_packed.h"
+
+namespace trinix {
+
+template <class O, class E, int OCC>
+__global__ __launch_bounds__(256, OCC) void packed_fwd_generic(const PackedParams p) {
+  using Store = typename O::Store;
+  constexpr int NW = 4, BM = NW * 32, D = O::kD, DB = D / 32, TILE = kTileRows * D * (int)sizeof(Store);
+  __shared__ __attribute__((aligned(1024))) char lds_k[2][TILE];
+  __shared__ __attribute__((aligned(1024))) char lds_v[2][TILE];
+  const PackedBlock w(p, (int)blockIdx.x, p.Hkv, p.G);
+  if (w.blk < 0) return;
+  const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int hq = w.h, hkv = hq / p.G, m0 = w.blk * BM, iw0 = m0 + wave * 32, i = iw0 + r, ic = min(i, w.lq - 1);
+  const bool wide = p.rows16 != 0;
+
+  const O ops(lane, 0);
+  const typename O::Frag qf = O::load_frag((const Store*)p.q + (int64_t)(w.q0 + ic) * p.q_ss + hq * p.q_sh, g);
+  const float slope_l2 = p.alibi ? -p.alibi[hq * p.al_sh] * kLog2e : 0.f;
+  const int off = w.lk - w.lq;
+  f32x16_t acc[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db) acc[db] = (f32x16_t){};
+  float m_run = -INFINITY, l_run = 0.f;
+
+  int t_lo, t_hi;
+  bwd_key_tiles(m0, BM, w.lq, w.lk, w.dlo, w.dhi, kTileRows, t_lo, t_hi);
+  const Store* kbase = (const Store*)p.k + (int64_t)w.k0 * p.k_ss + hkv * p.k_sh;
+  const Store* vbase = (const Store*)p.v + (int64_t)w.k0 * p.v_ss + hkv * p.v_sh;
+  const TileCopy<O, NW> copy_k(p.k_ss, wave, lane), copy_v(p.v_ss, wave, lane);
+  auto load = [&](int t, int slot) __attribute__((always_inline)) {
+    copy_k(kbase, t * kTileRows, w.lk, lds_k[slot], wide);
+    copy_v(vbase, t * kTileRows, w.lk, lds_v[slot], wide);
+  };
+  auto block = [&](int t, int slot) __attribute__((always_inline)) {
+    const int n0 = t * kTileRows;
+    if (!w.live(iw0, 32, n0, 32)) return;
+    const f32x16_t s = ops.scores(lds_k[slot], qf);
+    float x[16];
+#pragma unroll
+    for (int v = 0; v < 16; ++v) x[v] = s[v] * p.scale_log2;
+    if (p.alibi) {
+      const float fi = (float)(i + off - n0 - 4 * g);
+#pragma unroll
+      for (int v = 0; v < 16; ++v) x[v] = __builtin_fmaf(fabsf(fi - (float)((v >> 2) * 8 + (v & 3))), slope_l2, x[v]);
+    }
+    if (!w.full(iw0, 32, n0, 32)) {
+      const Span ks = w.keys_of(i);
+#pragma unroll
+      for (int v = 0; v < 16; ++v) x[v] = ks.ok(n0 + (v >> 2) * 8 + g * 4 + (v & 3)) ? x[v] : -INFINITY;
+    }
+    float mx = x[0];
+#pragma unroll
+    for (int v = 1; v < 16; ++v) mx = fmaxf(mx, x[v]);
+    mx = xlane_max(mx);
+    if (wave_any(mx > m_run)) {
+      const float m_new = fmaxf(m_run, mx);
+      const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
+      l_run *= alpha;
+#pragma unroll
+      for (int db = 0; db < DB; ++db) acc[db] *= alpha;
+      m_run = m_new;
+    }
+    // all keys so far hidden: exp2(-inf - 0) = 0.  P and l are held at
+    // 2^kPShift (attn_ops.h), which cancels in P / l
+    const float m_use = (m_run == -INFINITY ? 0.f : m_run) - O::kPShift;
+    float sum = 0.f;  // within the tile first: one rounding of the running sum per tile
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+      x[v] = __builtin_amdgcn_exp2f(x[v] - m_use);
+      sum += x[v];
+    }
+    l_run += sum;
+    ops.accum(acc, lds_v[slot], x);
+  };
+
+  if (t_lo < t_hi) load(t_lo, 0);
+  auto step = [&](auto slot_c, int t) __attribute__((always_inline)) {
+    constexpr int SL = decltype(slot_c)::value;
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (t + 1 < t_hi) load(t + 1, 1 - SL);
+    block(t, SL);
+  };
+  for (int t = t_lo; t < t_hi; t += 2) {
+    step(std::integral_constant<int, 0>{}, t);
+    if (t + 1 < t_hi) step(std::integral_constant<int, 1>{}, t + 1);
+  }
+
+  const float l = xlane_sum(l_run);
+  if (i >= w.lq) return;
+  const float inv = l > 0.f ? 1.f / l : 0.f;  // a row that sees no key: 0
+  const int64_t row = w.q0 + i;
+  Store* orow = (Store*)p.o + row * p.o_ss + hq * p.o_sh;
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int vq = 0; vq < 4; ++vq) {
+      const int d0 = db * 32 + vq * 8 + g * 4;
+      float x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = acc[db][vq * 4 + e] * inv;
+      O::store4(orow, d0, x[0], x[1], x[2], x[3]);
+      if constexpr (sizeof(Store) == 2) {
+        if (p.o_lo) {
+          constexpr float f = kLoScale<E>;
+          O::store4((Store*)p.o_lo + row * p.o_ss + hq * p.o_sh, d0, (x[0] - round_to<E>(x[0])) * f,
+                    (x[1] - round_to<E>(x[1])) * f, (x[2] - round_to<E>(x[2])) * f, (x[3] - round_to<E>(x[3])) * f);
+        }
+      }
+    }
+  if (p.lse && g == 0)
+    p.lse[(int64_t)hq * p.Tq + row] = l > 0.f ? (m_run - O::kPShift + log2f(l)) * kLn2 : -INFINITY;
+}
+
+template <class O, int OCC, int HS>
+__global__ __launch_bounds__(256, OCC) void packed_dkdv_generic(const PackedParams p) {
+  using Store = typename O::Store;
+  constexpr int NW = 4, BK = NW * 32, D = O::kD, DB = O::DB / HS, TILE = kTileRows * D * (int)sizeof(Store);
+  __shared__ __attribute__((aligned(1024))) char lds_q[2][TILE];
+  __shared__ __attribute__((aligned(1024))) char lds_o[2][TILE];
+  __shared__ __attribute__((aligned(128))) float lds_l[2][kTileRows];
+  __shared__ __attribute__((aligned(128))) float lds_d[2][kTileRows];
+  // HS workgroups share a key block, each summing D / HS of the columns
+  const PackedBlock w(p, (int)blockIdx.x / HS, p.Hkv, 1);
+  if (w.blk < 0) return;
+  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int hkv = w.h, kb0 = w.blk * BK, db0 = ((int)blockIdx.x % HS) * DB;
+  const int j0 = kb0 + wave * 32, j = j0 + (lane & 31), jc = min(j, w.lk - 1);
+  const bool wide = p.rows16 != 0;
+  const int off = w.lk - w.lq;
+
+  int qt_lo, qt_hi;
+  bwd_query_tiles(kb0, BK, w.lq, w.lk, w.dlo, w.dhi, kTileRows, qt_lo, qt_hi);
+  const int nqt = qt_hi - qt_lo;
+  const int n_items = nqt > 0 ? p.G * nqt : 0;  // item = (q-head of the group, query tile)
+
+  const O ops(lane, db0);
+  const typename O::Frag kf = O::load_frag((const Store*)p.k + (int64_t)(w.k0 + jc) * p.k_ss + hkv * p.k_sh, g);
+  const typename O::Frag vf = O::load_frag((const Store*)p.v + (int64_t)(w.k0 + jc) * p.v_ss + hkv * p.v_sh, g);
+  f32x16_t dk[DB], dv[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db) dk[db] = dv[db] = (f32x16_t){};
+  ZScale<O> zs;
+
+  const TileCopy<O, NW> copy_q(p.q_ss, wave, lane), copy_o(p.do_ss, wave, lane);
+  float lse_next = 0.f, del_next = 0.f;
+  auto load_item = [&](int it, int slot) __attribute__((always_inline)) {
+    const int hq = hkv * p.G + it / nqt, i0 = (qt_lo + it % nqt) * kTileRows;
+    copy_q((const Store*)p.q + (int64_t)w.q0 * p.q_ss + hq * p.q_sh, i0, w.lq, lds_q[slot], wide);
+    copy_o((const Store*)p.dout + (int64_t)w.q0 * p.do_ss + hq * p.do_sh, i0, w.lq, lds_o[slot], wide);
+    if (tid < kTileRows) {
+      const int64_t ro = (int64_t)hq * p.Tq + w.q0 + min(i0 + tid, w.lq - 1);
+      lse_next = p.lse[ro];
+      del_next = p.delta[ro];
+    }
+  };
+  // a row that sees no key has lse -inf and every score -inf: the finite floor
+  // keeps exp2(score - lse) at 0 instead of exp2(-inf + inf) = NaN
+  auto write_rows = [&](int slot) __attribute__((always_inline)) {
+    if (tid < kTileRows) {
+      lds_l[slot][tid] = fmaxf(lse_next * kLog2e, -0.5f * FLT_MAX) - O::kPShift;
+      lds_d[slot][tid] = del_next;
+    }
+  };
+  auto block = [&](int it, int slot) __attribute__((always_inline)) {
+    const int hq = hkv * p.G + it / nqt, i0 = (qt_lo + it % nqt) * kTileRows;
+    if (!w.live(i0, 32, j0, 32)) return;
+    const f32x16_t s = ops.scores(lds_q[slot], kf);
+    float x[16];
+#pragma unroll
+    for (int vq = 0; vq < 4; ++vq) {
+      const f32x4_t l4 = *(const f32x4_t*)(&lds_l[slot][vq * 8 + g * 4]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[vq * 4 + e] = __builtin_fmaf(s[vq * 4 + e], p.scale_log2, -l4[e]);
+    }
+    if (p.alibi) {
+      const float slope_l2 = -p.alibi[hq * p.al_sh] * kLog2e;
+      const float fj = (float)(j - off - (i0 + g * 4));
+#pragma unroll
+      for (int v = 0; v < 16; ++v) x[v] = __builtin_fmaf(fabsf(fj - (float)((v >> 2) * 8 + (v & 3))), slope_l2, x[v]);
+    }
+    if (!w.full(i0, 32, j0, 32)) {
+      int jo = j;  // (not held across the loop)
+      asm volatile("" : "+v"(jo));
+      const Span qs = w.rows_of(jo);
+#pragma unroll
+      for (int v = 0; v < 16; ++v) x[v] = qs.ok(i0 + (v >> 2) * 8 + g * 4 + (v & 3)) ? x[v] : -INFINITY;
+    }
+#pragma unroll
+    for (int v = 0; v < 16; ++v) x[v] = __builtin_amdgcn_exp2f(x[v]);
+    ops.accum(dv, lds_o[slot], x);
+    const f32x16_t dp = ops.scores(lds_o[slot], vf);
+#pragma unroll
+    for (int vq = 0; vq < 4; ++vq) {
+      const f32x4_t d4 = *(const f32x4_t*)(&lds_d[slot][vq * 8 + g * 4]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[vq * 4 + e] *= dp[vq * 4 + e] - d4[e];
+    }
+    zs.apply(x, dk);
+    ops.accum(dk, lds_q[slot], x);
+  };
+
+  if (n_items > 0) {
+    load_item(0, 0);
+    write_rows(0);
+  }
+  auto step = [&](auto slot_c, int it) __attribute__((always_inline)) {
+    constexpr int SL = decltype(slot_c)::value;
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (it + 1 < n_items) load_item(it + 1, 1 - SL);
+    block(it, SL);
+    if (it + 1 < n_items) write_rows(1 - SL);
+  };
+  for (int it = 0; it < n_items; it += 2) {
+    step(std::integral_constant<int, 0>{}, it);
+    if (it + 1 < n_items) step(std::integral_constant<int, 1>{}, it + 1);
+  }
+
+  if (j >= w.lk) return;
+  const float fv = exp2f(-O::kPShift), fk = p.scale * fv * zs.undo();
+  Store* krow = (Store*)p.dk + (int64_t)(w.k0 + j) * p.dk_ss + hkv * p.dk_sh;
+  Store* vrow = (Store*)p.dv + (int64_t)(w.k0 + j) * p.dv_ss + hkv * p.dv_sh;
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int vq = 0; vq < 4; ++vq) {
+      const int d0 = (db0 + db) * 32 + vq * 8 + g * 4;
+      O::store4(vrow, d0, dv[db][vq * 4] * fv, dv[db][vq * 4 + 1] * fv, dv[db][vq * 4 + 2] * fv, dv[db][vq * 4 + 3] * fv);
+      O::store4(krow, d0, dk[db][vq * 4] * fk, dk[db][vq * 4 + 1] * fk, dk[db][vq * 4 + 2] * fk, dk[db][vq * 4 + 3] * fk);
+    }
+}
+
+template <class O, int OCC, int HS>
+__global__ __launch_bounds__(256, OCC) void packed_dq_generic(const PackedParams p) {
+  using Store = typename O::Store;
+  constexpr int NW = 4, BM = NW * 32, D = O::kD, DB = O::DB / HS, TILE = kTileRows * D * (int)sizeof(Store);
+  __shared__ __attribute__((aligned(1024))) char lds_k[2][TILE];
+  __shared__ __attribute__((aligned(1024))) char lds_v[2][TILE];
+  const PackedBlock w(p, (int)blockIdx.x / HS, p.Hkv, p.G);
+  if (w.blk < 0) return;
+  const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int hq = w.h, hkv = hq / p.G, m0 = w.blk * BM, iw0 = m0 + wave * 32, i = iw0 + r, ic = min(i, w.lq - 1);
+  const int db0 = ((int)blockIdx.x % HS) * DB, off = w.lk - w.lq;
+  const bool wide = p.rows16 != 0;
+
+  const O ops(lane, db0);
+  const typename O::Frag qf = O::load_frag((const Store*)p.q + (int64_t)(w.q0 + ic) * p.q_ss + hq * p.q_sh, g);
+  const typename O::Frag of = O::load_frag((const Store*)p.dout + (int64_t)(w.q0 + ic) * p.do_ss + hq * p.do_sh, g);
+  const int64_t ro = (int64_t)hq * p.Tq + w.q0 + ic;
+  const float lse2 = fmaxf(p.lse[ro] * kLog2e, -0.5f * FLT_MAX), dlt = p.delta[ro];  // (finite: see above)
+  const float slope_l2 = p.alibi ? -p.alibi[hq * p.al_sh] * kLog2e : 0.f;
+  f32x16_t acc[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db) acc[db] = (f32x16_t){};
+  ZScale<O> zs;
+
+  int t_lo, t_hi;
+  bwd_key_tiles(m0, BM, w.lq, w.lk, w.dlo, w.dhi, kTileRows, t_lo, t_hi);
+  const Store* kbase = (const Store*)p.k + (int64_t)w.k0 * p.k_ss + hkv * p.k_sh;
+  const Store* vbase = (const Store*)p.v + (int64_t)w.k0 * p.v_ss + hkv * p.v_sh;
+  const TileCopy<O, NW> copy_k(p.k_ss, wave, lane), copy_v(p.v_ss, wave, lane);
+  auto load = [&](int t, int slot) __attribute__((always_inline)) {
+    copy_k(kbase, t * kTileRows, w.lk, lds_k[slot], wide);
+    copy_v(vbase, t * kTileRows, w.lk, lds_v[slot], wide);
+  };
+  auto block = [&](int t, int slot) __attribute__((always_inline)) {
+    const int n0 = t * kTileRows;
+    if (!w.live(iw0, 32, n0, 32)) return;
+    const f32x16_t s = ops.scores(lds_k[slot], qf);
+    const f32x16_t dp = ops.scores(lds_v[slot], of);
+    float x[16];
+#pragma unroll
+    for (int v = 0; v < 16; ++v) x[v] = __builtin_fmaf(s[v], p.scale_log2, -lse2);
+    if (p.alibi) {
+      const float fi = (float)(i + off - n0 - 4 * g);
+#pragma unroll
+      for (int v = 0; v < 16; ++v) x[v] = __builtin_fmaf(fabsf(fi - (float)((v >> 2) * 8 + (v & 3))), slope_l2, x[v]);
+    }
+    if (!w.full(iw0, 32, n0, 32)) {
+      int io = i;
+      asm volatile("" : "+v"(io));
+      const Span ks = w.keys_of(io);
+#pragma unroll
+      for (int v = 0; v < 16; ++v) x[v] = ks.ok(n0 + (v >> 2) * 8 + g * 4 + (v & 3)) ? x[v] : -INFINITY;
+    }
+#pragma unroll
+    for (int v = 0; v < 16; ++v) x[v] = __builtin_amdgcn_exp2f(x[v]) * (dp[v] - dlt);
+    zs.apply(x, acc);
+    ops.accum(acc, lds_k[slot], x);
+  };
+
+  if (t_lo < t_hi) load(t_lo, 0);
+  auto step = [&](auto slot_c, int t) __attribute__((always_inline)) {
+    constexpr int SL = decltype(slot_c)::value;
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (t + 1 < t_hi) load(t + 1, 1 - SL);
+    block(t, SL);
+  };
+  for (int t = t_lo; t < t_hi; t += 2) {
+    step(std::integral_constant<int, 0>{}, t);
+    if (t + 1 < t_hi) step(std::integral_constant<int, 1>{}, t + 1);
+  }
+
+  if (i >= w.lq) return;
+  const float f = p.scale * zs.undo();
+  Store* row = (Store*)p.dq + (int64_t)(w.q0 + i) * p.dq_ss + hq * p.dq_sh;
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int vq = 0; vq < 4; ++vq) {
+      const int d0 = (db0 + db) * 32 + vq * 8 + g * 4;
+      O::store4(row, d0, acc[db][vq * 4] * f, acc[db][vq * 4 + 1] * f, acc[db][vq * 4 + 2] * f, acc[db][vq * 4 + 3] * f);
+    }
+}
+
+template <class O, int OCC, int HS>
+hipError_t launch_packed_dkdv_g(const PackedParams& p, int grid, hipStream_t st) {
+  return launch_kernel(&packed_dkdv_generic<O, OCC, HS>, dim3((unsigned)(grid * HS)), dim3(256), 0, st, p);
+}
+template <class O, int OCC, int HS>
+hipError_t launch_packed_dq_g(const PackedParams& p, int grid, hipStream_t st) {
+  return launch_kernel(&packed_dq_generic<O, OCC, HS>, dim3((unsigned)(grid * HS)), dim3(256), 0, st, p);
+}
+
+}  // namespace trinix

@@ -4,6 +4,8 @@ from .attention import (
     FastMultiHeadAttention,
     FastMultiHeadSelfAttention,
     FastMultiQueryAttention,
+    PackedSequences,
+    packed_attn_func,
     triton_attn_func,
 )
 from .embeddings import FastALiBiPositionEmbedding, FastRoPEPositionEmbedding

@@ -1,5 +1,5 @@
 from .base import FastBaseAttention
-from .functional import triton_attn_func
+from .functional import PackedSequences, packed_attn_func, triton_attn_func
 from .grouped_query_attention import FastGroupedQueryAttention
 from .multi_query_attention import FastMultiQueryAttention
 from .multihead_attention import FastMultiHeadAttention
@@ -11,5 +11,7 @@ __all__ = [
     "FastMultiHeadAttention",
     "FastMultiHeadSelfAttention",
     "FastMultiQueryAttention",
+    "PackedSequences",
+    "packed_attn_func",
     "triton_attn_func",
 ]

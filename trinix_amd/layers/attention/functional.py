@@ -7,6 +7,7 @@ from typing import Optional, Tuple
 import torch
 
 from ...kernels.attention_kernel import TritonAttentionKernel, attention
+from ...kernels.packed_attention import PackedSequences, packed_attention
 
 
 def triton_attn_func(
@@ -95,3 +96,48 @@ def triton_attn_func(
         rotary_sin=rotary_sin,
         return_lse=return_lse,
     )
+
+
+def packed_attn_func(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    sequences: PackedSequences,
+    softmax_scale: Optional[float] = None,
+    causal: bool = False,
+    window_size: Optional[Tuple[int, int]] = None,
+    alibi_slopes: Optional[torch.Tensor] = None,
+    *,
+    return_lse: bool = False,
+):
+    """Attention over sequences of different lengths packed without padding.
+
+    Args:
+        q: (total_q, num_heads, head_dim) GPU tensor (fp32/fp16/bf16); head_dim
+            up to 256.
+        k, v: (total_k, num_kv_heads, head_dim); ``num_kv_heads`` divides
+            ``num_heads``.
+        sequences: ``PackedSequences`` with the boundaries of the rows of q, k
+            and v; no row sees another sequence.
+        softmax_scale: defaults to ``head_dim ** -0.5``.
+        causal: with Lq queries and Lk keys in a sequence, query i sees keys
+            j <= i + Lk - Lq: the queries are the sequence's last positions, so
+            a chunk of a prompt attends to its cache and to itself.
+        window_size: (left, right): keys with
+            -left <= j - (i + Lk - Lq) <= right.
+        alibi_slopes: (H,) or (1, H); adds ``-slope * |i + Lk - Lq - j|``.
+        return_lse: also return the fp32 (num_heads, total_q) log-sum-exp.
+
+    Returns:
+        (total_q, num_heads, head_dim) tensor of q.dtype, differentiable in q, k
+        and v.  A row that sees no key (a sequence without keys, a query before
+        the first key, padding behind the last sequence) gives 0 and a
+        log-sum-exp of -inf, where ``triton_attn_func`` gives NaN: packed
+        batches hold such rows by design.
+
+    Raises:
+        ValueError: non-GPU tensors, inconsistent shapes, types or devices.
+        RuntimeError: the HIP kernel library or a gfx950 GPU is unavailable, or
+            the sequences were rebuilt between a forward and its backward.
+    """
+    return packed_attention(q, k, v, sequences, softmax_scale, causal, window_size, alibi_slopes, return_lse)
