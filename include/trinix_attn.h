@@ -519,6 +519,45 @@ typedef struct trinix_packed_args {
 int trinix_packed_fwd(const trinix_packed_args* args, void* stream);
 int trinix_packed_bwd(const trinix_packed_args* args, void* stream);
 
+/* ---- attention of a batch behind one shared prefix (ABI version 7) -----------
+ * No counterpart in the reference.  Every request b of a batch has seqlen_q
+ * query rows, sees all of the prefix's keys, and keys of its own in a cache of
+ * `capacity` rows, of which the first len = seq_lens[b] are valid (the queries
+ * are the last seqlen_q of them):
+ *   keys of query i: prefix 0 .. prefix_len - 1 and own j <= len - seqlen_q + i
+ *   out = softmax(scale * q k^T) @ v over both;  lse = the log-sum-exp
+ * The prefix is read for all requests together.  seq_lens (device memory, read
+ * when the kernels run; clamped into [0, capacity]) may be NULL: len = capacity.
+ * Cache rows at and behind len are not read.  A row without any key has out 0
+ * and lse -inf.  prefix_len or capacity may be 0 (their pointers then are not
+ * read).  head_dim 64, 128 or 256; 16-bit rows 16-byte aligned, fp32 rows too.
+ *
+ * trinix_shared_prefix_workspace: bytes of fp32 workspace that a call takes
+ * (host only).  trinix_shared_prefix_fwd: the forward on `stream`; workspace
+ * 16-byte aligned, of at least that size.  No atomics. */
+typedef struct trinix_shared_prefix_args {
+  const void* q;         /* (B, Sq, Hq, D)      */
+  const void* prefix_k;  /* (prefix_len, Hkv, D) */
+  const void* prefix_v;
+  const void* k;         /* (B, capacity, Hkv, D) */
+  const void* v;
+  void* out;             /* (B, Sq, Hq, D)      */
+  float* lse;            /* (B, Hq, Sq) contiguous, or NULL */
+  const int32_t* seq_lens; /* (B), or NULL */
+  int64_t q_stride[4];   /* b, s, h, d (1) */
+  int64_t prefix_k_stride[3]; /* s, h, d (1) */
+  int64_t prefix_v_stride[3];
+  int64_t k_stride[4];
+  int64_t v_stride[4];
+  int64_t out_stride[4];
+  int64_t batch, seqlen_q, prefix_len, capacity, nheads_q, nheads_kv, head_dim;
+  int32_t dtype;
+  float softmax_scale;
+} trinix_shared_prefix_args;
+int trinix_shared_prefix_workspace(const trinix_shared_prefix_args* args, int64_t* bytes);
+int trinix_shared_prefix_fwd(const trinix_shared_prefix_args* args, void* workspace,
+                             int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

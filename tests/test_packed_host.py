@@ -36,6 +36,63 @@ def test_packed_args_layout(tmp_path):
     layout("trinix_packed_args", nat.PackedArgs, tmp_path)
 
 
+def test_shared_prefix_args_layout(tmp_path):
+    layout("trinix_shared_prefix_args", nat.SharedPrefixArgs, tmp_path)
+
+
+def shared_args(**kw):
+    a = nat.SharedPrefixArgs()
+    for f in ("q", "prefix_k", "prefix_v", "k", "v", "out"):
+        setattr(a, f, 4096)
+    a.q_stride = a.out_stride = nat.Int64x4(8 * 128, 8 * 128, 128, 1)
+    a.k_stride = a.v_stride = nat.Int64x4(500 * 256, 256, 128, 1)
+    a.prefix_k_stride = a.prefix_v_stride = nat.Int64x3(256, 128, 1)
+    a.batch, a.seqlen_q, a.prefix_len, a.capacity, a.nheads_q, a.nheads_kv, a.head_dim = 4, 1, 1000, 500, 8, 2, 128
+    a.dtype, a.softmax_scale = nat.TRINIX_BF16, 0.1
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(dtype=nat.TRINIX_U8), nat.TRINIX_ERR_BAD_DTYPE),
+    (dict(head_dim=80), nat.TRINIX_ERR_BAD_HEAD_DIM),
+    (dict(batch=0), nat.TRINIX_ERR_BAD_SHAPE),
+    (dict(seqlen_q=0), nat.TRINIX_ERR_BAD_SHAPE),
+    (dict(prefix_len=-1), nat.TRINIX_ERR_BAD_SHAPE),
+    (dict(capacity=1 << 30), nat.TRINIX_ERR_BAD_SHAPE),
+    (dict(nheads_kv=3), nat.TRINIX_ERR_BAD_SHAPE),
+    (dict(batch=1 << 23, seqlen_q=1 << 23), nat.TRINIX_ERR_BAD_SHAPE),
+    (dict(q=None), nat.TRINIX_ERR_NULL_POINTER),
+    (dict(prefix_v=None), nat.TRINIX_ERR_NULL_POINTER),
+    (dict(k=None), nat.TRINIX_ERR_NULL_POINTER),
+    (dict(out=4104), nat.TRINIX_ERR_BAD_STRIDE),
+    (dict(k_stride=nat.Int64x4(500 * 256, 256, 132, 1)), nat.TRINIX_ERR_BAD_STRIDE),
+    (dict(prefix_k_stride=nat.Int64x3(256, 128, 2)), nat.TRINIX_ERR_BAD_STRIDE),
+    (dict(seq_lens=4098), nat.TRINIX_ERR_BAD_STRIDE),
+    (dict(lse=4098), nat.TRINIX_ERR_BAD_STRIDE),
+])
+def test_shared_prefix_status_codes(lib, kw, code):
+    a, n = shared_args(**kw), ctypes.c_int64(0)
+    assert lib.trinix_shared_prefix_workspace(ctypes.byref(a), ctypes.byref(n)) == code
+    assert lib.trinix_shared_prefix_fwd(ctypes.byref(a), 4096, 1 << 40, None) == code
+
+
+def test_shared_prefix_workspace(lib):
+    n = ctypes.c_int64(0)
+    a = shared_args()
+    assert lib.trinix_shared_prefix_workspace(ctypes.byref(a), ctypes.byref(n)) == 0 and n.value > 0
+    for ws, size in ((None, n.value), (4096, n.value - 1), (4100, n.value)):
+        assert lib.trinix_shared_prefix_fwd(ctypes.byref(a), ws, size, None) == nat.TRINIX_ERR_BAD_ARGUMENT
+    assert lib.trinix_shared_prefix_workspace(None, ctypes.byref(n)) == nat.TRINIX_ERR_NULL_POINTER
+    assert lib.trinix_shared_prefix_workspace(ctypes.byref(a), None) == nat.TRINIX_ERR_NULL_POINTER
+    assert lib.trinix_shared_prefix_fwd(None, None, 0, None) == nat.TRINIX_ERR_NULL_POINTER
+    # absent prefix or caches: their pointers are not looked at
+    for kw in (dict(prefix_len=0, prefix_k=None, prefix_v=None), dict(capacity=0, k=None, v=None)):
+        a = shared_args(**kw)
+        assert lib.trinix_shared_prefix_workspace(ctypes.byref(a), ctypes.byref(n)) == 0
+
+
 def plan_bytes(lib, n, tq, tk):
     out = ctypes.c_int64(0)
     return lib.trinix_packed_plan_bytes(n, tq, tk, ctypes.byref(out)), out.value

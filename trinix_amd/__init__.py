@@ -14,6 +14,7 @@ from .layers.attention import (
     FastMultiQueryAttention,
     PackedSequences,
     packed_attn_func,
+    shared_prefix_attn_func,
     triton_attn_func,
 )
 from .layers.embeddings import FastALiBiPositionEmbedding, FastRoPEPositionEmbedding
@@ -26,6 +27,7 @@ __all__ = [
     "triton_attn_func",
     "PackedSequences",
     "packed_attn_func",
+    "shared_prefix_attn_func",
     "FastBaseAttention",
     "FastGroupedQueryAttention",
     "FastMultiHeadAttention",

@@ -184,6 +184,36 @@ class PackedArgs(ctypes.Structure):
     ]
 
 
+class SharedPrefixArgs(ctypes.Structure):
+    """Mirror of ``trinix_shared_prefix_args`` (field order and types identical)."""
+
+    _fields_ = [
+        ("q", c_void_p),
+        ("prefix_k", c_void_p),
+        ("prefix_v", c_void_p),
+        ("k", c_void_p),
+        ("v", c_void_p),
+        ("out", c_void_p),
+        ("lse", c_void_p),
+        ("seq_lens", c_void_p),
+        ("q_stride", Int64x4),
+        ("prefix_k_stride", Int64x3),
+        ("prefix_v_stride", Int64x3),
+        ("k_stride", Int64x4),
+        ("v_stride", Int64x4),
+        ("out_stride", Int64x4),
+        ("batch", c_int64),
+        ("seqlen_q", c_int64),
+        ("prefix_len", c_int64),
+        ("capacity", c_int64),
+        ("nheads_q", c_int64),
+        ("nheads_kv", c_int64),
+        ("head_dim", c_int64),
+        ("dtype", c_int32),
+        ("softmax_scale", c_float),
+    ]
+
+
 class TileCfg(ctypes.Structure):
     """Mirror of ``trinix_tile_cfg``."""
 
@@ -239,6 +269,8 @@ SIGNATURES = {
     "trinix_packed_plan": (c_int32, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p]),
     "trinix_packed_fwd": (c_int32, [POINTER(PackedArgs), c_void_p]),
     "trinix_packed_bwd": (c_int32, [POINTER(PackedArgs), c_void_p]),
+    "trinix_shared_prefix_workspace": (c_int32, [POINTER(SharedPrefixArgs), POINTER(c_int64)]),
+    "trinix_shared_prefix_fwd": (c_int32, [POINTER(SharedPrefixArgs), c_void_p, c_int64, c_void_p]),
     "trinix_attn_tile_config": (c_int32, [c_int64, c_int32, POINTER(TileCfg)]),
     "trinix_dropout_state_advance": (c_int32, [c_void_p, c_void_p, c_uint64, c_void_p]),
     "trinix_dropout_keep_map_bytes": (c_int32, [c_int64, c_int64, c_int64, c_int64, c_void_p]),

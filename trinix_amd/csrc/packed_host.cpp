@@ -62,9 +62,79 @@ int validate_packed(const trinix_packed_args* a, bool backward) {
   return TRINIX_OK;
 }
 
+namespace {
+
+// (batch, rows, heads, head_dim) or, without a batch, (rows, heads, head_dim):
+// head_dim stride 1, rows on 16 bytes.
+int check_vec(const void* ptr, const int64_t* st, int dims, int esize) {
+  if (!ptr) return TRINIX_ERR_NULL_POINTER;
+  if (st[dims - 1] != 1 || ((uintptr_t)ptr & 15) != 0) return TRINIX_ERR_BAD_STRIDE;
+  for (int d = 0; d < dims - 1; ++d)
+    if (st[d] * esize % 16 != 0) return TRINIX_ERR_BAD_STRIDE;
+  return TRINIX_OK;
+}
+
+}  // namespace
+
+int validate_shared(const trinix_shared_prefix_args* a) {
+  if (!a) return TRINIX_ERR_NULL_POINTER;
+  if (a->dtype != TRINIX_F32 && a->dtype != TRINIX_F16 && a->dtype != TRINIX_BF16) return TRINIX_ERR_BAD_DTYPE;
+  if (a->head_dim != 64 && a->head_dim != 128 && a->head_dim != 256) return TRINIX_ERR_BAD_HEAD_DIM;
+  constexpr int64_t kMax = 1ll << 30;
+  if (a->batch <= 0 || a->seqlen_q <= 0 || a->prefix_len < 0 || a->capacity < 0 || a->nheads_q <= 0 || a->nheads_kv <= 0 ||
+      a->batch >= (1ll << 24) || a->seqlen_q >= (1ll << 24) || a->prefix_len >= kMax || a->capacity >= kMax ||
+      a->nheads_q > (1 << 20) || a->nheads_q % a->nheads_kv != 0)
+    return TRINIX_ERR_BAD_SHAPE;
+  if (a->batch * a->seqlen_q > kMax / a->nheads_q) return TRINIX_ERR_BAD_SHAPE;
+  const int esz = a->dtype == TRINIX_F32 ? 4 : 2;
+  int rc = check_vec(a->q, a->q_stride, 4, esz);
+  if (rc == TRINIX_OK) rc = check_vec(a->out, a->out_stride, 4, esz);
+  if (rc == TRINIX_OK && a->prefix_len > 0) rc = check_vec(a->prefix_k, a->prefix_k_stride, 3, esz);
+  if (rc == TRINIX_OK && a->prefix_len > 0) rc = check_vec(a->prefix_v, a->prefix_v_stride, 3, esz);
+  if (rc == TRINIX_OK && a->capacity > 0) rc = check_vec(a->k, a->k_stride, 4, esz);
+  if (rc == TRINIX_OK && a->capacity > 0) rc = check_vec(a->v, a->v_stride, 4, esz);
+  if (rc != TRINIX_OK) return rc;
+  if (((uintptr_t)a->lse & 3) != 0 || ((uintptr_t)a->seq_lens & 3) != 0) return TRINIX_ERR_BAD_STRIDE;
+  return TRINIX_OK;
+}
+
+int plan_shared(const trinix_shared_prefix_args* a, SharedPlan* pl) {
+  const int64_t G = a->nheads_q / a->nheads_kv, own_rows = a->seqlen_q * G, rows = a->batch * own_rows;
+  const int64_t rgp = (rows + 15) / 16, rgs = (own_rows + 15) / 16;
+  // chunks of at least 128 keys, as many as give about kDecodeTargetWgs workgroups
+  const auto split = [](int64_t keys, int64_t groups, int* n, int* chunk) {
+    const int64_t want = lmax(1, kDecodeTargetWgs / groups), per = (keys + want - 1) / want;
+    const int64_t c = lmax(kDecodeMinChunk, (per + 63) / 64 * 64);
+    *n = (int)((keys + c - 1) / c);
+    *chunk = (int)c;
+  };
+  split(a->prefix_len, rgp * a->nheads_kv, &pl->n_p, &pl->chunk_p);
+  split(a->capacity, a->batch * rgs * a->nheads_kv, &pl->n_s, &pl->chunk_s);
+  const int64_t wg_p = rgp * a->nheads_kv * pl->n_p;
+  if (a->batch * rgs * a->nheads_kv >= INT32_MAX / lmax(1, pl->n_s)) return TRINIX_ERR_BAD_SHAPE;
+  const int64_t wg_s = a->batch * rgs * a->nheads_kv * pl->n_s;
+  if (wg_p + wg_s > INT32_MAX) return TRINIX_ERR_BAD_SHAPE;
+  pl->rows = (int)rows;
+  pl->rgp = (int)rgp;
+  pl->rgs = (int)rgs;
+  pl->wg_p = wg_p;
+  pl->wg_s = wg_s;
+  pl->ws_bytes = a->nheads_kv * rows * (pl->n_p + pl->n_s) * (a->head_dim + 1) * 4;
+  return TRINIX_OK;
+}
+
 }  // namespace trinix
 
 using namespace trinix;
+
+extern "C" int trinix_shared_prefix_workspace(const trinix_shared_prefix_args* a, int64_t* bytes) {
+  if (!bytes) return TRINIX_ERR_NULL_POINTER;
+  int rc = validate_shared(a);
+  SharedPlan pl;
+  if (rc == TRINIX_OK) rc = plan_shared(a, &pl);
+  if (rc == TRINIX_OK) *bytes = pl.ws_bytes;
+  return rc;
+}
 
 extern "C" int trinix_packed_plan_bytes(int64_t n_seqs, int64_t total_q, int64_t total_k, int64_t* bytes) {
   if (!bytes) return TRINIX_ERR_NULL_POINTER;

@@ -10,4 +10,22 @@ namespace trinix {
 // pointers and strides too.
 int validate_packed(const trinix_packed_args* a, bool backward);
 
+
+// Attention behind a shared prefix: the same checks, and the launch plan.
+int validate_shared(const trinix_shared_prefix_args* a);
+// A row is a (request, query, head of the KV group): row r = (b * Sq + i) * G + g
+// of a KV head.  Partial results (fp32, per row and chunk of keys) of n_p prefix
+// chunks and n_s chunks of the own keys are merged by a second kernel.
+struct SharedPlan {
+  int rows;            // rows per KV head
+  int rgp, rgs;        // 16-row groups: of all rows (prefix), of one request (own keys)
+  int n_p, chunk_p;    // chunks of the prefix, keys per chunk
+  int n_s, chunk_s;    // the same for the own keys (at the cache's capacity)
+  int64_t wg_p, wg_s;  // workgroups
+  int64_t ws_bytes;
+};
+// TRINIX_OK, or TRINIX_ERR_BAD_SHAPE where the grid or the workspace leaves 32
+// bits of workgroups.  For validated arguments.
+int plan_shared(const trinix_shared_prefix_args* a, SharedPlan* pl);
+
 }  // namespace trinix

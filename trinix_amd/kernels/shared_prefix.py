@@ -1,0 +1,107 @@
+"""Attention of a batch of requests behind one shared prefix through
+``libtrinix_attn.so`` (semantics: ``trinix_shared_prefix_args`` in
+``include/trinix_attn.h``).  The prefix's keys and values are read once for the
+whole batch instead of once per request; no counterpart in the reference.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional
+
+import torch
+
+from .. import _native as nat
+from .attention_kernel import _DTYPE_CODE, KERNEL_HEAD_DIMS, TritonAttentionKernel, current_stream_ptr, kernel_head_dim
+
+
+def _strides(t: torch.Tensor):
+    """Element strides; of a dimension of one element, which torch leaves open,
+    the contiguous one."""
+    st, inner = list(t.stride()), 1
+    for d in range(t.dim() - 1, -1, -1):
+        if t.shape[d] <= 1:
+            st[d] = inner
+        inner *= t.shape[d]
+    return st
+
+
+def _operand(t: torch.Tensor, d_kernel: int) -> torch.Tensor:
+    """t as the kernels read it: at their head_dim, rows on 16 bytes."""
+    if t.shape[-1] != d_kernel:
+        t = torch.nn.functional.pad(t, (0, d_kernel - t.shape[-1]))
+    per = 16 // t.element_size()
+
+    def ready(x):
+        st = _strides(x)
+        return st[-1] == 1 and x.data_ptr() % 16 == 0 and all(s % per == 0 for s in st[:-1])
+
+    if not ready(t):
+        t = t.contiguous()
+        if not ready(t):
+            t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def shared_prefix_attention(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Tensor, k: torch.Tensor,
+                            v: torch.Tensor, seq_lens: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                            return_lse: bool = False):
+    """``shared_prefix_attn_func`` (``layers/attention/functional.py``)."""
+    ts = (q, prefix_k, prefix_v, k, v)
+    if not all(t.is_cuda for t in ts):
+        raise ValueError("shared_prefix_attention requires GPU tensors")
+    if any(t.device != q.device for t in ts):
+        raise ValueError(f"the tensors are on different devices: {[str(t.device) for t in ts]}")
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4 or prefix_k.dim() != 3 or prefix_v.dim() != 3:
+        raise ValueError("Expected q, k, v (batch, seqlen, nheads, headdim) and prefix_k, prefix_v (seqlen, nheads, headdim), "
+                         f"got {[tuple(t.shape) for t in ts]}")
+    if q.dtype not in _DTYPE_CODE or any(t.dtype != q.dtype for t in ts):
+        raise ValueError(f"the tensors must share one type of float32, float16 and bfloat16, got {[t.dtype for t in ts]}")
+    B, Sq, H, D = q.shape
+    S, Hkv = k.shape[1], k.shape[2]
+    if k.shape != (B, S, Hkv, D) or v.shape != k.shape or prefix_k.shape[1:] != (Hkv, D) or prefix_v.shape != prefix_k.shape:
+        raise ValueError(f"shapes don't match: q, prefix_k, prefix_v, k, v are {[tuple(t.shape) for t in ts]}")
+    if Hkv <= 0 or H <= 0 or D <= 0 or H % Hkv != 0:
+        raise ValueError(f"num_heads ({H}) must be a multiple of the KV heads ({Hkv})")
+    d_kernel = kernel_head_dim(D)
+    if d_kernel is None:
+        raise ValueError(f"head_dim {D} > {KERNEL_HEAD_DIMS[-1]} is not supported")
+    if seq_lens is not None and (seq_lens.shape != (B,) or seq_lens.device != q.device
+                                 or seq_lens.dtype not in (torch.int32, torch.int64)):
+        raise ValueError(f"seq_lens must be {B} int32 or int64 lengths on {q.device}, got {tuple(seq_lens.shape)} "
+                         f"{seq_lens.dtype} on {seq_lens.device}")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
+        raise ValueError("shared_prefix_attention has no backward; call it under torch.no_grad()")
+    if not TritonAttentionKernel.is_available():
+        raise RuntimeError("HIP attention kernel not available (build trinix_amd; needs a gfx950 GPU)")
+    out = torch.empty((B, Sq, H, d_kernel), dtype=q.dtype, device=q.device)
+    lse = torch.empty((B, H, Sq), dtype=torch.float32, device=q.device) if return_lse else None
+    if B and Sq:
+        ops = [_operand(t, d_kernel) for t in ts]
+        a = nat.SharedPrefixArgs()
+        a.q, a.prefix_k, a.prefix_v, a.k, a.v = (t.data_ptr() for t in ops)
+        a.q_stride, a.k_stride, a.v_stride = (nat.Int64x4(*_strides(ops[n])) for n in (0, 3, 4))
+        a.prefix_k_stride, a.prefix_v_stride = (nat.Int64x3(*_strides(ops[n])) for n in (1, 2))
+        a.out, a.out_stride = out.data_ptr(), nat.Int64x4(*_strides(out))
+        if lse is not None:
+            a.lse = lse.data_ptr()
+        if seq_lens is not None:
+            seq_lens = seq_lens.to(torch.int32).contiguous()
+            a.seq_lens = seq_lens.data_ptr()
+        a.batch, a.seqlen_q, a.prefix_len, a.capacity = B, Sq, prefix_k.shape[0], S
+        a.nheads_q, a.nheads_kv, a.head_dim, a.dtype = H, Hkv, d_kernel, _DTYPE_CODE[q.dtype]
+        a.softmax_scale = float(D ** -0.5 if scale is None else scale)
+        _launch(a, q.device)
+    if d_kernel != D:
+        out = out[..., :D].contiguous()
+    return (out, lse) if return_lse else out
+
+
+def _launch(a: nat.SharedPrefixArgs, device: torch.device) -> None:
+    if torch.cuda.current_device() != device.index:
+        with torch.cuda.device(device):
+            return _launch(a, device)
+    lib, n = nat.load_library(), ctypes.c_int64(0)
+    nat.check(lib.trinix_shared_prefix_workspace(ctypes.byref(a), ctypes.byref(n)), "trinix_shared_prefix_workspace")
+    ws = torch.empty(n.value, dtype=torch.uint8, device=device)
+    nat.check(lib.trinix_shared_prefix_fwd(ctypes.byref(a), ws.data_ptr(), n.value, current_stream_ptr(device)),
+              "trinix_shared_prefix_fwd")

@@ -1,5 +1,5 @@
 from .base import FastBaseAttention
-from .functional import PackedSequences, packed_attn_func, triton_attn_func
+from .functional import PackedSequences, packed_attn_func, shared_prefix_attn_func, triton_attn_func
 from .grouped_query_attention import FastGroupedQueryAttention
 from .multi_query_attention import FastMultiQueryAttention
 from .multihead_attention import FastMultiHeadAttention
@@ -13,5 +13,6 @@ __all__ = [
     "FastMultiQueryAttention",
     "PackedSequences",
     "packed_attn_func",
+    "shared_prefix_attn_func",
     "triton_attn_func",
 ]

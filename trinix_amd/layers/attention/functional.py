@@ -8,6 +8,7 @@ import torch
 
 from ...kernels.attention_kernel import TritonAttentionKernel, attention
 from ...kernels.packed_attention import PackedSequences, packed_attention
+from ...kernels.shared_prefix import shared_prefix_attention
 
 
 def triton_attn_func(
@@ -141,3 +142,49 @@ def packed_attn_func(
             the sequences were rebuilt between a forward and its backward.
     """
     return packed_attention(q, k, v, sequences, softmax_scale, causal, window_size, alibi_slopes, return_lse)
+
+
+def shared_prefix_attn_func(
+    q: torch.Tensor,
+    prefix_k: torch.Tensor,
+    prefix_v: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    seq_lens: Optional[torch.Tensor] = None,
+    softmax_scale: Optional[float] = None,
+    *,
+    return_lse: bool = False,
+):
+    """Attention of a batch of requests that share a long prefix, whose keys and
+    values are read once for all of them.
+
+    Args:
+        q: (batch, seq_len_q, num_heads, head_dim) GPU tensor (fp32/fp16/bf16);
+            head_dim up to 256.  One row for a decode step, several for drafts
+            or an appended turn.
+        prefix_k, prefix_v: (prefix_len, num_kv_heads, head_dim), seen by every
+            query; ``num_kv_heads`` divides ``num_heads``.
+        k, v: (batch, capacity, num_kv_heads, head_dim): the requests' own
+            caches, any strides (a (batch, num_kv_heads, capacity, head_dim)
+            cache is passed as ``cache.transpose(1, 2)``).  RoPE is the caller's:
+            own position j stands at prefix_len + j.
+        seq_lens: (batch,) int32 or int64 GPU tensor: valid own keys, the queries'
+            among them; query i sees the own keys j <= seq_lens[b] - seq_len_q + i.
+            Rows of the cache behind them are not read.  Values are read on the
+            GPU (a captured graph replays with new ones) and clamped into
+            [0, capacity].  By default capacity.
+        softmax_scale: defaults to ``head_dim ** -0.5``.
+        return_lse: also return the fp32 (batch, num_heads, seq_len_q)
+            log-sum-exp.
+
+    Returns:
+        (batch, seq_len_q, num_heads, head_dim) tensor of q.dtype, without a
+        backward.  A row that sees no key (no prefix, nothing of its own) gives 0
+        and a log-sum-exp of -inf.
+
+    Raises:
+        ValueError: non-GPU tensors, inconsistent shapes, types or devices, or
+            inputs that require gradients.
+        RuntimeError: the HIP kernel library or a gfx950 GPU is unavailable.
+    """
+    return shared_prefix_attention(q, prefix_k, prefix_v, k, v, seq_lens, softmax_scale, return_lse)
