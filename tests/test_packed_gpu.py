@@ -85,6 +85,18 @@ def test_windows_beside_the_diagonal(window):
     check([90, 200, 3], causal=False, window=window, D=64, seed=1)
 
 
+@pytest.mark.parametrize("shape", ["0", "1", "2"])
+@pytest.mark.parametrize("dtype,D", [(BF, 64), (HF, 128), (BF, 256)])
+def test_forced_tile_shapes(shape, dtype, D, monkeypatch):
+    # 64, 128 and 256 rows per workgroup (where the head_dim has that shape)
+    monkeypatch.setenv("TRINIX_PACKED_FWD", shape)
+    kw = dict(D=D, dtype=dtype, grad=False)
+    check([1, 257, 33, 0, 700, 128], pad=9, **kw)
+    check([200, 64, 3], [900, 64, 33], window=(150, 0), **kw)
+    check([300, 40], [10, 555], causal=False, alibi=True, **kw)
+    check([100, 513], window=(-2, 40), causal=False, **kw)
+
+
 def test_single_tokens_and_many_sequences():
     check([1] * 300, D=64, seed=2)
     check([(7 * i) % 23 for i in range(1500)], H=2, Hkv=1, D=64, seed=2)

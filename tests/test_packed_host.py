@@ -243,6 +243,11 @@ int main() {
         int lo, hi;
         bwd_key_tiles(m0, BM, lq, lk, dlo, dhi, 32, lo, hi);
         EXPECT(lo >= hi || (lo >= 0 && (hi - 1) * 32 < lk));
+        int flo, fhi;
+        packed_full_tiles(m0, std::min(m0 + BM, lq) - 1, lk, dlo, dhi, 32, lo, hi, flo, fhi);
+        EXPECT(lo <= flo && flo <= fhi && fhi <= std::max(lo, hi));
+        for (int i = m0; i < std::min(lq, m0 + BM); ++i) for (int j = flo * 32; j < fhi * 32; ++j)
+          EXPECT(j < lk && j - i >= dlo && j - i <= dhi);
         for (int i = m0; i < std::min(lq, m0 + BM); ++i) for (int j = 0; j < lk; ++j) {
           const bool ok = (!causal || j <= i + off) && (!win || (j - i - off >= -wl && j - i - off <= wr));
           EXPECT(ok == (j - i >= dlo && j - i <= dhi));

@@ -72,11 +72,15 @@ struct PackedBlock {
 template <class E>
 constexpr float kLoScale = std::is_same<E, F16>::value ? 2048.f : 1.f;
 
+// Tile shape of a 16-bit forward: kPair 64 rows, two wavefronts per 32 of them
+// taking alternate key tiles; kPlain 128 rows; kWide 256 rows (head_dim 128).
+enum class PackedShape { kPair, kPlain, kWide };
+
 // Launchers, one translation unit per type (attn_packed_*.hip).  rows: block
 // size of the item list that p.items points at.
-hipError_t launch_packed_fwd_bf16(const PackedParams& p, int D, int grid, hipStream_t st);
-hipError_t launch_packed_fwd_f16(const PackedParams& p, int D, int grid, hipStream_t st);
-hipError_t launch_packed_fwd_f32(const PackedParams& p, int D, int grid, hipStream_t st);
+hipError_t launch_packed_fwd_bf16(const PackedParams& p, int D, PackedShape shape, int grid, hipStream_t st);
+hipError_t launch_packed_fwd_f16(const PackedParams& p, int D, PackedShape shape, int grid, hipStream_t st);
+hipError_t launch_packed_fwd_f32(const PackedParams& p, int D, PackedShape shape, int grid, hipStream_t st);
 hipError_t launch_packed_dkdv_bf16(const PackedParams& p, int D, int grid, hipStream_t st);
 hipError_t launch_packed_dkdv_f16(const PackedParams& p, int D, int grid, hipStream_t st);
 hipError_t launch_packed_dkdv_f32(const PackedParams& p, int D, int grid, hipStream_t st);

@@ -1,5 +1,7 @@
 // Entry points of attention over packed sequences, and the delta pass of its
 // backward.
+#include <cstdlib>
+
 #include "attn_packed.h"
 #include "packed_host.h"
 
@@ -96,6 +98,34 @@ int64_t use_list(PackedParams& p, const trinix_packed_args* a, int list) {
   return packed_list_cap(packed_list_is_keys(list) ? a->total_k : a->total_q, a->n_seqs, packed_list_block(list));
 }
 constexpr int kRows128 = 1, kKeys128 = 4;
+constexpr int kListOf[3] = {0, kRows128, 2};  // of a PackedShape
+
+// Shape of the 16-bit forward.  The host knows the totals and the number of
+// sequences, not their lengths.  Measured, bf16 causal, graph-timed, us pair |
+// plain | wide:
+//  - pair where 128-row blocks leave CUs idle and the average sequence is worth
+//    halving: D=128 8192 rows x 4 heads 116 | 134 | 176; 1024 x 32 21.4 | 22.3 |
+//    28.8; 512 x 32 12.6 | 13.3; D=64 2 x 1024 x 12 13.1 | 16.6.  It loses on short
+//    sequences (1 + 17 + 64 x 32: 6.4 | 5.5; D=64 20 x 200 x 16 16.6 | 10.5) and on more
+//    blocks (2048 x 32 52.4 | 47.8 | 54.3);
+//  - wide (D=128) on long sequences that fill the chip with 256-row blocks: 4096 x 32
+//    170 | 141 | 131, 8192 x 16 317 | 269 | 246, 1814 rows behind 34000 keys, window
+//    4096, 143 | 119 | 112; even at an average of 4096 (8192 + 4099 + 2500 + 1593: 703 |
+//    703), it loses below (4096 + 2047 + 1000 + ..., average 1365: 183 | 191; 8 x 1000
+//    90 | 103; 40 x 300 85 | 121).
+// TRINIX_PACKED_FWD = 0, 1, 2 forces pair, plain, wide (tuning and tests).
+PackedShape packed_shape(const trinix_packed_args* a) {
+  const int64_t n = a->n_seqs, blocks = (a->total_q / 128 + lmin(n, a->total_q) / 2) * a->nheads_q;
+  PackedShape s = PackedShape::kPlain;
+  if (blocks <= 256 && a->total_k / n >= 256) s = PackedShape::kPair;
+  else if (a->total_k / n >= 4096 && a->total_q * a->nheads_q / 256 >= 192) s = PackedShape::kWide;
+  if (const char* env = getenv("TRINIX_PACKED_FWD")) {
+    const int want = atoi(env);
+    if (want >= 0 && want <= 2) s = (PackedShape)want;
+  }
+  if ((a->head_dim == 256 && s == PackedShape::kPair) || (a->head_dim != 128 && s == PackedShape::kWide)) s = PackedShape::kPlain;
+  return s;
+}
 
 }  // namespace
 }  // namespace trinix
@@ -108,13 +138,15 @@ extern "C" int trinix_packed_fwd(const trinix_packed_args* a, void* stream) {
   if (a->total_q == 0) return TRINIX_OK;
   PackedParams p = params(a);
   hipStream_t st = (hipStream_t)stream;
-  const int D = (int)a->head_dim, grid = (int)(use_list(p, a, kRows128) * p.Hq);
+  const int D = (int)a->head_dim;
+  const PackedShape shape = a->dtype == TRINIX_F32 ? PackedShape::kPlain : packed_shape(a);
+  const int grid = (int)(use_list(p, a, kListOf[(int)shape]) * p.Hq);
   hipError_t e;
   if (a->dtype == TRINIX_F32) {
     p.rows16 = rows16(a->k, a->k_stride) && rows16(a->v, a->v_stride);
-    e = launch_packed_fwd_f32(p, D, grid, st);
+    e = launch_packed_fwd_f32(p, D, shape, grid, st);
   } else {
-    e = a->dtype == TRINIX_BF16 ? launch_packed_fwd_bf16(p, D, grid, st) : launch_packed_fwd_f16(p, D, grid, st);
+    e = a->dtype == TRINIX_BF16 ? launch_packed_fwd_bf16(p, D, shape, grid, st) : launch_packed_fwd_f16(p, D, shape, grid, st);
   }
   return e == hipSuccess ? TRINIX_OK : TRINIX_ERR_LAUNCH;
 }

@@ -1,16 +1,11 @@
 // Packed-sequence attention kernels, bf16.
+#include "attn_packed16.h"
 #include "attn_packed_generic.h"
 
 namespace trinix {
 
-hipError_t launch_packed_fwd_bf16(const PackedParams& p, int D, int grid, hipStream_t st) {
-  const dim3 g((unsigned)grid), b(256);
-  switch (D) {
-    case 64: return launch_kernel(&packed_fwd_generic<Ops16<BF16, 64>, BF16, 2>, g, b, 0, st, p);
-    case 128: return launch_kernel(&packed_fwd_generic<Ops16<BF16, 128>, BF16, 2>, g, b, 0, st, p);
-    case 256: return launch_kernel(&packed_fwd_generic<Ops16<BF16, 256>, BF16, 1>, g, b, 0, st, p);
-  }
-  return hipErrorNotSupported;
+hipError_t launch_packed_fwd_bf16(const PackedParams& p, int D, PackedShape shape, int grid, hipStream_t st) {
+  return launch_packed_fwd16<BF16>(p, D, shape, grid, st);
 }
 hipError_t launch_packed_dkdv_bf16(const PackedParams& p, int D, int grid, hipStream_t st) {
   switch (D) {

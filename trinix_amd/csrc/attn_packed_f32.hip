@@ -3,7 +3,7 @@
 
 namespace trinix {
 
-hipError_t launch_packed_fwd_f32(const PackedParams& p, int D, int grid, hipStream_t st) {
+hipError_t launch_packed_fwd_f32(const PackedParams& p, int D, PackedShape, int grid, hipStream_t st) {
   const dim3 g((unsigned)grid), b(256);
   switch (D) {
     case 64: return launch_kernel(&packed_fwd_generic<Ops32<64>, BF16, 2>, g, b, 0, st, p);

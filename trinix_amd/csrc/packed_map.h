@@ -109,4 +109,12 @@ __host__ __device__ inline void packed_band(int lq, int lk, bool causal, bool ha
   dhi = (int)lmin(lmax(hi, -kFar), kFar);
 }
 
+// Tiles of BN keys, within [t_lo, t_hi), whose keys all of rows m0 .. mlast see.
+__host__ __device__ inline void packed_full_tiles(int m0, int mlast, int lk, int dlo, int dhi, int BN, int t_lo, int t_hi,
+                                                  int& t_flo, int& t_fhi) {
+  const int64_t flo = lmax(0, (int64_t)mlast + dlo), fhi = lmin((int64_t)lk, (int64_t)m0 + dhi + 1);
+  t_flo = (int)lmin(lmax((flo + BN - 1) / BN, t_lo), t_hi);
+  t_fhi = (int)lmin(lmax(fhi > 0 ? fhi / BN : 0, t_flo), t_hi);
+}
+
 }  // namespace trinix
