@@ -69,6 +69,8 @@ def shared_args(**kw):
     (dict(out=4104), nat.TRINIX_ERR_BAD_STRIDE),
     (dict(k_stride=nat.Int64x4(500 * 256, 256, 132, 1)), nat.TRINIX_ERR_BAD_STRIDE),
     (dict(prefix_k_stride=nat.Int64x3(256, 128, 2)), nat.TRINIX_ERR_BAD_STRIDE),
+    (dict(prefix_v_stride=nat.Int64x3(1 << 22, 128, 1)), nat.TRINIX_ERR_BAD_STRIDE),
+    (dict(v_stride=nat.Int64x4(500 * 256, -256, 128, 1)), nat.TRINIX_ERR_BAD_STRIDE),
     (dict(seq_lens=4098), nat.TRINIX_ERR_BAD_STRIDE),
     (dict(lse=4098), nat.TRINIX_ERR_BAD_STRIDE),
 ])

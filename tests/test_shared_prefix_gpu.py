@@ -130,6 +130,17 @@ def test_strided_and_unaligned_operands(dtype):
     close("out", got, out, tol, dtype)
 
 
+@pytest.mark.parametrize("kind", ["1", "2", "3"])
+@pytest.mark.parametrize("dtype,D", [(BF, 64), (HF, 128), (BF, 256)])
+def test_forced_kinds(kind, dtype, D, monkeypatch):
+    # 64 or 128 rows by a chunk of keys, whole rows of 64 and of 128
+    monkeypatch.setenv("TRINIX_SHARED_KIND", kind)
+    check(5, 1, 300, 200, [1, 200, 64, 0, 129], D=D, dtype=dtype)
+    check(3, 40, 1000, 500, [500, 3, 97], D=D, dtype=dtype)
+    check(2, 100, 0, 260, [260, 0], H=6, Hkv=3, D=D, dtype=dtype)
+    check(2, 7, 65, 0, [0, 0], H=6, Hkv=3, D=D, dtype=dtype)
+
+
 def test_lengths_outside_the_cache_are_clamped():
     check(4, 1, 60, 64, [-5, 1000, 64, 0], poison=False)
 

@@ -7,6 +7,8 @@
 #endif
 #include "packed_map.h"
 
+#include <cstdlib>
+
 namespace trinix {
 namespace {
 
@@ -65,13 +67,14 @@ int validate_packed(const trinix_packed_args* a, bool backward) {
 namespace {
 
 // (batch, rows, heads, head_dim) or, without a batch, (rows, heads, head_dim):
-// head_dim stride 1, rows on 16 bytes.
+// head_dim stride 1, rows on 16 bytes, a row stride that the kernels' 32-bit
+// in-tile offsets reach.
 int check_vec(const void* ptr, const int64_t* st, int dims, int esize) {
   if (!ptr) return TRINIX_ERR_NULL_POINTER;
   if (st[dims - 1] != 1 || ((uintptr_t)ptr & 15) != 0) return TRINIX_ERR_BAD_STRIDE;
   for (int d = 0; d < dims - 1; ++d)
-    if (st[d] * esize % 16 != 0) return TRINIX_ERR_BAD_STRIDE;
-  return TRINIX_OK;
+    if (st[d] % (16 / esize) != 0) return TRINIX_ERR_BAD_STRIDE;
+  return st[dims - 3] >= 0 && st[dims - 3] < kMaxKvRowStride ? TRINIX_OK : TRINIX_ERR_BAD_STRIDE;
 }
 
 }  // namespace
@@ -98,28 +101,55 @@ int validate_shared(const trinix_shared_prefix_args* a) {
   return TRINIX_OK;
 }
 
+// Blocks of whole rows that fill the chip: from 192 on one workgroup per block walks
+// all keys.  Measured, bf16, us split | whole 64 | whole 128: 256 blocks of 64 rows (B=32
+// Sq=16 G=4, P=4096) 85 | 66; 64 of them 30 | 62; 512 blocks of 32 rows (B=64 Sq=8 16/4
+// D=64, P=2048) 30 | 27; of 16 rows (Sq=4, P=8192) 76 | 149; 512 blocks of 128 rows (B=8
+// Sq=256 G=4, P=6000) 309 | 246 | 204; 256 of them (B=16 Sq=100 16/16 D=64) 51 | 22 | 22;
+// 56 (B=2 Sq=200 16/4) 41 | 63 | 78.
+constexpr int64_t kSharedWhole = 192;
+
 int plan_shared(const trinix_shared_prefix_args* a, SharedPlan* pl) {
-  const int64_t G = a->nheads_q / a->nheads_kv, own_rows = a->seqlen_q * G, rows = a->batch * own_rows;
-  const int64_t rgp = (rows + 15) / 16, rgs = (own_rows + 15) / 16;
-  // chunks of at least 128 keys, as many as give about kDecodeTargetWgs workgroups
-  const auto split = [](int64_t keys, int64_t groups, int* n, int* chunk) {
-    const int64_t want = lmax(1, kDecodeTargetWgs / groups), per = (keys + want - 1) / want;
-    const int64_t c = lmax(kDecodeMinChunk, (per + 63) / 64 * 64);
-    *n = (int)((keys + c - 1) / c);
+  const int64_t G = a->nheads_q / a->nheads_kv, own = a->seqlen_q * G, rows = a->batch * own, kv = a->nheads_kv;
+  const bool f32 = a->dtype == TRINIX_F32;
+  const auto blocks = [](int64_t n, int64_t per) { return (n + per - 1) / per; };
+  pl->rows = (int)rows;
+  const bool d256 = a->head_dim == 256;
+  pl->kind = f32 ? SharedKind::kRows16 : SharedKind::kSplit;
+  if (!f32 && !d256 && own >= 32 && own <= 64 && a->batch * kv >= kSharedWhole) pl->kind = SharedKind::kWhole64;
+  else if (!f32 && own > 64 && a->batch * blocks(own, 128) * kv >= kSharedWhole) pl->kind = SharedKind::kWhole128;
+  if (const char* env = getenv("TRINIX_SHARED_KIND")) {  // 1, 2, 3: split, whole 64, whole 128 (tuning and tests)
+    const int want = atoi(env);
+    if (!f32 && want >= 1 && want <= 3 && !(d256 && want == 2)) pl->kind = (SharedKind)want;
+  }
+  if (pl->kind == SharedKind::kWhole64 || pl->kind == SharedKind::kWhole128) {
+    pl->n_p = pl->n_s = 0;
+    pl->chunk_p = pl->chunk_s = 0;
+    pl->wg_p = 0;
+    pl->wg_s = a->batch * blocks(own, pl->kind == SharedKind::kWhole64 ? 64 : 128) * kv;
+    pl->ws_bytes = 0;
+    return pl->wg_s > INT32_MAX ? TRINIX_ERR_BAD_SHAPE : TRINIX_OK;
+  }
+  const bool r16 = pl->kind == SharedKind::kRows16;
+  const int64_t bm = r16 ? 16 : d256 ? 128 : 64;
+  const int64_t gp = blocks(rows, bm) * kv, gs = a->batch * blocks(own, bm) * kv;
+  // Chunks of whole 64 keys, at least 128, as many as give about `target`
+  // workgroups.  16-bit: 256 for the prefix and 1024 for the own keys; targets of
+  // 128 / 256 / 512 / 1024 for the prefix: B=64 P=8192 40.8 | 38.9 | 49.3 | 58.7 us, B=1
+  // Sq=256 P=8192 114 | 68 | 60 | 67, B=64 Sq=4 117 | 72 | 79 | 85; of 256 / 512 / 1024 / 2048
+  // for the own keys: B=64 caches of 1024 41.5 | 41.1 | 38.9 | 42.9.
+  const auto split = [&](int64_t keys, int64_t groups, int64_t target, int* n, int* chunk) {
+    const int64_t c = lmax(kDecodeMinChunk, blocks(blocks(keys, lmax(1, target / groups)), 64) * 64);
+    *n = (int)blocks(keys, c);
     *chunk = (int)c;
   };
-  split(a->prefix_len, rgp * a->nheads_kv, &pl->n_p, &pl->chunk_p);
-  split(a->capacity, a->batch * rgs * a->nheads_kv, &pl->n_s, &pl->chunk_s);
-  const int64_t wg_p = rgp * a->nheads_kv * pl->n_p;
-  if (a->batch * rgs * a->nheads_kv >= INT32_MAX / lmax(1, pl->n_s)) return TRINIX_ERR_BAD_SHAPE;
-  const int64_t wg_s = a->batch * rgs * a->nheads_kv * pl->n_s;
-  if (wg_p + wg_s > INT32_MAX) return TRINIX_ERR_BAD_SHAPE;
-  pl->rows = (int)rows;
-  pl->rgp = (int)rgp;
-  pl->rgs = (int)rgs;
-  pl->wg_p = wg_p;
-  pl->wg_s = wg_s;
-  pl->ws_bytes = a->nheads_kv * rows * (pl->n_p + pl->n_s) * (a->head_dim + 1) * 4;
+  split(a->prefix_len, gp, r16 ? kDecodeTargetWgs : 256, &pl->n_p, &pl->chunk_p);
+  split(a->capacity, gs, r16 ? 2 * kDecodeTargetWgs : 1024, &pl->n_s, &pl->chunk_s);
+  if (gp >= INT32_MAX / lmax(1, pl->n_p) || gs >= INT32_MAX / lmax(1, pl->n_s)) return TRINIX_ERR_BAD_SHAPE;
+  pl->wg_p = gp * pl->n_p;
+  pl->wg_s = gs * pl->n_s;
+  if (pl->wg_p + pl->wg_s > INT32_MAX) return TRINIX_ERR_BAD_SHAPE;
+  pl->ws_bytes = kv * rows * (pl->n_p + pl->n_s) * (a->head_dim + 1) * 4;
   return TRINIX_OK;
 }
 

@@ -15,13 +15,20 @@ int validate_packed(const trinix_packed_args* a, bool backward);
 int validate_shared(const trinix_shared_prefix_args* a);
 // A row is a (request, query, head of the KV group): row r = (b * Sq + i) * G + g
 // of a KV head.  Partial results (fp32, per row and chunk of keys) of n_p prefix
-// chunks and n_s chunks of the own keys are merged by a second kernel.
+// chunks and n_s chunks of the own keys are merged by a second kernel; the whole
+// kinds have none.
+enum class SharedKind {
+  kRows16,    // 16 rows by a chunk of keys (fp32)
+  kSplit,     // 64 rows by a chunk of keys (head_dim 256: 128)
+  kWhole64,   // 64 rows of a request by all its keys
+  kWhole128,  // 128 rows
+};
 struct SharedPlan {
+  SharedKind kind;
   int rows;            // rows per KV head
-  int rgp, rgs;        // 16-row groups: of all rows (prefix), of one request (own keys)
   int n_p, chunk_p;    // chunks of the prefix, keys per chunk
   int n_s, chunk_s;    // the same for the own keys (at the cache's capacity)
-  int64_t wg_p, wg_s;  // workgroups
+  int64_t wg_p, wg_s;  // workgroups of the prefix and of the own keys (whole: all in wg_s)
   int64_t ws_bytes;
 };
 // TRINIX_OK, or TRINIX_ERR_BAD_SHAPE where the grid or the workspace leaves 32

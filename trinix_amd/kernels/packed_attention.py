@@ -70,6 +70,7 @@ class PackedSequences:
         nat.check(nat.load_library().trinix_packed_plan_bytes(self.n_seqs, self.total_q, self.total_k, ctypes.byref(n)),
                   "trinix_packed_plan_bytes")
         self._bytes = n.value
+        self._launches: dict = {}  # of calls with these sequences (_Launch)
         self.plan = torch.empty(n.value // 4, dtype=torch.int32, device=device)
         self.generation = 0
         self.rebuild()
@@ -148,8 +149,6 @@ def _check(q, k, v, seqs: PackedSequences, alibi_slopes) -> None:
         raise ValueError(f"Unsupported dtype {q.dtype}; use float32, float16 or bfloat16")
     if k.dtype != q.dtype or v.dtype != q.dtype:
         raise ValueError(f"q, k, v dtypes differ: {q.dtype}, {k.dtype}, {v.dtype}")
-    if not isinstance(seqs, PackedSequences):
-        raise ValueError(f"sequences must be PackedSequences, got {type(seqs)}")
     if not (q.device == k.device == v.device == seqs.device):
         raise ValueError(f"q, k, v and the sequences are on different devices: {q.device}, {k.device}, {v.device}, "
                          f"{seqs.device}")
@@ -185,6 +184,20 @@ def _args(q, k, v, seqs, scale, causal, window_size, slopes) -> nat.PackedArgs:
     return a
 
 
+# Launch cache (see attention_kernel.py), kept with the sequences: a call whose
+# operands the kernels read in place is described, apart from its pointers, by
+# shapes, strides, types and scalars.  The first one goes through every check and
+# leaves its arguments; the first backward leaves its own, per strides of dout.
+class _Launch:
+    __slots__ = ("fwd", "bwd", "slopes_as_given")
+
+    def __init__(self, fwd, slopes_as_given):
+        self.fwd, self.bwd, self.slopes_as_given = fwd, {}, slopes_as_given
+
+
+_MAX_LAUNCHES = 64
+
+
 def _launch(fn: str, a: nat.PackedArgs, device: torch.device) -> None:
     lib = nat.load_library()
     if torch.cuda.current_device() == device.index:
@@ -194,31 +207,34 @@ def _launch(fn: str, a: nat.PackedArgs, device: torch.device) -> None:
             nat.check(getattr(lib, fn)(ctypes.byref(a), current_stream_ptr(device)), fn)
 
 
-def _forward(q, k, v, seqs, scale, causal, window_size, slopes, want_lse, keep):
-    """(out at the kernel's head_dim, out_lo, lse, operands as the kernel read them)"""
-    d_kernel = kernel_head_dim(q.shape[-1])
-    q, k, v = (_operand(t, d_kernel) for t in (q, k, v))
+def _run(a, q, slopes, want_lse, keep):
+    """Allocates the outputs of a forward (arguments a, operands set) and launches
+    it: (out at the kernel's head_dim, out_lo, lse)."""
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    out_lo = torch.empty_like(out) if keep and q.dtype != torch.float32 else None
-    lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device) if want_lse or keep else None
-    a = _args(q, k, v, seqs, scale, causal, window_size, slopes)
-    a.out, a.out_stride = out.data_ptr(), nat.Int64x3(*_strides(out))
-    if out_lo is not None:
+    a.out = out.data_ptr()
+    out_lo = lse = None
+    if keep and q.dtype != torch.float32:
+        out_lo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         a.out_lo = out_lo.data_ptr()
-    if lse is not None:
+    if want_lse or keep:
+        lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device)
         a.lse = lse.data_ptr()
+    if slopes is not None:
+        a.alibi_slopes = slopes.data_ptr()
     _launch("trinix_packed_fwd", a, q.device)
-    return out, out_lo, lse, (q, k, v)
+    return out, out_lo, lse
 
 
 class _PackedAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, seqs, scale, causal, window_size, slopes, return_lse):
-        out, out_lo, lse, ops = _forward(q, k, v, seqs, scale, causal, window_size, slopes, True, True)
-        D = q.shape[-1]
-        ctx.save_for_backward(*ops, out, out_lo, lse, slopes)
-        ctx.call = (seqs, seqs.generation, scale, causal, window_size, D)
-        res = out if out.shape[-1] == D else out[..., :D].contiguous()
+    def forward(ctx, q, k, v, ent, a, seqs, slopes, return_lse):
+        D, d_kernel = q.shape[-1], int(a.head_dim)
+        if ent is None:
+            q, k, v = _set_operands(a, q, k, v, d_kernel)
+        out, out_lo, lse = _run(a, q, slopes, True, True)
+        ctx.save_for_backward(q, k, v, out, out_lo, lse, slopes)
+        ctx.call = (ent, a, seqs, seqs.generation, D)
+        res = out if d_kernel == D else out[..., :D].contiguous()
         if return_lse:
             ctx.mark_non_differentiable(lse)
             return res, lse
@@ -227,23 +243,58 @@ class _PackedAttention(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dout, *unused):
         q, k, v, out, out_lo, lse, slopes = ctx.saved_tensors
-        seqs, generation, scale, causal, window_size, D = ctx.call
+        ent, fwd, seqs, generation, D = ctx.call
         if seqs.generation != generation:
             raise RuntimeError("the packed sequences were rebuilt between the forward and its backward")
-        do = _operand(dout.to(q.dtype), q.shape[-1])
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        delta = torch.empty_like(lse)
-        a = _args(q, k, v, seqs, scale, causal, window_size, slopes)
+        delta = torch.empty(lse.shape, dtype=torch.float32, device=lse.device)
+        tpl = None
+        if ent is not None and dout.dtype == q.dtype and not dout.data_ptr() % 16:
+            tpl = ent.bwd.get(dout.stride())
+        if tpl is not None:
+            a, do = nat.PackedArgs.from_buffer_copy(tpl), dout
+        else:
+            a, do = nat.PackedArgs.from_buffer_copy(fwd), _operand(dout.to(q.dtype), q.shape[-1])
+            for name, t in (("out", out), ("dout", do), ("dq", dq), ("dk", dk), ("dv", dv)):
+                setattr(a, name + "_stride", nat.Int64x3(*_strides(t)))
+            if ent is not None and do is dout and len(ent.bwd) < _MAX_LAUNCHES:
+                ent.bwd[dout.stride()] = nat.PackedArgs.from_buffer_copy(a)
+        a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
         a.out, a.dout, a.lse, a.delta = out.data_ptr(), do.data_ptr(), lse.data_ptr(), delta.data_ptr()
-        if out_lo is not None:
-            a.out_lo = out_lo.data_ptr()
+        a.out_lo = None if out_lo is None else out_lo.data_ptr()
         a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
-        for name, t in (("out", out), ("dout", do), ("dq", dq), ("dk", dk), ("dv", dv)):
-            setattr(a, name + "_stride", nat.Int64x3(*_strides(t)))
+        if slopes is not None:
+            a.alibi_slopes = slopes.data_ptr()
         _launch("trinix_packed_bwd", a, q.device)
         if q.shape[-1] != D:
             dq, dk, dv = dq[..., :D], dk[..., :D], dv[..., :D]
-        return dq, dk, dv, None, None, None, None, None, None
+        return dq, dk, dv, None, None, None, None, None
+
+
+def _set_operands(a, q, k, v, d_kernel):
+    """The operands as the kernels read them, entered into a."""
+    q, k, v = (_operand(t, d_kernel) for t in (q, k, v))
+    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    a.q_stride, a.k_stride, a.v_stride = (nat.Int64x3(*_strides(t)) for t in (q, k, v))
+    H = q.shape[1]
+    a.out_stride = nat.Int64x3(H * d_kernel, d_kernel, 1)
+    return q, k, v
+
+
+def _args(q, k, seqs, scale, causal, window_size, slopes, d_kernel) -> nat.PackedArgs:
+    a = nat.PackedArgs()
+    a.plan, a.plan_bytes = seqs.plan.data_ptr(), seqs._bytes
+    a.n_seqs, a.total_q, a.total_k = seqs.n_seqs, seqs.total_q, seqs.total_k
+    a.nheads_q, a.nheads_kv, a.head_dim = q.shape[1], k.shape[1], d_kernel
+    a.dtype = _DTYPE_CODE[q.dtype]
+    a.softmax_scale = float(q.shape[-1] ** -0.5 if scale is None else scale)
+    a.causal = 1 if causal else 0
+    if window_size is not None:
+        a.has_window = 1
+        a.window_left, a.window_right = int(window_size[0]), int(window_size[1])
+    if slopes is not None:
+        a.alibi_stride = 1
+    return a
 
 
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sequences: PackedSequences,
@@ -252,15 +303,45 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sequence
                      return_lse: bool = False):
     """``packed_attn_func`` (``layers/attention/functional.py``), with gradients
     when q, k or v require them."""
-    _check(q, k, v, sequences, alibi_slopes)
-    if scale is None:
-        scale = q.shape[-1] ** -0.5
-    slopes = None
-    if alibi_slopes is not None:
+    if not isinstance(sequences, PackedSequences):
+        raise ValueError(f"sequences must be PackedSequences, got {type(sequences)}")
+    if window_size is not None:
+        window_size = (int(window_size[0]), int(window_size[1]))
+    grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
+    key = (q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), q.dtype, k.dtype, v.dtype, q.device, k.device,
+           v.device, scale, bool(causal), window_size,
+           None if alibi_slopes is None else (alibi_slopes.shape, alibi_slopes.dtype, alibi_slopes.stride(), alibi_slopes.device))
+    ent = sequences._launches.get(key)
+    if ent is not None and (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16:
+        ent = None
+    if ent is None:
+        _check(q, k, v, sequences, alibi_slopes)
+    slopes = alibi_slopes
+    if slopes is not None and (ent is None or not ent.slopes_as_given):
         slopes = alibi_slopes.detach().reshape(-1).to(device=q.device, dtype=torch.float32).contiguous()
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _PackedAttention.apply(q, k, v, sequences, float(scale), causal, window_size, slopes, return_lse)
-    out, _, lse, _ = _forward(q, k, v, sequences, float(scale), causal, window_size, slopes, return_lse, False)
-    if out.shape[-1] != q.shape[-1]:
-        out = out[..., :q.shape[-1]].contiguous()
+    elif slopes is not None:
+        slopes = slopes.detach()
+    if ent is not None:
+        a = nat.PackedArgs.from_buffer_copy(ent.fwd)
+        a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    else:
+        d_kernel = kernel_head_dim(q.shape[-1])
+        a = _args(q, k, sequences, scale, causal, window_size, slopes, d_kernel)
+        if d_kernel == q.shape[-1] and _ready(q) and _ready(k) and _ready(v):
+            _set_operands(a, q, k, v, d_kernel)
+            as_given = alibi_slopes is not None and (alibi_slopes.dim() == 1 and alibi_slopes.dtype == torch.float32
+                                                     and alibi_slopes.device == q.device and alibi_slopes.is_contiguous())
+            ent = _Launch(nat.PackedArgs.from_buffer_copy(a), as_given)
+            ent.fwd.q = ent.fwd.k = ent.fwd.v = None
+            if not (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16:
+                if len(sequences._launches) >= _MAX_LAUNCHES:
+                    sequences._launches.clear()
+                sequences._launches[key] = ent
+    if grad:
+        return _PackedAttention.apply(q, k, v, ent, a, sequences, slopes, return_lse)
+    D = q.shape[-1]
+    ops = (q, k, v) if ent is not None else _set_operands(a, q, k, v, int(a.head_dim))  # held until the launch returns
+    out, _, lse = _run(a, ops[0], slopes, return_lse, False)
+    if out.shape[-1] != D:
+        out = out[..., :D].contiguous()
     return (out, lse) if return_lse else out
