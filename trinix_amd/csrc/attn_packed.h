@@ -29,16 +29,17 @@ struct PackedParams {
   int64_t al_sh;
   int rows16;             // fp32: q, k, v and dout take 16-byte copies
   const int32_t* items;   // of the launch's list
+  const int32_t* items_q; // of its second one (packed_bwd16)
 };
 
 // The block of rows or keys that a workgroup runs: its sequence (first row and
 // rows, first key and keys), block number (-1: none) and head, all wave-uniform.
 struct PackedBlock {
   int q0, lq, k0, lk, blk, h, dlo, dhi;
-  __device__ PackedBlock(const PackedParams& p, int wg, int heads_kv, int G) {
+  __device__ PackedBlock(const PackedParams& p, const int32_t* items, int wg, int heads_kv, int G) {
     typedef int i32x4 __attribute__((ext_vector_type(4)));
     const PackedWork w = packed_work(wg, heads_kv, G);
-    const i32x4* it = (const i32x4*)(p.items + (int64_t)w.item * kPackedItemInts);
+    const i32x4* it = (const i32x4*)(items + (int64_t)w.item * kPackedItemInts);
     const i32x4 a = it[0];
     q0 = __builtin_amdgcn_readfirstlane(a[0]);
     lq = __builtin_amdgcn_readfirstlane(a[1]);
@@ -81,11 +82,14 @@ enum class PackedShape { kPair, kPlain, kWide };
 hipError_t launch_packed_fwd_bf16(const PackedParams& p, int D, PackedShape shape, int grid, hipStream_t st);
 hipError_t launch_packed_fwd_f16(const PackedParams& p, int D, PackedShape shape, int grid, hipStream_t st);
 hipError_t launch_packed_fwd_f32(const PackedParams& p, int D, PackedShape shape, int grid, hipStream_t st);
-hipError_t launch_packed_dkdv_bf16(const PackedParams& p, int D, int grid, hipStream_t st);
-hipError_t launch_packed_dkdv_f16(const PackedParams& p, int D, int grid, hipStream_t st);
+// dK and dV, and dQ (16-bit: head_dim 256; 64 and 128 run both in one launch).
+hipError_t launch_packed_dkdv_bf16(const PackedParams& p, int grid, hipStream_t st);
+hipError_t launch_packed_dkdv_f16(const PackedParams& p, int grid, hipStream_t st);
 hipError_t launch_packed_dkdv_f32(const PackedParams& p, int D, int grid, hipStream_t st);
-hipError_t launch_packed_dq_bf16(const PackedParams& p, int D, int grid, hipStream_t st);
-hipError_t launch_packed_dq_f16(const PackedParams& p, int D, int grid, hipStream_t st);
+hipError_t launch_packed_dq_bf16(const PackedParams& p, int grid, hipStream_t st);
+hipError_t launch_packed_dq_f16(const PackedParams& p, int grid, hipStream_t st);
 hipError_t launch_packed_dq_f32(const PackedParams& p, int D, int grid, hipStream_t st);
+hipError_t launch_packed_bwd_bf16(const PackedParams& p, int D, int ks, int n_kv, int n_q, hipStream_t st);
+hipError_t launch_packed_bwd_f16(const PackedParams& p, int D, int ks, int n_kv, int n_q, hipStream_t st);
 
 }  // namespace trinix

@@ -97,8 +97,8 @@ int64_t use_list(PackedParams& p, const trinix_packed_args* a, int list) {
   p.items = a->plan + packed_list_offset(list, a->total_q, a->total_k, a->n_seqs);
   return packed_list_cap(packed_list_is_keys(list) ? a->total_k : a->total_q, a->n_seqs, packed_list_block(list));
 }
-constexpr int kRows128 = 1, kKeys128 = 4;
-constexpr int kListOf[3] = {0, kRows128, 2};  // of a PackedShape
+constexpr int kRows128 = 1, kRows256 = 2, kKeys128 = 4;
+constexpr int kListOf[3] = {0, kRows128, kRows256};  // of a PackedShape
 
 // Shape of the 16-bit forward.  The host knows the totals and the number of
 // sequences, not their lengths.  Measured, bf16 causal, graph-timed, us pair |
@@ -125,6 +125,12 @@ PackedShape packed_shape(const trinix_packed_args* a) {
   }
   if ((a->head_dim == 256 && s == PackedShape::kPair) || (a->head_dim != 128 && s == PackedShape::kWide)) s = PackedShape::kPlain;
   return s;
+}
+
+// dQ of packed_bwd16 in blocks of 128 rows, two wavefronts per 32.
+bool bwd_pairs(const trinix_packed_args* a) {
+  if (const char* env = getenv("TRINIX_PACKED_BWD")) return atoi(env) == 2;
+  return a->total_q / a->n_seqs < 256;
 }
 
 }  // namespace
@@ -164,15 +170,24 @@ extern "C" int trinix_packed_bwd(const trinix_packed_args* a, void* stream) {
     e = f32 ? launch_delta<BF16, true>(p, D, st) : bf ? launch_delta<BF16, false>(p, D, st) : launch_delta<F16, false>(p, D, st);
     if (e != hipSuccess) return TRINIX_ERR_LAUNCH;
   }
+  if (!f32 && D != 256) {
+    const int ks = bwd_pairs(a) ? 2 : 1;
+    const int n_q = (int)(use_list(p, a, ks == 2 ? kRows128 : kRows256) * p.Hq);
+    p.items_q = p.items;
+    const int n_kv = (int)(use_list(p, a, kKeys128) * p.Hkv);
+    if (n_kv + n_q > 0)
+      e = bf ? launch_packed_bwd_bf16(p, D, ks, n_kv, n_q, st) : launch_packed_bwd_f16(p, D, ks, n_kv, n_q, st);
+    return e == hipSuccess ? TRINIX_OK : TRINIX_ERR_LAUNCH;
+  }
   if (a->total_k > 0) {
     const int grid = (int)(use_list(p, a, kKeys128) * p.Hkv);
-    e = f32 ? launch_packed_dkdv_f32(p, D, grid, st) : bf ? launch_packed_dkdv_bf16(p, D, grid, st) : launch_packed_dkdv_f16(p, D, grid, st);
+    e = f32 ? launch_packed_dkdv_f32(p, D, grid, st) : bf ? launch_packed_dkdv_bf16(p, grid, st) : launch_packed_dkdv_f16(p, grid, st);
     if (e != hipSuccess) return TRINIX_ERR_LAUNCH;
   }
   if (a->total_q > 0) {
     if (f32) p.rows16 = rows16(a->k, a->k_stride) && rows16(a->v, a->v_stride);
     const int grid = (int)(use_list(p, a, kRows128) * p.Hq);
-    e = f32 ? launch_packed_dq_f32(p, D, grid, st) : bf ? launch_packed_dq_bf16(p, D, grid, st) : launch_packed_dq_f16(p, D, grid, st);
+    e = f32 ? launch_packed_dq_f32(p, D, grid, st) : bf ? launch_packed_dq_bf16(p, grid, st) : launch_packed_dq_f16(p, grid, st);
   }
   return e == hipSuccess ? TRINIX_OK : TRINIX_ERR_LAUNCH;
 }

@@ -10,7 +10,7 @@ template <class E, int D, int BN, int NW, int OCC, int KS, bool ALIBI>
 __global__ __launch_bounds__(NW * 64, OCC) void packed_fwd16(const PackedParams p) {
   constexpr int BM = NW * 32 / KS, DB = D / 32;
   TRINIX_TILE16_LDS(D, BN, KS);
-  const PackedBlock w(p, (int)blockIdx.x, p.Hkv, p.G);
+  const PackedBlock w(p, p.items, (int)blockIdx.x, p.Hkv, p.G);
   if (w.blk < 0) return;
   Tile16<E, D, BN, NW, KS, ALIBI> T(lds_k0, lds_k1, lds_v0, lds_v1);
   const int hq = w.h, hkv = hq / p.G, m0 = w.blk * BM, iw0 = m0 + (T.wave / KS) * 32, i = iw0 + T.r;

@@ -21,7 +21,7 @@ __global__ __launch_bounds__(256, OCC) void packed_fwd_generic(const PackedParam
   constexpr int NW = 4, BM = NW * 32, D = O::kD, DB = D / 32, TILE = kTileRows * D * (int)sizeof(Store);
   __shared__ __attribute__((aligned(1024))) char lds_k[2][TILE];
   __shared__ __attribute__((aligned(1024))) char lds_v[2][TILE];
-  const PackedBlock w(p, (int)blockIdx.x, p.Hkv, p.G);
+  const PackedBlock w(p, p.items, (int)blockIdx.x, p.Hkv, p.G);
   if (w.blk < 0) return;
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -136,7 +136,7 @@ __global__ __launch_bounds__(256, OCC) void packed_dkdv_generic(const PackedPara
   __shared__ __attribute__((aligned(128))) float lds_l[2][kTileRows];
   __shared__ __attribute__((aligned(128))) float lds_d[2][kTileRows];
   // HS workgroups share a key block, each summing D / HS of the columns
-  const PackedBlock w(p, (int)blockIdx.x / HS, p.Hkv, 1);
+  const PackedBlock w(p, p.items, (int)blockIdx.x / HS, p.Hkv, 1);
   if (w.blk < 0) return;
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -253,7 +253,7 @@ __global__ __launch_bounds__(256, OCC) void packed_dq_generic(const PackedParams
   constexpr int NW = 4, BM = NW * 32, D = O::kD, DB = O::DB / HS, TILE = kTileRows * D * (int)sizeof(Store);
   __shared__ __attribute__((aligned(1024))) char lds_k[2][TILE];
   __shared__ __attribute__((aligned(1024))) char lds_v[2][TILE];
-  const PackedBlock w(p, (int)blockIdx.x / HS, p.Hkv, p.G);
+  const PackedBlock w(p, p.items, (int)blockIdx.x / HS, p.Hkv, p.G);
   if (w.blk < 0) return;
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
