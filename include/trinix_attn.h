@@ -511,12 +511,17 @@ typedef struct trinix_packed_args {
   int64_t window_left, window_right;
   const float* alibi_slopes; /* (Hq) fp32, or NULL */
   int64_t alibi_stride;
+  void* workspace;      /* backward: trinix_packed_bwd_workspace bytes, 16-byte aligned */
+  int64_t workspace_bytes;
 } trinix_packed_args;
 
 /* Forward and backward on `stream`; 16-bit rows 16-byte aligned.  The backward
  * takes the forward's out, out_lo and lse.  No atomics: the same call gives the
- * same bits. */
+ * same bits.
+ * trinix_packed_bwd_workspace: bytes of workspace that the backward of these
+ * arguments takes (host only; 0 where the KV heads alone fill the GPU). */
 int trinix_packed_fwd(const trinix_packed_args* args, void* stream);
+int trinix_packed_bwd_workspace(const trinix_packed_args* args, int64_t* bytes);
 int trinix_packed_bwd(const trinix_packed_args* args, void* stream);
 
 /* ---- attention of a batch behind one shared prefix (ABI version 7) -----------

@@ -97,6 +97,14 @@ def test_forced_tile_shapes(shape, dtype, D, monkeypatch):
     check([100, 513], window=(-2, 40), causal=False, **kw)
 
 
+@pytest.mark.parametrize("splits", ["1", "2", "3", "16"])
+@pytest.mark.parametrize("dtype,D", [(BF, 64), (HF, 128), (BF, 256), (F32, 64)])
+def test_heads_shared_out(splits, dtype, D, monkeypatch):
+    # the query heads of a KV head over several workgroups, summed in order
+    monkeypatch.setenv("TRINIX_PACKED_SPLITS", splits)
+    check([70, 1, 0, 190], [90, 1, 7, 190], H=5, Hkv=1, D=D, dtype=dtype, pad=4)
+
+
 def test_single_tokens_and_many_sequences():
     check([1] * 300, D=64, seed=2)
     check([(7 * i) % 23 for i in range(1500)], H=2, Hkv=1, D=64, seed=2)

@@ -165,6 +165,22 @@ def test_packed_backward_needs_its_tensors(lib, field):
     assert lib.trinix_packed_bwd(ctypes.byref(a), None) == nat.TRINIX_ERR_NULL_POINTER
 
 
+def test_packed_backward_workspace(lib):
+    n = ctypes.c_int64(-1)
+    a = args(lib)  # 8 heads of their own: no head to share out
+    assert lib.trinix_packed_bwd_workspace(ctypes.byref(a), ctypes.byref(n)) == 0 and n.value == 0
+    a = args(lib, nheads_kv=1)
+    assert lib.trinix_packed_bwd_workspace(ctypes.byref(a), ctypes.byref(n)) == 0
+    assert n.value % (2 * 1000 * 128 * 4) == 0 and n.value > 0
+    for ws, size in ((None, n.value), (4096, n.value - 1), (4104, n.value)):
+        a.workspace, a.workspace_bytes = ws, size
+        assert lib.trinix_packed_bwd(ctypes.byref(a), None) == nat.TRINIX_ERR_BAD_ARGUMENT
+    assert lib.trinix_packed_bwd_workspace(None, ctypes.byref(n)) == nat.TRINIX_ERR_NULL_POINTER
+    assert lib.trinix_packed_bwd_workspace(ctypes.byref(a), None) == nat.TRINIX_ERR_NULL_POINTER
+    for bad in (dict(nheads_kv=0), dict(nheads_kv=3), dict(head_dim=96), dict(total_k=-1), dict(n_seqs=0)):
+        assert lib.trinix_packed_bwd_workspace(ctypes.byref(args(lib, **bad)), ctypes.byref(n)) == nat.TRINIX_ERR_BAD_SHAPE
+
+
 def test_python_layer_without_a_gpu():
     x = torch.zeros(4, 2, 64)
     if not torch.cuda.is_available():

@@ -181,6 +181,8 @@ class PackedArgs(ctypes.Structure):
         ("window_right", c_int64),
         ("alibi_slopes", c_void_p),
         ("alibi_stride", c_int64),
+        ("workspace", c_void_p),
+        ("workspace_bytes", c_int64),
     ]
 
 
@@ -268,6 +270,7 @@ SIGNATURES = {
     "trinix_packed_plan_bytes": (c_int32, [c_int64, c_int64, c_int64, POINTER(c_int64)]),
     "trinix_packed_plan": (c_int32, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p]),
     "trinix_packed_fwd": (c_int32, [POINTER(PackedArgs), c_void_p]),
+    "trinix_packed_bwd_workspace": (c_int32, [POINTER(PackedArgs), POINTER(c_int64)]),
     "trinix_packed_bwd": (c_int32, [POINTER(PackedArgs), c_void_p]),
     "trinix_shared_prefix_workspace": (c_int32, [POINTER(SharedPrefixArgs), POINTER(c_int64)]),
     "trinix_shared_prefix_fwd": (c_int32, [POINTER(SharedPrefixArgs), c_void_p, c_int64, c_void_p]),

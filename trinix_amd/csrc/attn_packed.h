@@ -27,6 +27,10 @@ struct PackedParams {
   int64_t wl, wr;  // clamped to +-2^30
   const float* alibi;
   int64_t al_sh;
+  // dK and dV: a group's heads over n_split workgroups, fp32 partial sums (split, dV
+  // and dK, key, KV head, head_dim), or 1 and null
+  int n_split, Tk;
+  float* part;
   int rows16;             // fp32: q, k, v and dout take 16-byte copies
   const int32_t* items;   // of the launch's list
   const int32_t* items_q; // of its second one (packed_bwd16)
@@ -68,6 +72,19 @@ struct PackedBlock {
   }
 };
 
+// KV head, heads of its group [gh0, gh1) and split of a dK, dV workgroup.
+struct PackedHeads {
+  int hkv, split, gh0, gh1;
+  __device__ PackedHeads(const PackedParams& p, int h) {
+    hkv = h / p.n_split, split = h % p.n_split;
+    gh0 = p.G * split / p.n_split, gh1 = p.G * (split + 1) / p.n_split;
+  }
+};
+// Partial sums of key row `row` (which = 0: dV, 1: dK).
+__device__ inline float* packed_partial(const PackedParams& p, int split, int which, int64_t row, int hkv, int D) {
+  return p.part + ((((int64_t)split * 2 + which) * p.Tk + row) * p.Hkv + hkv) * D;
+}
+
 // fp16 keeps its output's rounding residue times 2^11 (half a step of the
 // largest fp16 number is 2^4; unscaled, the residue of 2^-10 would be denormal).
 template <class E>
@@ -89,7 +106,7 @@ hipError_t launch_packed_dkdv_f32(const PackedParams& p, int D, int grid, hipStr
 hipError_t launch_packed_dq_bf16(const PackedParams& p, int grid, hipStream_t st);
 hipError_t launch_packed_dq_f16(const PackedParams& p, int grid, hipStream_t st);
 hipError_t launch_packed_dq_f32(const PackedParams& p, int D, int grid, hipStream_t st);
-hipError_t launch_packed_bwd_bf16(const PackedParams& p, int D, int ks, int n_kv, int n_q, hipStream_t st);
-hipError_t launch_packed_bwd_f16(const PackedParams& p, int D, int ks, int n_kv, int n_q, hipStream_t st);
+hipError_t launch_packed_bwd_bf16(const PackedParams& p, int D, int n_kv, int n_q, hipStream_t st);
+hipError_t launch_packed_bwd_f16(const PackedParams& p, int D, int n_kv, int n_q, hipStream_t st);
 
 }  // namespace trinix

@@ -47,6 +47,33 @@ __global__ __launch_bounds__(256) void packed_delta_kernel(const PackedParams p,
   }
 }
 
+// Adds the partial sums of dV (blockIdx.y = 0) and dK (1) over the splits, in order:
+// four head_dim elements of a key per thread.
+template <class E, bool F32>
+__global__ __launch_bounds__(256) void packed_dkdv_sum(const PackedParams p, int D) {
+  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4, per = (int64_t)p.Tk * p.Hkv * D;
+  if (at >= per) return;
+  const int which = blockIdx.y;
+  const float* x = p.part + which * per + at;
+  f32x4_t s = *(const f32x4_t*)x;
+  for (int k = 1; k < p.n_split; ++k) s += *(const f32x4_t*)(x + 2 * k * per);
+  const int64_t row = at / D / p.Hkv;
+  const int hkv = (int)(at / D % p.Hkv), d = (int)(at % D);
+  void* base = which ? p.dk : p.dv;
+  const int64_t to = row * (which ? p.dk_ss : p.dv_ss) + hkv * (which ? p.dk_sh : p.dv_sh) + d;
+  if constexpr (F32) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) ((float*)base)[to + e] = s[e];
+  } else {
+    *(u32x2_t*)((uint16_t*)base + to) = (u32x2_t){E::pack(s[0], s[1]), E::pack(s[2], s[3])};
+  }
+}
+template <class E, bool F32>
+hipError_t launch_sum(const PackedParams& p, int D, hipStream_t st) {
+  const int64_t units = (int64_t)p.Tk * p.Hkv * D / 4;
+  return launch_kernel(&packed_dkdv_sum<E, F32>, dim3((unsigned)((units + 255) / 256), 2), dim3(256), 0, st, p, D);
+}
+
 template <class E, bool F32>
 hipError_t launch_delta(const PackedParams& p, int D, hipStream_t st) {
   const int64_t rows = (int64_t)p.Tq * p.Hq;
@@ -97,7 +124,7 @@ int64_t use_list(PackedParams& p, const trinix_packed_args* a, int list) {
   p.items = a->plan + packed_list_offset(list, a->total_q, a->total_k, a->n_seqs);
   return packed_list_cap(packed_list_is_keys(list) ? a->total_k : a->total_q, a->n_seqs, packed_list_block(list));
 }
-constexpr int kRows128 = 1, kRows256 = 2, kKeys128 = 4;
+constexpr int kRows128 = 1, kRows256 = 2, kKeys64 = 3, kKeys128 = 4;
 constexpr int kListOf[3] = {0, kRows128, kRows256};  // of a PackedShape
 
 // Shape of the 16-bit forward.  The host knows the totals and the number of
@@ -125,12 +152,6 @@ PackedShape packed_shape(const trinix_packed_args* a) {
   }
   if ((a->head_dim == 256 && s == PackedShape::kPair) || (a->head_dim != 128 && s == PackedShape::kWide)) s = PackedShape::kPlain;
   return s;
-}
-
-// dQ of packed_bwd16 in blocks of 128 rows, two wavefronts per 32.
-bool bwd_pairs(const trinix_packed_args* a) {
-  if (const char* env = getenv("TRINIX_PACKED_BWD")) return atoi(env) == 2;
-  return a->total_q / a->n_seqs < 256;
 }
 
 }  // namespace
@@ -170,24 +191,28 @@ extern "C" int trinix_packed_bwd(const trinix_packed_args* a, void* stream) {
     e = f32 ? launch_delta<BF16, true>(p, D, st) : bf ? launch_delta<BF16, false>(p, D, st) : launch_delta<F16, false>(p, D, st);
     if (e != hipSuccess) return TRINIX_ERR_LAUNCH;
   }
+  p.Tk = (int)a->total_k;
+  p.n_split = packed_head_splits(a);
+  p.part = (float*)a->workspace;
   if (!f32 && D != 256) {
-    const int ks = bwd_pairs(a) ? 2 : 1;
-    const int n_q = (int)(use_list(p, a, ks == 2 ? kRows128 : kRows256) * p.Hq);
+    const int n_q = (int)(use_list(p, a, kRows128) * p.Hq);
     p.items_q = p.items;
-    const int n_kv = (int)(use_list(p, a, kKeys128) * p.Hkv);
+    const int n_kv = (int)(use_list(p, a, kKeys64) * p.Hkv * p.n_split);
     if (n_kv + n_q > 0)
-      e = bf ? launch_packed_bwd_bf16(p, D, ks, n_kv, n_q, st) : launch_packed_bwd_f16(p, D, ks, n_kv, n_q, st);
-    return e == hipSuccess ? TRINIX_OK : TRINIX_ERR_LAUNCH;
+      e = bf ? launch_packed_bwd_bf16(p, D, n_kv, n_q, st) : launch_packed_bwd_f16(p, D, n_kv, n_q, st);
+  } else {
+    if (a->total_k > 0) {
+      const int grid = (int)(use_list(p, a, kKeys128) * p.Hkv * p.n_split);
+      e = f32 ? launch_packed_dkdv_f32(p, D, grid, st) : bf ? launch_packed_dkdv_bf16(p, grid, st) : launch_packed_dkdv_f16(p, grid, st);
+      if (e != hipSuccess) return TRINIX_ERR_LAUNCH;
+    }
+    if (a->total_q > 0) {
+      if (f32) p.rows16 = rows16(a->k, a->k_stride) && rows16(a->v, a->v_stride);
+      const int grid = (int)(use_list(p, a, kRows128) * p.Hq);
+      e = f32 ? launch_packed_dq_f32(p, D, grid, st) : bf ? launch_packed_dq_bf16(p, grid, st) : launch_packed_dq_f16(p, grid, st);
+    }
   }
-  if (a->total_k > 0) {
-    const int grid = (int)(use_list(p, a, kKeys128) * p.Hkv);
-    e = f32 ? launch_packed_dkdv_f32(p, D, grid, st) : bf ? launch_packed_dkdv_bf16(p, grid, st) : launch_packed_dkdv_f16(p, grid, st);
-    if (e != hipSuccess) return TRINIX_ERR_LAUNCH;
-  }
-  if (a->total_q > 0) {
-    if (f32) p.rows16 = rows16(a->k, a->k_stride) && rows16(a->v, a->v_stride);
-    const int grid = (int)(use_list(p, a, kRows128) * p.Hq);
-    e = f32 ? launch_packed_dq_f32(p, D, grid, st) : bf ? launch_packed_dq_bf16(p, grid, st) : launch_packed_dq_f16(p, grid, st);
-  }
+  if (e == hipSuccess && p.n_split > 1 && a->total_k > 0)
+    e = f32 ? launch_sum<BF16, true>(p, D, st) : bf ? launch_sum<BF16, false>(p, D, st) : launch_sum<F16, false>(p, D, st);
   return e == hipSuccess ? TRINIX_OK : TRINIX_ERR_LAUNCH;
 }

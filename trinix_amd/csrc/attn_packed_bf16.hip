@@ -8,8 +8,8 @@ namespace trinix {
 hipError_t launch_packed_fwd_bf16(const PackedParams& p, int D, PackedShape shape, int grid, hipStream_t st) {
   return launch_packed_fwd16<BF16>(p, D, shape, grid, st);
 }
-hipError_t launch_packed_bwd_bf16(const PackedParams& p, int D, int ks, int n_kv, int n_q, hipStream_t st) {
-  return launch_packed_bwd16<BF16>(p, D, ks, n_kv, n_q, st);
+hipError_t launch_packed_bwd_bf16(const PackedParams& p, int D, int n_kv, int n_q, hipStream_t st) {
+  return launch_packed_bwd16<BF16>(p, D, n_kv, n_q, st);
 }
 hipError_t launch_packed_dkdv_bf16(const PackedParams& p, int grid, hipStream_t st) {
   return launch_packed_dkdv_g<Ops16<BF16, 256>, 1, 2>(p, grid, st);

@@ -1,19 +1,23 @@
 // Gradients of packed-sequence attention, 16-bit types at head_dim 64 and 128, in one
-// launch of 8-wavefront workgroups (no atomics):
-//   dK, dV  128 keys of one sequence and KV head, a pair of wavefronts per 32 keys: the
+// launch (no atomics) of 4-wavefront workgroups, two per CU:
+//   dK, dV  64 keys of one sequence and KV head, a pair of wavefronts per 32 keys: the
 //           first computes S = Q K^T, P = exp(scale S - lse) and dV^T += dO^T P, hands P in
 //           fp32 to the second through LDS, which runs a step behind on dP = dO V^T, dZ = P
 //           (dP - delta) and dK^T += Q^T dZ.  Both walk every head of the group and
 //           every query tile of the band; a pair shares a SIMD, so that one's exponentials
 //           run beside the other's products.  Q, dO tiles rotate through three LDS slots, P
 //           through two; one barrier per tile;
-//   dQ      256 query rows (KS = 2: 128, two wavefronts per 32 taking alternate tiles) of
-//           one sequence and head, 32 per wavefront, over 32-key tiles: S^T, dP^T, dZ^T in
-//           registers, dQ^T += K^T dZ^T.
+//   dQ      128 query rows of one sequence and head, 32 per wavefront, over 32-key
+//           tiles: S^T, dP^T, dZ^T in registers, dQ^T += K^T dZ^T.
 // The dK, dV items come first, longest first, and the dQ items, whose chains are
 // shorter by the heads of a group, fill the CUs that these leave idle: the longest key
 // block of a 4096-row sequence in a batch of 8192 rows has 1.4 times the work of an
-// average CU.
+// average CU.  Forward and backward, bf16 causal, us with 4-wavefront | 8-wavefront
+// workgroups: 4096 + 2047 + 1000 + 3 short, 32/8 heads of 128 1065 | 1089; 40 x 300 434 |
+// 497; 8 documents of 4096 rows, 12 heads of 64 72 | 88; 8192 rows 2880 | 2933 (dK, dV and
+// dQ in kernels of their own, one wavefront per 32 keys, 3290).  A 32x32 block of pairs
+// takes 5 + 4 products of D; 8192 rows run at 1041 TFLOP/s of them, where the library's
+// large bf16 product reaches 1240 on the same card.
 //
 // Roundings: P enters dV in one 16-bit term (the error of dV: 1.2 to 1.4 times that of
 // rounding dV alone); dZ is formed from the fp32 P and enters dK and dQ in two terms x =
@@ -31,38 +35,38 @@ namespace trinix {
 // LDS of the launch, in bytes: the larger of the two parts.
 template <int D>
 struct PackedBwdLds {
-  static constexpr int BQ = D == 64 ? 64 : 32, NST = BQ / 32, NSL = 3, NG = 4;  // dK, dV: rows per item, sub-tiles, slots
-  static constexpr int kQ = BQ * D * 2, kP = NG * NST * 64 * 64;
-  static constexpr int kKv = NSL * 2 * kQ + 2 * kP + NSL * 2 * BQ * 4;
-  static constexpr int KT = D == 64 ? 2 : 1, kK = KT * kTileRows * D * 2;  // dQ: tiles per step and KS
-  static constexpr int kDq(int ks) { return 2 * 2 * ks * kK; }
-  static constexpr int kBytes = kKv > kDq(2) ? kKv : kDq(2);
+  static constexpr int NG = 2, NSL = 3;  // dK, dV: pairs, tile slots
+  static constexpr int kTile = kTileRows * D * 2, kP = NG * 64 * 64;
+  static constexpr int kKv = NSL * 2 * kTile + 2 * kP + NSL * 2 * kTileRows * 4;
+  static constexpr int KT = D == 64 ? 2 : 1, kDq = 2 * 2 * KT * kTile;  // dQ: tiles per step
+  static constexpr int kBytes = kKv > kDq ? kKv : kDq;
 };
 
 template <class E, int D>
 __device__ __forceinline__ void packed_dkdv_body(const PackedParams& p, const PackedBlock& w, char* pool) {
   using O = Ops16<E, D>;
   using L = PackedBwdLds<D>;
-  constexpr int NW = 8, NG = L::NG, BK = NG * 32, BQ = L::BQ, NST = L::NST, NSL = L::NSL;
+  constexpr int NG = L::NG, NW = 2 * NG, BK = NG * 32, BQ = kTileRows, NSL = L::NSL;
   constexpr int DS = D / 16, DB = D / 32, UPR = D / 8, LPW = BQ * UPR / (64 * NW);
   constexpr int RPF = 4, TPF = 2;  // row and transpose reads ahead of their MFMA
   static_assert(LPW >= 1 && BQ * UPR % (64 * NW) == 0, "tile shape");
   char* const lds_q = pool;
-  char* const lds_o = lds_q + NSL * L::kQ;
-  char* const lds_p = lds_o + NSL * L::kQ;
+  char* const lds_o = lds_q + NSL * L::kTile;
+  char* const lds_p = lds_o + NSL * L::kTile;
   float* const lds_l = (float*)(lds_p + 2 * L::kP);
   float* const lds_d = lds_l + NSL * BQ;
 
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kg = wave % NG;
-  const int hkv = w.h, kb0 = w.blk * BK, j0 = kb0 + kg * 32, j = j0 + (lane & 31), jc = min(j, w.lk - 1);
+  const PackedHeads hd(p, w.h);
+  const int hkv = hd.hkv, kb0 = w.blk * BK, j0 = kb0 + kg * 32, j = j0 + (lane & 31), jc = min(j, w.lk - 1);
   const int off = w.lk - w.lq;
   const Span qspan = w.rows_of(j);
 
   int qt_lo, qt_hi;
   bwd_query_tiles(kb0, BK, w.lq, w.lk, w.dlo, w.dhi, BQ, qt_lo, qt_hi);
   qt_lo = __builtin_amdgcn_readfirstlane(qt_lo), qt_hi = __builtin_amdgcn_readfirstlane(qt_hi);
-  const int n_items = qt_hi > qt_lo ? p.G * (qt_hi - qt_lo) : 0;
+  const int n_items = qt_hi > qt_lo ? (hd.gh1 - hd.gh0) * (qt_hi - qt_lo) : 0;
   struct Item {
     int gh, qt;  // head of the group, query tile
   };
@@ -89,8 +93,8 @@ __device__ __forceinline__ void packed_dkdv_body(const PackedParams& p, const Pa
   auto load_item = [&](Item it, auto slot_c) __attribute__((always_inline)) {
     constexpr int SL = decltype(slot_c)::value;
     const int hq = hkv * p.G + it.gh, i0 = it.qt * BQ;
-    load_rows((const uint16_t*)p.q + (int64_t)w.q0 * p.q_ss + hq * p.q_sh, p.q_ss, lds_q + SL * L::kQ, i0);
-    load_rows((const uint16_t*)p.dout + (int64_t)w.q0 * p.do_ss + hq * p.do_sh, p.do_ss, lds_o + SL * L::kQ, i0);
+    load_rows((const uint16_t*)p.q + (int64_t)w.q0 * p.q_ss + hq * p.q_sh, p.q_ss, lds_q + SL * L::kTile, i0);
+    load_rows((const uint16_t*)p.dout + (int64_t)w.q0 * p.do_ss + hq * p.do_sh, p.do_ss, lds_o + SL * L::kTile, i0);
     if (wave == 0 && lane < BQ) {
       const int64_t at = (int64_t)hq * p.Tq + w.q0 + min(i0 + lane, w.lq - 1);
       lse_pend = p.lse[at];
@@ -108,8 +112,8 @@ __device__ __forceinline__ void packed_dkdv_body(const PackedParams& p, const Pa
     }
   };
   const Tile16Reader<D> rd(lane, 0);
-  auto p_slot = [&](int ps, int st, int vq) __attribute__((always_inline)) {
-    return (f32x4_t*)(lds_p + ps * L::kP) + ((kg * NST + st) * 4 + vq) * 64 + lane;
+  auto p_slot = [&](int ps, int vq) __attribute__((always_inline)) {
+    return (f32x4_t*)(lds_p + ps * L::kP) + (kg * 4 + vq) * 64 + lane;
   };
 
   // One of the pair: operand rows, the step loop, the epilogue.  Both run the same
@@ -174,66 +178,60 @@ __device__ __forceinline__ void packed_dkdv_body(const PackedParams& p, const Pa
     auto stage_a = [&](Item it, auto sl_c, auto ps_c) __attribute__((always_inline)) {
       constexpr int SL = decltype(sl_c)::value, PS = decltype(ps_c)::value;
       const int hq = hkv * p.G + it.gh;
+      const int i0 = it.qt * BQ;
+      if (!w.live(i0, 32, j0, 32)) return;
+      const char *q = lds_q + SL * L::kTile, *o = lds_o + SL * L::kTile;
+      const float* l = lds_l + SL * BQ;
+      __builtin_amdgcn_s_setprio(1);
+      const f32x16_t s = scores(q);
+      u32x4_t t0[TPF];
 #pragma unroll
-      for (int st = 0; st < NST; ++st) {
-        const int i0 = it.qt * BQ + st * 32;
-        if (!w.live(i0, 32, j0, 32)) continue;
-        const char *q = lds_q + SL * L::kQ + st * 32 * D * 2, *o = lds_o + SL * L::kQ + st * 32 * D * 2;
-        const float* l = lds_l + SL * BQ + st * 32;
-        __builtin_amdgcn_s_setprio(1);
-        const f32x16_t s = scores(q);
-        u32x4_t t0[TPF];
+      for (int m = 0; m < TPF; ++m) t0[m] = rd.tr(o, m / 2, m % 2);
+      __builtin_amdgcn_s_setprio(0);
+      float x[16];
 #pragma unroll
-        for (int m = 0; m < TPF; ++m) t0[m] = rd.tr(o, m / 2, m % 2);
-        __builtin_amdgcn_s_setprio(0);
-        float x[16];
+      for (int vq = 0; vq < 4; ++vq) {
+        const f32x4_t l4 = *(const f32x4_t*)(l + vq * 8 + g * 4);
 #pragma unroll
-        for (int vq = 0; vq < 4; ++vq) {
-          const f32x4_t l4 = *(const f32x4_t*)(l + vq * 8 + g * 4);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[vq * 4 + e] = __builtin_fmaf(s[vq * 4 + e], p.scale_log2, -l4[e]);
-        }
-        if (p.alibi) {
-          const float slope_l2 = -p.alibi[hq * p.al_sh] * kLog2e;
-          const float fj = (float)(j - off - (i0 + g * 4));
-#pragma unroll
-          for (int v = 0; v < 16; ++v) x[v] = __builtin_fmaf(fabsf(fj - (float)((v >> 2) * 8 + (v & 3))), slope_l2, x[v]);
-        }
-        if (!w.full(i0, 32, j0, 32)) {
-#pragma unroll
-          for (int v = 0; v < 16; ++v) x[v] = qspan.ok(i0 + (v >> 2) * 8 + g * 4 + (v & 3)) ? x[v] : -INFINITY;
-        }
-#pragma unroll
-        for (int v = 0; v < 16; ++v) x[v] = __builtin_amdgcn_exp2f(x[v]);
-#pragma unroll
-        for (int vq = 0; vq < 4; ++vq) *p_slot(PS, st, vq) = (f32x4_t){x[vq * 4], x[vq * 4 + 1], x[vq * 4 + 2], x[vq * 4 + 3]};
-        grad(o, x, t0);
+        for (int e = 0; e < 4; ++e) x[vq * 4 + e] = __builtin_fmaf(s[vq * 4 + e], p.scale_log2, -l4[e]);
       }
+      if (p.alibi) {
+        const float slope_l2 = -p.alibi[hq * p.al_sh] * kLog2e;
+        const float fj = (float)(j - off - (i0 + g * 4));
+#pragma unroll
+        for (int v = 0; v < 16; ++v) x[v] = __builtin_fmaf(fabsf(fj - (float)((v >> 2) * 8 + (v & 3))), slope_l2, x[v]);
+      }
+      if (!w.full(i0, 32, j0, 32)) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v) x[v] = qspan.ok(i0 + (v >> 2) * 8 + g * 4 + (v & 3)) ? x[v] : -INFINITY;
+      }
+#pragma unroll
+      for (int v = 0; v < 16; ++v) x[v] = __builtin_amdgcn_exp2f(x[v]);
+#pragma unroll
+      for (int vq = 0; vq < 4; ++vq) *p_slot(PS, vq) = (f32x4_t){x[vq * 4], x[vq * 4 + 1], x[vq * 4 + 2], x[vq * 4 + 3]};
+      grad(o, x, t0);
     };
     auto stage_b = [&](Item it, auto sl_c, auto ps_c) __attribute__((always_inline)) {
       constexpr int SL = decltype(sl_c)::value, PS = decltype(ps_c)::value;
+      const int i0 = it.qt * BQ;
+      if (!w.live(i0, 32, j0, 32)) return;  // (as the first of the pair: P was written)
+      const char *q = lds_q + SL * L::kTile, *o = lds_o + SL * L::kTile;
+      const float* dl = lds_d + SL * BQ;
+      __builtin_amdgcn_s_setprio(1);
+      const f32x16_t dp = scores(o);
+      u32x4_t t0[TPF];
 #pragma unroll
-      for (int st = 0; st < NST; ++st) {
-        const int i0 = it.qt * BQ + st * 32;
-        if (!w.live(i0, 32, j0, 32)) continue;  // (as the first of the pair: P was written)
-        const char *q = lds_q + SL * L::kQ + st * 32 * D * 2, *o = lds_o + SL * L::kQ + st * 32 * D * 2;
-        const float* dl = lds_d + SL * BQ + st * 32;
-        __builtin_amdgcn_s_setprio(1);
-        const f32x16_t dp = scores(o);
-        u32x4_t t0[TPF];
+      for (int m = 0; m < TPF; ++m) t0[m] = rd.tr(q, m / 2, m % 2);
+      __builtin_amdgcn_s_setprio(0);
+      float z[16];
 #pragma unroll
-        for (int m = 0; m < TPF; ++m) t0[m] = rd.tr(q, m / 2, m % 2);
-        __builtin_amdgcn_s_setprio(0);
-        float z[16];
+      for (int vq = 0; vq < 4; ++vq) {
+        const f32x4_t p4 = *p_slot(PS, vq), d4 = *(const f32x4_t*)(dl + vq * 8 + g * 4);
 #pragma unroll
-        for (int vq = 0; vq < 4; ++vq) {
-          const f32x4_t p4 = *p_slot(PS, st, vq), d4 = *(const f32x4_t*)(dl + vq * 8 + g * 4);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) z[vq * 4 + e] = p4[e] * (dp[vq * 4 + e] - d4[e]);
-        }
-        zs.apply(z, acc);
-        grad(q, z, t0);
+        for (int e = 0; e < 4; ++e) z[vq * 4 + e] = p4[e] * (dp[vq * 4 + e] - d4[e]);
       }
+      zs.apply(z, acc);
+      grad(q, z, t0);
     };
     // Step s: the first on item s (tile slot s % 3, P slot s % 2), the second on item s
     // - 1, item s + 1 loading into slot (s + 1) % 3.  The barrier at its top is where
@@ -241,7 +239,7 @@ __device__ __forceinline__ void packed_dkdv_body(const PackedParams& p, const Pa
     using I0 = std::integral_constant<int, 0>;
     using I1 = std::integral_constant<int, 1>;
     using I2 = std::integral_constant<int, 2>;
-    Item ia{0, qt_lo}, ib{0, qt_lo};
+    Item ia{hd.gh0, qt_lo}, ib = ia;
     if (n_items > 0) load_item(ia, I0{});
     write_rows();
     auto step = [&](auto sa_c, auto pa_c, int s) __attribute__((always_inline)) {
@@ -271,6 +269,16 @@ __device__ __forceinline__ void packed_dkdv_body(const PackedParams& p, const Pa
     uint16_t* row = SB ? (uint16_t*)p.dk + (int64_t)(w.k0 + j) * p.dk_ss + hkv * p.dk_sh
                        : (uint16_t*)p.dv + (int64_t)(w.k0 + j) * p.dv_ss + hkv * p.dv_sh;
     const float f = exp2f(-O::kPShift) * (SB ? p.scale * zs.undo() : 1.f);
+    if (p.n_split > 1) {
+      float* part = packed_partial(p, hd.split, SB ? 1 : 0, w.k0 + j, hkv, D);
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int vq = 0; vq < 4; ++vq)
+          *(f32x4_t*)(part + db * 32 + vq * 8 + g * 4) =
+              (f32x4_t){acc[db][vq * 4] * f, acc[db][vq * 4 + 1] * f, acc[db][vq * 4 + 2] * f, acc[db][vq * 4 + 3] * f};
+      return;
+    }
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -282,16 +290,16 @@ __device__ __forceinline__ void packed_dkdv_body(const PackedParams& p, const Pa
   else run(std::false_type{});
 }
 
-template <class E, int D, int KS>
+template <class E, int D>
 __device__ __forceinline__ void packed_dq_body(const PackedParams& p, const PackedBlock& w, char* pool) {
   using O = Ops16<E, D>;
   using L = PackedBwdLds<D>;
-  constexpr int NW = 8, BM = NW * 32 / KS, DB = D / 32, TILE = kTileRows * D * 2, NT = L::KT * KS;  // tiles per step
+  constexpr int NG = L::NG, BM = NG * 64, DB = D / 32, TILE = kTileRows * D * 2, NT = L::KT;  // tiles per step
   char* const lds_k = pool;
   char* const lds_v = pool + 2 * NT * TILE;
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, g = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kp = wave % KS;
-  const int hq = w.h, hkv = hq / p.G, m0 = w.blk * BM, iw0 = m0 + wave / KS * 32, i = iw0 + r, ic = min(i, w.lq - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int hq = w.h, hkv = hq / p.G, m0 = w.blk * BM, iw0 = m0 + wave * 32, i = iw0 + r, ic = min(i, w.lq - 1);
   const int off = w.lk - w.lq;
 
   const O ops(lane, 0);
@@ -308,12 +316,12 @@ __device__ __forceinline__ void packed_dq_body(const PackedParams& p, const Pack
   int t_lo, t_hi;
   bwd_key_tiles(m0, BM, w.lq, w.lk, w.dlo, w.dhi, kTileRows, t_lo, t_hi);
   t_lo = __builtin_amdgcn_readfirstlane(t_lo), t_hi = __builtin_amdgcn_readfirstlane(t_hi);
-  // the first four wavefronts copy K, the others V
-  const bool cv = wave >= 4;
+  // half of the wavefronts copy K, the others V
+  const bool cv = wave >= NG;
   const int64_t css = cv ? p.v_ss : p.k_ss;
   const uint16_t* cbase = cv ? (const uint16_t*)p.v + (int64_t)w.k0 * p.v_ss + hkv * p.v_sh
                              : (const uint16_t*)p.k + (int64_t)w.k0 * p.k_ss + hkv * p.k_sh;
-  const TileCopy<O, 4> copy(css, wave % 4, lane);
+  const TileCopy<O, NG> copy(css, wave % NG, lane);
   auto load = [&](int t, int slot) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < NT; ++u)
@@ -349,44 +357,21 @@ __device__ __forceinline__ void packed_dq_body(const PackedParams& p, const Pack
     __builtin_amdgcn_s_setprio(0);
   };
   if (t_lo < t_hi) load(t_lo, 0);
-  // step: NT tiles from one slot while the next land in the other; KS = 2: this
-  // wavefront takes every second one
+  // step: NT tiles from one slot while the next land in the other
   auto step = [&](auto slot_c, int t) __attribute__((always_inline)) {
     constexpr int SL = decltype(slot_c)::value;
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
     if (t + NT < t_hi) load(t + NT, 1 - SL);
 #pragma unroll
-    for (int u = 0; u < L::KT; ++u) {
-      const int k = u * KS + kp;
-      if (t + k < t_hi) block(t + k, lds_k + (SL * NT + k) * TILE, lds_v + (SL * NT + k) * TILE);
-    }
+    for (int u = 0; u < NT; ++u)
+      if (t + u < t_hi) block(t + u, lds_k + (SL * NT + u) * TILE, lds_v + (SL * NT + u) * TILE);
   };
   for (int t = t_lo; t < t_hi; t += 2 * NT) {
     step(std::integral_constant<int, 0>{}, t);
     if (t + NT < t_hi) step(std::integral_constant<int, 1>{}, t + NT);
   }
-  float f = p.scale * zs.undo();
-  if constexpr (KS == 2) {
-    // the second of a pair hands its sums over, four groups (merge_pair holds two)
-    constexpr int HB = DB;
-    static_assert(4 * HB * 4096 <= L::kBytes, "exchange");
-    float* x = (float*)pool + (wave / 2) * HB * 16 * 64 + lane;
-    __syncthreads();
-    if (kp == 1) {
-#pragma unroll
-      for (int db = 0; db < DB; ++db)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) x[(db * 16 + v) * 64] = acc[db][v] * f;
-    }
-    __syncthreads();
-    if (kp == 1) return;
-#pragma unroll
-    for (int db = 0; db < DB; ++db)
-#pragma unroll
-      for (int v = 0; v < 16; ++v) acc[db][v] = __builtin_fmaf(acc[db][v], f, x[(db * 16 + v) * 64]);
-    f = 1.f;
-  }
+  const float f = p.scale * zs.undo();
   if (i >= w.lq) return;
   uint16_t* row = (uint16_t*)p.dq + (int64_t)(w.q0 + i) * p.dq_ss + hq * p.dq_sh;
 #pragma unroll
@@ -398,27 +383,24 @@ __device__ __forceinline__ void packed_dq_body(const PackedParams& p, const Pack
 }
 
 // Workgroups [0, n_kv): dK and dV of p.items; behind them dQ of p.items_q.
-template <class E, int D, int KS>
-__global__ __launch_bounds__(512, 2) void packed_bwd16(const PackedParams p, int n_kv) {
+template <class E, int D>
+__global__ __launch_bounds__(256, 2) void packed_bwd16(const PackedParams p, int n_kv) {
   __shared__ __attribute__((aligned(1024))) char pool[PackedBwdLds<D>::kBytes];
   const int wg = (int)blockIdx.x;
   if (wg < n_kv) {
-    const PackedBlock w(p, p.items, wg, p.Hkv, 1);
+    const PackedBlock w(p, p.items, wg, p.Hkv * p.n_split, 1);
     if (w.blk >= 0) packed_dkdv_body<E, D>(p, w, pool);
   } else {
     const PackedBlock w(p, p.items_q, wg - n_kv, p.Hkv, p.G);
-    if (w.blk >= 0) packed_dq_body<E, D, KS>(p, w, pool);
+    if (w.blk >= 0) packed_dq_body<E, D>(p, w, pool);
   }
 }
 
 template <class E>
-hipError_t launch_packed_bwd16(const PackedParams& p, int D, int ks, int n_kv, int n_q, hipStream_t st) {
-  const dim3 grid((unsigned)(n_kv + n_q)), block(512);
-  if (D == 64)
-    return ks == 2 ? launch_kernel(&packed_bwd16<E, 64, 2>, grid, block, 0, st, p, n_kv)
-                   : launch_kernel(&packed_bwd16<E, 64, 1>, grid, block, 0, st, p, n_kv);
-  return ks == 2 ? launch_kernel(&packed_bwd16<E, 128, 2>, grid, block, 0, st, p, n_kv)
-                 : launch_kernel(&packed_bwd16<E, 128, 1>, grid, block, 0, st, p, n_kv);
+hipError_t launch_packed_bwd16(const PackedParams& p, int D, int n_kv, int n_q, hipStream_t st) {
+  const dim3 grid((unsigned)(n_kv + n_q)), block(256);
+  return D == 64 ? launch_kernel(&packed_bwd16<E, 64>, grid, block, 0, st, p, n_kv)
+                 : launch_kernel(&packed_bwd16<E, 128>, grid, block, 0, st, p, n_kv);
 }
 
 }  // namespace trinix

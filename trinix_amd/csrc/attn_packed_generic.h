@@ -136,11 +136,12 @@ __global__ __launch_bounds__(256, OCC) void packed_dkdv_generic(const PackedPara
   __shared__ __attribute__((aligned(128))) float lds_l[2][kTileRows];
   __shared__ __attribute__((aligned(128))) float lds_d[2][kTileRows];
   // HS workgroups share a key block, each summing D / HS of the columns
-  const PackedBlock w(p, p.items, (int)blockIdx.x / HS, p.Hkv, 1);
+  const PackedBlock w(p, p.items, (int)blockIdx.x / HS, p.Hkv * p.n_split, 1);
   if (w.blk < 0) return;
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int hkv = w.h, kb0 = w.blk * BK, db0 = ((int)blockIdx.x % HS) * DB;
+  const PackedHeads hd(p, w.h);
+  const int hkv = hd.hkv, kb0 = w.blk * BK, db0 = ((int)blockIdx.x % HS) * DB;
   const int j0 = kb0 + wave * 32, j = j0 + (lane & 31), jc = min(j, w.lk - 1);
   const bool wide = p.rows16 != 0;
   const int off = w.lk - w.lq;
@@ -148,7 +149,7 @@ __global__ __launch_bounds__(256, OCC) void packed_dkdv_generic(const PackedPara
   int qt_lo, qt_hi;
   bwd_query_tiles(kb0, BK, w.lq, w.lk, w.dlo, w.dhi, kTileRows, qt_lo, qt_hi);
   const int nqt = qt_hi - qt_lo;
-  const int n_items = nqt > 0 ? p.G * nqt : 0;  // item = (q-head of the group, query tile)
+  const int n_items = nqt > 0 ? (hd.gh1 - hd.gh0) * nqt : 0;  // item = (q-head of the group, query tile)
 
   const O ops(lane, db0);
   const typename O::Frag kf = O::load_frag((const Store*)p.k + (int64_t)(w.k0 + jc) * p.k_ss + hkv * p.k_sh, g);
@@ -161,7 +162,7 @@ __global__ __launch_bounds__(256, OCC) void packed_dkdv_generic(const PackedPara
   const TileCopy<O, NW> copy_q(p.q_ss, wave, lane), copy_o(p.do_ss, wave, lane);
   float lse_next = 0.f, del_next = 0.f;
   auto load_item = [&](int it, int slot) __attribute__((always_inline)) {
-    const int hq = hkv * p.G + it / nqt, i0 = (qt_lo + it % nqt) * kTileRows;
+    const int hq = hkv * p.G + hd.gh0 + it / nqt, i0 = (qt_lo + it % nqt) * kTileRows;
     copy_q((const Store*)p.q + (int64_t)w.q0 * p.q_ss + hq * p.q_sh, i0, w.lq, lds_q[slot], wide);
     copy_o((const Store*)p.dout + (int64_t)w.q0 * p.do_ss + hq * p.do_sh, i0, w.lq, lds_o[slot], wide);
     if (tid < kTileRows) {
@@ -179,7 +180,7 @@ __global__ __launch_bounds__(256, OCC) void packed_dkdv_generic(const PackedPara
     }
   };
   auto block = [&](int it, int slot) __attribute__((always_inline)) {
-    const int hq = hkv * p.G + it / nqt, i0 = (qt_lo + it % nqt) * kTileRows;
+    const int hq = hkv * p.G + hd.gh0 + it / nqt, i0 = (qt_lo + it % nqt) * kTileRows;
     if (!w.live(i0, 32, j0, 32)) return;
     const f32x16_t s = ops.scores(lds_q[slot], kf);
     float x[16];
@@ -235,6 +236,19 @@ __global__ __launch_bounds__(256, OCC) void packed_dkdv_generic(const PackedPara
 
   if (j >= w.lk) return;
   const float fv = exp2f(-O::kPShift), fk = p.scale * fv * zs.undo();
+  if (p.n_split > 1) {
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int vq = 0; vq < 4; ++vq) {
+        const int d0 = (db0 + db) * 32 + vq * 8 + g * 4;
+        *(f32x4_t*)(packed_partial(p, hd.split, 0, w.k0 + j, hkv, D) + d0) =
+            (f32x4_t){dv[db][vq * 4] * fv, dv[db][vq * 4 + 1] * fv, dv[db][vq * 4 + 2] * fv, dv[db][vq * 4 + 3] * fv};
+        *(f32x4_t*)(packed_partial(p, hd.split, 1, w.k0 + j, hkv, D) + d0) =
+            (f32x4_t){dk[db][vq * 4] * fk, dk[db][vq * 4 + 1] * fk, dk[db][vq * 4 + 2] * fk, dk[db][vq * 4 + 3] * fk};
+      }
+    return;
+  }
   Store* krow = (Store*)p.dk + (int64_t)(w.k0 + j) * p.dk_ss + hkv * p.dk_sh;
   Store* vrow = (Store*)p.dv + (int64_t)(w.k0 + j) * p.dv_ss + hkv * p.dv_sh;
 #pragma unroll

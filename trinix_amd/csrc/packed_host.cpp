@@ -57,11 +57,29 @@ int validate_packed(const trinix_packed_args* a, bool backward) {
       const int rc = check_rows(t.ptr, t.st, t.rows, f32);
       if (rc != TRINIX_OK) return rc;
     }
+    const int64_t ws = packed_partial_bytes(a);
+    if (ws > 0 && (!a->workspace || a->workspace_bytes < ws || ((uintptr_t)a->workspace & 15) != 0))
+      return TRINIX_ERR_BAD_ARGUMENT;
     if (a->total_q > 0 && (!a->lse || !a->delta || (!f32 && !a->out_lo))) return TRINIX_ERR_NULL_POINTER;
   }
   if (((uintptr_t)a->lse & 3) != 0 || ((uintptr_t)a->delta & 3) != 0 || ((uintptr_t)a->alibi_slopes & 3) != 0)
     return TRINIX_ERR_BAD_STRIDE;
   return TRINIX_OK;
+}
+
+// dK and dV of a KV head walk the query heads of its group one after the other; with
+// few key blocks that leaves CUs idle and one long chain.  Their heads then go over as
+// many workgroups as give 256, whose fp32 partial sums are added in order.
+int packed_head_splits(const trinix_packed_args* a) {
+  const int64_t G = a->nheads_q / a->nheads_kv, blocks = lmax(1, a->total_k / 128 + lmin(a->n_seqs, a->total_k) / 2);
+  int64_t n = lmin(G, 256 / (blocks * a->nheads_kv));
+  if (const char* env = getenv("TRINIX_PACKED_SPLITS")) n = lmin(G, atoi(env));  // (tuning and tests)
+  const int64_t per = (G + lmax(1, n) - 1) / lmax(1, n);  // heads of the longest chain
+  return (int)((G + per - 1) / per);
+}
+int64_t packed_partial_bytes(const trinix_packed_args* a) {
+  const int n = packed_head_splits(a);
+  return n > 1 ? 2ll * n * a->total_k * a->nheads_kv * a->head_dim * 4 : 0;
 }
 
 namespace {
@@ -156,6 +174,15 @@ int plan_shared(const trinix_shared_prefix_args* a, SharedPlan* pl) {
 }  // namespace trinix
 
 using namespace trinix;
+
+extern "C" int trinix_packed_bwd_workspace(const trinix_packed_args* a, int64_t* bytes) {
+  if (!a || !bytes) return TRINIX_ERR_NULL_POINTER;
+  if (a->nheads_q <= 0 || a->nheads_kv <= 0 || a->nheads_q > (1 << 20) || a->nheads_q % a->nheads_kv != 0 || a->n_seqs < 1 ||
+      a->total_k < 0 || a->total_k >= (1ll << 30) || (a->head_dim != 64 && a->head_dim != 128 && a->head_dim != 256))
+    return TRINIX_ERR_BAD_SHAPE;
+  *bytes = packed_partial_bytes(a);
+  return TRINIX_OK;
+}
 
 extern "C" int trinix_shared_prefix_workspace(const trinix_shared_prefix_args* a, int64_t* bytes) {
   if (!bytes) return TRINIX_ERR_NULL_POINTER;

@@ -9,6 +9,11 @@ namespace trinix {
 // TRINIX_OK or the status to return; no launch.  `backward`: the gradient
 // pointers and strides too.
 int validate_packed(const trinix_packed_args* a, bool backward);
+// Workgroups that share the query heads of a KV head in dK and dV (1: none), each
+// leaving fp32 partial sums of all keys.
+int packed_head_splits(const trinix_packed_args* a);
+// Bytes of those partial sums.
+int64_t packed_partial_bytes(const trinix_packed_args* a);
 
 
 // Attention behind a shared prefix: the same checks, and the launch plan.

@@ -265,6 +265,12 @@ class _PackedAttention(torch.autograd.Function):
         a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
         if slopes is not None:
             a.alibi_slopes = slopes.data_ptr()
+        n = ctypes.c_int64(0)
+        nat.check(nat.load_library().trinix_packed_bwd_workspace(ctypes.byref(a), ctypes.byref(n)),
+                  "trinix_packed_bwd_workspace")
+        if n.value:
+            ws = torch.empty(n.value, dtype=torch.uint8, device=q.device)
+            a.workspace, a.workspace_bytes = ws.data_ptr(), n.value
         _launch("trinix_packed_bwd", a, q.device)
         if q.shape[-1] != D:
             dq, dk, dv = dq[..., :D], dk[..., :D], dv[..., :D]
