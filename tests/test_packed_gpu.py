@@ -105,6 +105,16 @@ def test_heads_shared_out(splits, dtype, D, monkeypatch):
     check([70, 1, 0, 190], [90, 1, 7, 190], H=5, Hkv=1, D=D, dtype=dtype, pad=4)
 
 
+@pytest.mark.parametrize("pairs", ["1", "2"])
+@pytest.mark.parametrize("dtype,D", [(F32, 64), (F32, 128), (F32, 256), (BF, 256), (HF, 256)])
+def test_forced_pairs(pairs, dtype, D, monkeypatch):
+    # one or two wavefronts per 32 rows
+    monkeypatch.setenv("TRINIX_PACKED_PAIRS", pairs)
+    check([1, 257, 33, 0, 300, 128], D=D, dtype=dtype, pad=9)
+    check([200, 64, 3], [500, 64, 33], D=D, dtype=dtype, window=(150, 0))
+    check([300, 40], [10, 255], D=D, dtype=dtype, causal=False, alibi=True)
+
+
 def test_single_tokens_and_many_sequences():
     check([1] * 300, D=64, seed=2)
     check([(7 * i) % 23 for i in range(1500)], H=2, Hkv=1, D=64, seed=2)

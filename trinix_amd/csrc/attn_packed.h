@@ -98,14 +98,14 @@ enum class PackedShape { kPair, kPlain, kWide };
 // size of the item list that p.items points at.
 hipError_t launch_packed_fwd_bf16(const PackedParams& p, int D, PackedShape shape, int grid, hipStream_t st);
 hipError_t launch_packed_fwd_f16(const PackedParams& p, int D, PackedShape shape, int grid, hipStream_t st);
-hipError_t launch_packed_fwd_f32(const PackedParams& p, int D, PackedShape shape, int grid, hipStream_t st);
+hipError_t launch_packed_fwd_f32(const PackedParams& p, int D, int ks, int grid, hipStream_t st);
 // dK and dV, and dQ (16-bit: head_dim 256; 64 and 128 run both in one launch).
-hipError_t launch_packed_dkdv_bf16(const PackedParams& p, int grid, hipStream_t st);
-hipError_t launch_packed_dkdv_f16(const PackedParams& p, int grid, hipStream_t st);
-hipError_t launch_packed_dkdv_f32(const PackedParams& p, int D, int grid, hipStream_t st);
-hipError_t launch_packed_dq_bf16(const PackedParams& p, int grid, hipStream_t st);
-hipError_t launch_packed_dq_f16(const PackedParams& p, int grid, hipStream_t st);
-hipError_t launch_packed_dq_f32(const PackedParams& p, int D, int grid, hipStream_t st);
+hipError_t launch_packed_dkdv_bf16(const PackedParams& p, int ks, int grid, hipStream_t st);
+hipError_t launch_packed_dkdv_f16(const PackedParams& p, int ks, int grid, hipStream_t st);
+hipError_t launch_packed_dkdv_f32(const PackedParams& p, int D, int ks, int grid, hipStream_t st);
+hipError_t launch_packed_dq_bf16(const PackedParams& p, int ks, int grid, hipStream_t st);
+hipError_t launch_packed_dq_f16(const PackedParams& p, int ks, int grid, hipStream_t st);
+hipError_t launch_packed_dq_f32(const PackedParams& p, int D, int ks, int grid, hipStream_t st);
 hipError_t launch_packed_bwd_bf16(const PackedParams& p, int D, int n_kv, int n_q, hipStream_t st);
 hipError_t launch_packed_bwd_f16(const PackedParams& p, int D, int n_kv, int n_q, hipStream_t st);
 

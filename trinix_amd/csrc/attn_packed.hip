@@ -124,8 +124,8 @@ int64_t use_list(PackedParams& p, const trinix_packed_args* a, int list) {
   p.items = a->plan + packed_list_offset(list, a->total_q, a->total_k, a->n_seqs);
   return packed_list_cap(packed_list_is_keys(list) ? a->total_k : a->total_q, a->n_seqs, packed_list_block(list));
 }
-constexpr int kRows128 = 1, kRows256 = 2, kKeys64 = 3, kKeys128 = 4;
-constexpr int kListOf[3] = {0, kRows128, kRows256};  // of a PackedShape
+constexpr int kRows64 = 0, kRows128 = 1, kRows256 = 2, kKeys64 = 3, kKeys128 = 4;
+constexpr int kListOf[3] = {kRows64, kRows128, kRows256};  // of a PackedShape
 
 // Shape of the 16-bit forward.  The host knows the totals and the number of
 // sequences, not their lengths.  Measured, bf16 causal, graph-timed, us pair |
@@ -154,6 +154,25 @@ PackedShape packed_shape(const trinix_packed_args* a) {
   return s;
 }
 
+// Wavefronts per 32 rows (or keys) of the fp32 kernels and of the gradients at
+// head_dim 256; `chain`: heads that a block walks one after the other.  Measured,
+// forward and backward, us one | two:
+//  - fp32: two wins wherever blocks are few or sequences short (D=128 8 heads 1090 rows 321
+//    | 183; D=64 12 heads 4 x 1024 459 | 316, 24 x 100 99 | 82; 16/4 heads of 128 200 x 40 674
+//    | 482) and loses where long sequences fill the chip (D=64 16 heads 8 x 2048, 2112
+//    blocks, 2471 | 2541; even at 1560);
+//  - bf16 D=256, whose workgroup fills a CU either way: only chains worth halving (8/4
+//    heads 2048 + 1000 340 | 294; 16/4 4 x 1000: dK, dV in two 413 | 352, dQ as well 372; 8/4
+//    3 x 1000 201 | 206, 9 x 300 111 | 129).
+// TRINIX_PACKED_PAIRS = 1, 2 forces either (tuning and tests).
+int two_per_group(const trinix_packed_args* a, int64_t total, int64_t heads, int64_t chain) {
+  if (a->dtype == TRINIX_F32 && a->head_dim == 256) return 1;
+  if (const char* env = getenv("TRINIX_PACKED_PAIRS")) return atoi(env) == 1 ? 1 : 2;
+  const int64_t blocks = (total / 128 + lmin(a->n_seqs, total) / 2) * heads, keys = a->total_k / a->n_seqs;
+  if (a->dtype == TRINIX_F32) return blocks > 1536 && keys >= 1024 ? 1 : 2;
+  return blocks <= 384 && chain * keys >= 2500 ? 2 : 1;
+}
+
 }  // namespace
 }  // namespace trinix
 
@@ -166,13 +185,14 @@ extern "C" int trinix_packed_fwd(const trinix_packed_args* a, void* stream) {
   PackedParams p = params(a);
   hipStream_t st = (hipStream_t)stream;
   const int D = (int)a->head_dim;
-  const PackedShape shape = a->dtype == TRINIX_F32 ? PackedShape::kPlain : packed_shape(a);
-  const int grid = (int)(use_list(p, a, kListOf[(int)shape]) * p.Hq);
   hipError_t e;
   if (a->dtype == TRINIX_F32) {
     p.rows16 = rows16(a->k, a->k_stride) && rows16(a->v, a->v_stride);
-    e = launch_packed_fwd_f32(p, D, shape, grid, st);
+    const int ks = two_per_group(a, a->total_q, a->nheads_q, 1);
+    e = launch_packed_fwd_f32(p, D, ks, (int)(use_list(p, a, ks == 2 ? kRows64 : kRows128) * p.Hq), st);
   } else {
+    const PackedShape shape = packed_shape(a);
+    const int grid = (int)(use_list(p, a, kListOf[(int)shape]) * p.Hq);
     e = a->dtype == TRINIX_BF16 ? launch_packed_fwd_bf16(p, D, shape, grid, st) : launch_packed_fwd_f16(p, D, shape, grid, st);
   }
   return e == hipSuccess ? TRINIX_OK : TRINIX_ERR_LAUNCH;
@@ -202,14 +222,16 @@ extern "C" int trinix_packed_bwd(const trinix_packed_args* a, void* stream) {
       e = bf ? launch_packed_bwd_bf16(p, D, n_kv, n_q, st) : launch_packed_bwd_f16(p, D, n_kv, n_q, st);
   } else {
     if (a->total_k > 0) {
-      const int grid = (int)(use_list(p, a, kKeys128) * p.Hkv * p.n_split);
-      e = f32 ? launch_packed_dkdv_f32(p, D, grid, st) : bf ? launch_packed_dkdv_bf16(p, grid, st) : launch_packed_dkdv_f16(p, grid, st);
+      const int ks = two_per_group(a, a->total_k, a->nheads_kv * p.n_split, p.G / p.n_split);
+      const int grid = (int)(use_list(p, a, ks == 2 ? kKeys64 : kKeys128) * p.Hkv * p.n_split);
+      e = f32 ? launch_packed_dkdv_f32(p, D, ks, grid, st) : bf ? launch_packed_dkdv_bf16(p, ks, grid, st) : launch_packed_dkdv_f16(p, ks, grid, st);
       if (e != hipSuccess) return TRINIX_ERR_LAUNCH;
     }
     if (a->total_q > 0) {
       if (f32) p.rows16 = rows16(a->k, a->k_stride) && rows16(a->v, a->v_stride);
-      const int grid = (int)(use_list(p, a, kRows128) * p.Hq);
-      e = f32 ? launch_packed_dq_f32(p, D, grid, st) : bf ? launch_packed_dq_bf16(p, grid, st) : launch_packed_dq_f16(p, grid, st);
+      const int ks = two_per_group(a, a->total_q, a->nheads_q, 1);
+      const int grid = (int)(use_list(p, a, ks == 2 ? kRows64 : kRows128) * p.Hq);
+      e = f32 ? launch_packed_dq_f32(p, D, ks, grid, st) : bf ? launch_packed_dq_bf16(p, ks, grid, st) : launch_packed_dq_f16(p, ks, grid, st);
     }
   }
   if (e == hipSuccess && p.n_split > 1 && a->total_k > 0)

@@ -11,11 +11,13 @@ hipError_t launch_packed_fwd_f16(const PackedParams& p, int D, PackedShape shape
 hipError_t launch_packed_bwd_f16(const PackedParams& p, int D, int n_kv, int n_q, hipStream_t st) {
   return launch_packed_bwd16<F16>(p, D, n_kv, n_q, st);
 }
-hipError_t launch_packed_dkdv_f16(const PackedParams& p, int grid, hipStream_t st) {
-  return launch_packed_dkdv_g<Ops16<F16, 256>, 1, 2>(p, grid, st);
+hipError_t launch_packed_dkdv_f16(const PackedParams& p, int ks, int grid, hipStream_t st) {
+  using O = Ops16<F16, 256>;
+  return ks == 2 ? launch_packed_dkdv_g<O, 1, 2, 2>(p, grid, st) : launch_packed_dkdv_g<O, 1, 2, 1>(p, grid, st);
 }
-hipError_t launch_packed_dq_f16(const PackedParams& p, int grid, hipStream_t st) {
-  return launch_packed_dq_g<Ops16<F16, 256>, 1, 2>(p, grid, st);
+hipError_t launch_packed_dq_f16(const PackedParams& p, int ks, int grid, hipStream_t st) {
+  using O = Ops16<F16, 256>;
+  return ks == 2 ? launch_packed_dq_g<O, 1, 1, 2>(p, grid, st) : launch_packed_dq_g<O, 1, 1, 1>(p, grid, st);
 }
 
 }  // namespace trinix

@@ -3,28 +3,37 @@
 
 namespace trinix {
 
-hipError_t launch_packed_fwd_f32(const PackedParams& p, int D, PackedShape, int grid, hipStream_t st) {
+// ks: wavefronts per 32 rows (keys); head_dim 256 (registers, LDS): 1
+hipError_t launch_packed_fwd_f32(const PackedParams& p, int D, int ks, int grid, hipStream_t st) {
   const dim3 g((unsigned)grid), b(256);
   switch (D) {
-    case 64: return launch_kernel(&packed_fwd_generic<Ops32<64>, BF16, 2>, g, b, 0, st, p);
-    case 128: return launch_kernel(&packed_fwd_generic<Ops32<128>, BF16, 1>, g, b, 0, st, p);
-    case 256: return launch_kernel(&packed_fwd_generic<Ops32<256>, BF16, 1>, g, b, 0, st, p);
+    case 64:
+      return ks == 2 ? launch_kernel(&packed_fwd_f32<Ops32<64>, 2, 2>, g, b, 0, st, p)
+                     : launch_kernel(&packed_fwd_f32<Ops32<64>, 2, 1>, g, b, 0, st, p);
+    case 128:
+      return ks == 2 ? launch_kernel(&packed_fwd_f32<Ops32<128>, 1, 2>, g, b, 0, st, p)
+                     : launch_kernel(&packed_fwd_f32<Ops32<128>, 1, 1>, g, b, 0, st, p);
+    case 256: return launch_kernel(&packed_fwd_f32<Ops32<256>, 1, 1>, g, b, 0, st, p);
   }
   return hipErrorNotSupported;
 }
-hipError_t launch_packed_dkdv_f32(const PackedParams& p, int D, int grid, hipStream_t st) {
+hipError_t launch_packed_dkdv_f32(const PackedParams& p, int D, int ks, int grid, hipStream_t st) {
   switch (D) {
-    case 64: return launch_packed_dkdv_g<Ops32<64>, 2, 1>(p, grid, st);
-    case 128: return launch_packed_dkdv_g<Ops32<128>, 1, 1>(p, grid, st);
-    case 256: return launch_packed_dkdv_g<Ops32<256>, 1, 4>(p, grid, st);  // as bwd_dkdv_generic: registers
+    case 64:
+      return ks == 2 ? launch_packed_dkdv_g<Ops32<64>, 2, 1, 2>(p, grid, st) : launch_packed_dkdv_g<Ops32<64>, 2, 1, 1>(p, grid, st);
+    case 128:
+      return ks == 2 ? launch_packed_dkdv_g<Ops32<128>, 1, 1, 2>(p, grid, st) : launch_packed_dkdv_g<Ops32<128>, 1, 1, 1>(p, grid, st);
+    case 256: return launch_packed_dkdv_g<Ops32<256>, 1, 4, 1>(p, grid, st);  // K and V rows fill the registers
   }
   return hipErrorNotSupported;
 }
-hipError_t launch_packed_dq_f32(const PackedParams& p, int D, int grid, hipStream_t st) {
+hipError_t launch_packed_dq_f32(const PackedParams& p, int D, int ks, int grid, hipStream_t st) {
   switch (D) {
-    case 64: return launch_packed_dq_g<Ops32<64>, 2, 1>(p, grid, st);
-    case 128: return launch_packed_dq_g<Ops32<128>, 1, 1>(p, grid, st);
-    case 256: return launch_packed_dq_g<Ops32<256>, 1, 2>(p, grid, st);
+    case 64:
+      return ks == 2 ? launch_packed_dq_g<Ops32<64>, 2, 1, 2>(p, grid, st) : launch_packed_dq_g<Ops32<64>, 2, 1, 1>(p, grid, st);
+    case 128:
+      return ks == 2 ? launch_packed_dq_g<Ops32<128>, 1, 1, 2>(p, grid, st) : launch_packed_dq_g<Ops32<128>, 1, 1, 1>(p, grid, st);
+    case 256: return launch_packed_dq_g<Ops32<256>, 1, 2, 1>(p, grid, st);
   }
   return hipErrorNotSupported;
 }

@@ -1,31 +1,35 @@
-// Packed-sequence attention on the operand policies of attn_ops.h (fp32 on fp32
-// matrix products, 16-bit types with their coefficients in two terms):
-//   packed_fwd_generic    128 query rows of one sequence and head, 32 per wavefront,
+// Packed-sequence attention on the operand policies of attn_ops.h: fp32 on fp32
+// matrix products, the gradients of 16-bit types at head_dim 256 with their
+// coefficients in two terms:
+//   packed_fwd_f32        128 query rows of one sequence and head, 32 per wavefront,
 //                         over 32-key tiles: S^T = K Q^T, online softmax, O^T += V^T P^T;
 //   packed_dkdv_generic   128 keys of one sequence and KV head, 32 per wavefront, over
 //                         32-row tiles of Q and dO of every head of the group:
 //                         dV += P^T dO, dZ = P (dO V^T - delta), dK += dZ^T Q;
 //   packed_dq_generic     128 query rows as in the forward: dQ += dZ K.
-// Tiles go global -> LDS asynchronously into two slots, one barrier per tile.
+// KS = 2: 64 of them, two wavefronts per 32 taking alternate tiles, joined through LDS
+// at the end: half the chain of tiles, which bounds small batches.  Tiles go global ->
+// LDS asynchronously into two slots, one barrier per step.
 #pragma once
 #include <cfloat>
 
+#include "attn_bwd_generic.h"
 #include "attn_ops.h"
 #include "attn_packed.h"
 
 namespace trinix {
 
-template <class O, class E, int OCC>
-__global__ __launch_bounds__(256, OCC) void packed_fwd_generic(const PackedParams p) {
+template <class O, int OCC, int KS>
+__global__ __launch_bounds__(256, OCC) void packed_fwd_f32(const PackedParams p) {
   using Store = typename O::Store;
-  constexpr int NW = 4, BM = NW * 32, D = O::kD, DB = D / 32, TILE = kTileRows * D * (int)sizeof(Store);
-  __shared__ __attribute__((aligned(1024))) char lds_k[2][TILE];
-  __shared__ __attribute__((aligned(1024))) char lds_v[2][TILE];
+  constexpr int NW = 4, BM = NW * 32 / KS, D = O::kD, DB = D / 32, TILE = kTileRows * D * (int)sizeof(Store);
+  __shared__ __attribute__((aligned(1024))) char lds_k[2][KS * TILE];
+  __shared__ __attribute__((aligned(1024))) char lds_v[2][KS * TILE];
   const PackedBlock w(p, p.items, (int)blockIdx.x, p.Hkv, p.G);
   if (w.blk < 0) return;
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int hq = w.h, hkv = hq / p.G, m0 = w.blk * BM, iw0 = m0 + wave * 32, i = iw0 + r, ic = min(i, w.lq - 1);
+  const int hq = w.h, hkv = hq / p.G, m0 = w.blk * BM, kp = wave % KS, iw0 = m0 + wave / KS * 32, i = iw0 + r, ic = min(i, w.lq - 1);
   const bool wide = p.rows16 != 0;
 
   const O ops(lane, 0);
@@ -43,13 +47,17 @@ __global__ __launch_bounds__(256, OCC) void packed_fwd_generic(const PackedParam
   const Store* vbase = (const Store*)p.v + (int64_t)w.k0 * p.v_ss + hkv * p.v_sh;
   const TileCopy<O, NW> copy_k(p.k_ss, wave, lane), copy_v(p.v_ss, wave, lane);
   auto load = [&](int t, int slot) __attribute__((always_inline)) {
-    copy_k(kbase, t * kTileRows, w.lk, lds_k[slot], wide);
-    copy_v(vbase, t * kTileRows, w.lk, lds_v[slot], wide);
+#pragma unroll
+    for (int u = 0; u < KS; ++u)
+      if (t + u < t_hi) {
+        copy_k(kbase, (t + u) * kTileRows, w.lk, lds_k[slot] + u * TILE, wide);
+        copy_v(vbase, (t + u) * kTileRows, w.lk, lds_v[slot] + u * TILE, wide);
+      }
   };
   auto block = [&](int t, int slot) __attribute__((always_inline)) {
     const int n0 = t * kTileRows;
     if (!w.live(iw0, 32, n0, 32)) return;
-    const f32x16_t s = ops.scores(lds_k[slot], qf);
+    const f32x16_t s = ops.scores(lds_k[slot] + kp * TILE, qf);
     float x[16];
 #pragma unroll
     for (int v = 0; v < 16; ++v) x[v] = s[v] * p.scale_log2;
@@ -75,9 +83,7 @@ __global__ __launch_bounds__(256, OCC) void packed_fwd_generic(const PackedParam
       for (int db = 0; db < DB; ++db) acc[db] *= alpha;
       m_run = m_new;
     }
-    // all keys so far hidden: exp2(-inf - 0) = 0.  P and l are held at
-    // 2^kPShift (attn_ops.h), which cancels in P / l
-    const float m_use = (m_run == -INFINITY ? 0.f : m_run) - O::kPShift;
+    const float m_use = m_run == -INFINITY ? 0.f : m_run;  // all keys so far hidden: exp2(-inf - 0) = 0
     float sum = 0.f;  // within the tile first: one rounding of the running sum per tile
 #pragma unroll
     for (int v = 0; v < 16; ++v) {
@@ -85,7 +91,7 @@ __global__ __launch_bounds__(256, OCC) void packed_fwd_generic(const PackedParam
       sum += x[v];
     }
     l_run += sum;
-    ops.accum(acc, lds_v[slot], x);
+    ops.accum(acc, lds_v[slot] + kp * TILE, x);
   };
 
   if (t_lo < t_hi) load(t_lo, 0);
@@ -93,15 +99,41 @@ __global__ __launch_bounds__(256, OCC) void packed_fwd_generic(const PackedParam
     constexpr int SL = decltype(slot_c)::value;
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    if (t + 1 < t_hi) load(t + 1, 1 - SL);
-    block(t, SL);
+    if (t + KS < t_hi) load(t + KS, 1 - SL);
+    if (t + kp < t_hi) block(t + kp, SL);
   };
-  for (int t = t_lo; t < t_hi; t += 2) {
+  for (int t = t_lo; t < t_hi; t += 2 * KS) {
     step(std::integral_constant<int, 0>{}, t);
-    if (t + 1 < t_hi) step(std::integral_constant<int, 1>{}, t + 1);
+    if (t + KS < t_hi) step(std::integral_constant<int, 1>{}, t + KS);
   }
 
-  const float l = xlane_sum(l_run);
+  float l = xlane_sum(l_run);
+  if constexpr (KS == 2) {
+    // the second wavefront's (max, sum, O) merge into the first's
+    constexpr int WORDS = DB * 16 + 2;
+    static_assert(2 * WORDS * 64 * 4 <= 2 * KS * TILE, "exchange fits the K tiles");
+    float* x = (float*)&lds_k[0][0] + wave / KS * WORDS * 64 + lane;
+    __syncthreads();
+    if (kp == 1) {
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) x[(db * 16 + v) * 64] = acc[db][v];
+      x[DB * 16 * 64] = m_run;
+      x[(DB * 16 + 1) * 64] = l;
+    }
+    __syncthreads();
+    if (kp == 1) return;
+    const float m1 = x[DB * 16 * 64], l1 = x[(DB * 16 + 1) * 64];
+    const float m_new = fmaxf(m_run, m1), m_use = m_new == -INFINITY ? 0.f : m_new;
+    const float a0 = __builtin_amdgcn_exp2f(m_run - m_use), a1 = __builtin_amdgcn_exp2f(m1 - m_use);
+    l = l * a0 + l1 * a1;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) acc[db][v] = acc[db][v] * a0 + x[(db * 16 + v) * 64] * a1;
+    m_run = m_new;
+  }
   if (i >= w.lq) return;
   const float inv = l > 0.f ? 1.f / l : 0.f;  // a row that sees no key: 0
   const int64_t row = w.q0 + i;
@@ -109,32 +141,20 @@ __global__ __launch_bounds__(256, OCC) void packed_fwd_generic(const PackedParam
 #pragma unroll
   for (int db = 0; db < DB; ++db)
 #pragma unroll
-    for (int vq = 0; vq < 4; ++vq) {
-      const int d0 = db * 32 + vq * 8 + g * 4;
-      float x[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = acc[db][vq * 4 + e] * inv;
-      O::store4(orow, d0, x[0], x[1], x[2], x[3]);
-      if constexpr (sizeof(Store) == 2) {
-        if (p.o_lo) {
-          constexpr float f = kLoScale<E>;
-          O::store4((Store*)p.o_lo + row * p.o_ss + hq * p.o_sh, d0, (x[0] - round_to<E>(x[0])) * f,
-                    (x[1] - round_to<E>(x[1])) * f, (x[2] - round_to<E>(x[2])) * f, (x[3] - round_to<E>(x[3])) * f);
-        }
-      }
-    }
-  if (p.lse && g == 0)
-    p.lse[(int64_t)hq * p.Tq + row] = l > 0.f ? (m_run - O::kPShift + log2f(l)) * kLn2 : -INFINITY;
+    for (int vq = 0; vq < 4; ++vq)
+      O::store4(orow, db * 32 + vq * 8 + g * 4, acc[db][vq * 4] * inv, acc[db][vq * 4 + 1] * inv, acc[db][vq * 4 + 2] * inv,
+                acc[db][vq * 4 + 3] * inv);
+  if (p.lse && g == 0) p.lse[(int64_t)hq * p.Tq + row] = l > 0.f ? (m_run + log2f(l)) * kLn2 : -INFINITY;
 }
 
-template <class O, int OCC, int HS>
+template <class O, int OCC, int HS, int KS>
 __global__ __launch_bounds__(256, OCC) void packed_dkdv_generic(const PackedParams p) {
   using Store = typename O::Store;
-  constexpr int NW = 4, BK = NW * 32, D = O::kD, DB = O::DB / HS, TILE = kTileRows * D * (int)sizeof(Store);
-  __shared__ __attribute__((aligned(1024))) char lds_q[2][TILE];
-  __shared__ __attribute__((aligned(1024))) char lds_o[2][TILE];
-  __shared__ __attribute__((aligned(128))) float lds_l[2][kTileRows];
-  __shared__ __attribute__((aligned(128))) float lds_d[2][kTileRows];
+  constexpr int NW = 4, BK = NW * 32 / KS, D = O::kD, DB = O::DB / HS, TILE = kTileRows * D * (int)sizeof(Store);
+  __shared__ __attribute__((aligned(1024))) char lds_q[2][KS * TILE];
+  __shared__ __attribute__((aligned(1024))) char lds_o[2][KS * TILE];
+  __shared__ __attribute__((aligned(128))) float lds_l[2][KS * kTileRows];
+  __shared__ __attribute__((aligned(128))) float lds_d[2][KS * kTileRows];
   // HS workgroups share a key block, each summing D / HS of the columns
   const PackedBlock w(p, p.items, (int)blockIdx.x / HS, p.Hkv * p.n_split, 1);
   if (w.blk < 0) return;
@@ -142,7 +162,7 @@ __global__ __launch_bounds__(256, OCC) void packed_dkdv_generic(const PackedPara
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const PackedHeads hd(p, w.h);
   const int hkv = hd.hkv, kb0 = w.blk * BK, db0 = ((int)blockIdx.x % HS) * DB;
-  const int j0 = kb0 + wave * 32, j = j0 + (lane & 31), jc = min(j, w.lk - 1);
+  const int kp = wave % KS, j0 = kb0 + wave / KS * 32, j = j0 + (lane & 31), jc = min(j, w.lk - 1);
   const bool wide = p.rows16 != 0;
   const int off = w.lk - w.lq;
 
@@ -161,20 +181,24 @@ __global__ __launch_bounds__(256, OCC) void packed_dkdv_generic(const PackedPara
 
   const TileCopy<O, NW> copy_q(p.q_ss, wave, lane), copy_o(p.do_ss, wave, lane);
   float lse_next = 0.f, del_next = 0.f;
-  auto load_item = [&](int it, int slot) __attribute__((always_inline)) {
-    const int hq = hkv * p.G + hd.gh0 + it / nqt, i0 = (qt_lo + it % nqt) * kTileRows;
-    copy_q((const Store*)p.q + (int64_t)w.q0 * p.q_ss + hq * p.q_sh, i0, w.lq, lds_q[slot], wide);
-    copy_o((const Store*)p.dout + (int64_t)w.q0 * p.do_ss + hq * p.do_sh, i0, w.lq, lds_o[slot], wide);
-    if (tid < kTileRows) {
-      const int64_t ro = (int64_t)hq * p.Tq + w.q0 + min(i0 + tid, w.lq - 1);
-      lse_next = p.lse[ro];
-      del_next = p.delta[ro];
+  auto load_step = [&](int it, int slot) __attribute__((always_inline)) {  // items it .. it + KS - 1
+#pragma unroll
+    for (int u = 0; u < KS; ++u) {
+      if (it + u >= n_items) break;
+      const int hq = hkv * p.G + hd.gh0 + (it + u) / nqt, i0 = (qt_lo + (it + u) % nqt) * kTileRows;
+      copy_q((const Store*)p.q + (int64_t)w.q0 * p.q_ss + hq * p.q_sh, i0, w.lq, lds_q[slot] + u * TILE, wide);
+      copy_o((const Store*)p.dout + (int64_t)w.q0 * p.do_ss + hq * p.do_sh, i0, w.lq, lds_o[slot] + u * TILE, wide);
+      if (tid / kTileRows == u) {
+        const int64_t ro = (int64_t)hq * p.Tq + w.q0 + min(i0 + tid % kTileRows, w.lq - 1);
+        lse_next = p.lse[ro];
+        del_next = p.delta[ro];
+      }
     }
   };
   // a row that sees no key has lse -inf and every score -inf: the finite floor
   // keeps exp2(score - lse) at 0 instead of exp2(-inf + inf) = NaN
   auto write_rows = [&](int slot) __attribute__((always_inline)) {
-    if (tid < kTileRows) {
+    if (tid < KS * kTileRows) {
       lds_l[slot][tid] = fmaxf(lse_next * kLog2e, -0.5f * FLT_MAX) - O::kPShift;
       lds_d[slot][tid] = del_next;
     }
@@ -182,11 +206,12 @@ __global__ __launch_bounds__(256, OCC) void packed_dkdv_generic(const PackedPara
   auto block = [&](int it, int slot) __attribute__((always_inline)) {
     const int hq = hkv * p.G + hd.gh0 + it / nqt, i0 = (qt_lo + it % nqt) * kTileRows;
     if (!w.live(i0, 32, j0, 32)) return;
-    const f32x16_t s = ops.scores(lds_q[slot], kf);
+    const char *q_lds = lds_q[slot] + kp * TILE, *o_lds = lds_o[slot] + kp * TILE;
+    const f32x16_t s = ops.scores(q_lds, kf);
     float x[16];
 #pragma unroll
     for (int vq = 0; vq < 4; ++vq) {
-      const f32x4_t l4 = *(const f32x4_t*)(&lds_l[slot][vq * 8 + g * 4]);
+      const f32x4_t l4 = *(const f32x4_t*)(&lds_l[slot][kp * kTileRows + vq * 8 + g * 4]);
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[vq * 4 + e] = __builtin_fmaf(s[vq * 4 + e], p.scale_log2, -l4[e]);
     }
@@ -205,37 +230,43 @@ __global__ __launch_bounds__(256, OCC) void packed_dkdv_generic(const PackedPara
     }
 #pragma unroll
     for (int v = 0; v < 16; ++v) x[v] = __builtin_amdgcn_exp2f(x[v]);
-    ops.accum(dv, lds_o[slot], x);
-    const f32x16_t dp = ops.scores(lds_o[slot], vf);
+    ops.accum(dv, o_lds, x);
+    const f32x16_t dp = ops.scores(o_lds, vf);
 #pragma unroll
     for (int vq = 0; vq < 4; ++vq) {
-      const f32x4_t d4 = *(const f32x4_t*)(&lds_d[slot][vq * 8 + g * 4]);
+      const f32x4_t d4 = *(const f32x4_t*)(&lds_d[slot][kp * kTileRows + vq * 8 + g * 4]);
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[vq * 4 + e] *= dp[vq * 4 + e] - d4[e];
     }
     zs.apply(x, dk);
-    ops.accum(dk, lds_q[slot], x);
+    ops.accum(dk, q_lds, x);
   };
 
   if (n_items > 0) {
-    load_item(0, 0);
+    load_step(0, 0);
     write_rows(0);
   }
   auto step = [&](auto slot_c, int it) __attribute__((always_inline)) {
     constexpr int SL = decltype(slot_c)::value;
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    if (it + 1 < n_items) load_item(it + 1, 1 - SL);
-    block(it, SL);
-    if (it + 1 < n_items) write_rows(1 - SL);
+    if (it + KS < n_items) load_step(it + KS, 1 - SL);
+    if (it + kp < n_items) block(it + kp, SL);
+    if (it + KS < n_items) write_rows(1 - SL);
   };
-  for (int it = 0; it < n_items; it += 2) {
+  for (int it = 0; it < n_items; it += 2 * KS) {
     step(std::integral_constant<int, 0>{}, it);
-    if (it + 1 < n_items) step(std::integral_constant<int, 1>{}, it + 1);
+    if (it + KS < n_items) step(std::integral_constant<int, 1>{}, it + KS);
   }
 
+  float fv = exp2f(-O::kPShift), fk = p.scale * fv * zs.undo();
+  if constexpr (KS == 2) {
+    merge_pair<2 * KS * TILE>(dv, fv, (float*)&lds_q[0][0], wave / KS, kp, lane);
+    merge_pair<2 * KS * TILE>(dk, fk, (float*)&lds_q[0][0], wave / KS, kp, lane);
+    if (kp == 1) return;
+    fv = fk = 1.f;
+  }
   if (j >= w.lk) return;
-  const float fv = exp2f(-O::kPShift), fk = p.scale * fv * zs.undo();
   if (p.n_split > 1) {
 #pragma unroll
     for (int db = 0; db < DB; ++db)
@@ -261,17 +292,17 @@ __global__ __launch_bounds__(256, OCC) void packed_dkdv_generic(const PackedPara
     }
 }
 
-template <class O, int OCC, int HS>
+template <class O, int OCC, int HS, int KS>
 __global__ __launch_bounds__(256, OCC) void packed_dq_generic(const PackedParams p) {
   using Store = typename O::Store;
-  constexpr int NW = 4, BM = NW * 32, D = O::kD, DB = O::DB / HS, TILE = kTileRows * D * (int)sizeof(Store);
-  __shared__ __attribute__((aligned(1024))) char lds_k[2][TILE];
-  __shared__ __attribute__((aligned(1024))) char lds_v[2][TILE];
+  constexpr int NW = 4, BM = NW * 32 / KS, D = O::kD, DB = O::DB / HS, TILE = kTileRows * D * (int)sizeof(Store);
+  __shared__ __attribute__((aligned(1024))) char lds_k[2][KS * TILE];
+  __shared__ __attribute__((aligned(1024))) char lds_v[2][KS * TILE];
   const PackedBlock w(p, p.items, (int)blockIdx.x / HS, p.Hkv, p.G);
   if (w.blk < 0) return;
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int hq = w.h, hkv = hq / p.G, m0 = w.blk * BM, iw0 = m0 + wave * 32, i = iw0 + r, ic = min(i, w.lq - 1);
+  const int hq = w.h, hkv = hq / p.G, m0 = w.blk * BM, kp = wave % KS, iw0 = m0 + wave / KS * 32, i = iw0 + r, ic = min(i, w.lq - 1);
   const int db0 = ((int)blockIdx.x % HS) * DB, off = w.lk - w.lq;
   const bool wide = p.rows16 != 0;
 
@@ -292,14 +323,18 @@ __global__ __launch_bounds__(256, OCC) void packed_dq_generic(const PackedParams
   const Store* vbase = (const Store*)p.v + (int64_t)w.k0 * p.v_ss + hkv * p.v_sh;
   const TileCopy<O, NW> copy_k(p.k_ss, wave, lane), copy_v(p.v_ss, wave, lane);
   auto load = [&](int t, int slot) __attribute__((always_inline)) {
-    copy_k(kbase, t * kTileRows, w.lk, lds_k[slot], wide);
-    copy_v(vbase, t * kTileRows, w.lk, lds_v[slot], wide);
+#pragma unroll
+    for (int u = 0; u < KS; ++u)
+      if (t + u < t_hi) {
+        copy_k(kbase, (t + u) * kTileRows, w.lk, lds_k[slot] + u * TILE, wide);
+        copy_v(vbase, (t + u) * kTileRows, w.lk, lds_v[slot] + u * TILE, wide);
+      }
   };
   auto block = [&](int t, int slot) __attribute__((always_inline)) {
     const int n0 = t * kTileRows;
     if (!w.live(iw0, 32, n0, 32)) return;
-    const f32x16_t s = ops.scores(lds_k[slot], qf);
-    const f32x16_t dp = ops.scores(lds_v[slot], of);
+    const f32x16_t s = ops.scores(lds_k[slot] + kp * TILE, qf);
+    const f32x16_t dp = ops.scores(lds_v[slot] + kp * TILE, of);
     float x[16];
 #pragma unroll
     for (int v = 0; v < 16; ++v) x[v] = __builtin_fmaf(s[v], p.scale_log2, -lse2);
@@ -318,7 +353,7 @@ __global__ __launch_bounds__(256, OCC) void packed_dq_generic(const PackedParams
 #pragma unroll
     for (int v = 0; v < 16; ++v) x[v] = __builtin_amdgcn_exp2f(x[v]) * (dp[v] - dlt);
     zs.apply(x, acc);
-    ops.accum(acc, lds_k[slot], x);
+    ops.accum(acc, lds_k[slot] + kp * TILE, x);
   };
 
   if (t_lo < t_hi) load(t_lo, 0);
@@ -326,16 +361,21 @@ __global__ __launch_bounds__(256, OCC) void packed_dq_generic(const PackedParams
     constexpr int SL = decltype(slot_c)::value;
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    if (t + 1 < t_hi) load(t + 1, 1 - SL);
-    block(t, SL);
+    if (t + KS < t_hi) load(t + KS, 1 - SL);
+    if (t + kp < t_hi) block(t + kp, SL);
   };
-  for (int t = t_lo; t < t_hi; t += 2) {
+  for (int t = t_lo; t < t_hi; t += 2 * KS) {
     step(std::integral_constant<int, 0>{}, t);
-    if (t + 1 < t_hi) step(std::integral_constant<int, 1>{}, t + 1);
+    if (t + KS < t_hi) step(std::integral_constant<int, 1>{}, t + KS);
   }
 
+  float f = p.scale * zs.undo();
+  if constexpr (KS == 2) {
+    merge_pair<2 * KS * TILE>(acc, f, (float*)&lds_k[0][0], wave / KS, kp, lane);
+    if (kp == 1) return;
+    f = 1.f;
+  }
   if (i >= w.lq) return;
-  const float f = p.scale * zs.undo();
   Store* row = (Store*)p.dq + (int64_t)(w.q0 + i) * p.dq_ss + hq * p.dq_sh;
 #pragma unroll
   for (int db = 0; db < DB; ++db)
@@ -346,13 +386,13 @@ __global__ __launch_bounds__(256, OCC) void packed_dq_generic(const PackedParams
     }
 }
 
-template <class O, int OCC, int HS>
+template <class O, int OCC, int HS, int KS>
 hipError_t launch_packed_dkdv_g(const PackedParams& p, int grid, hipStream_t st) {
-  return launch_kernel(&packed_dkdv_generic<O, OCC, HS>, dim3((unsigned)(grid * HS)), dim3(256), 0, st, p);
+  return launch_kernel(&packed_dkdv_generic<O, OCC, HS, KS>, dim3((unsigned)(grid * HS)), dim3(256), 0, st, p);
 }
-template <class O, int OCC, int HS>
+template <class O, int OCC, int HS, int KS>
 hipError_t launch_packed_dq_g(const PackedParams& p, int grid, hipStream_t st) {
-  return launch_kernel(&packed_dq_generic<O, OCC, HS>, dim3((unsigned)(grid * HS)), dim3(256), 0, st, p);
+  return launch_kernel(&packed_dq_generic<O, OCC, HS, KS>, dim3((unsigned)(grid * HS)), dim3(256), 0, st, p);
 }
 
 }  // namespace trinix
