@@ -6,7 +6,7 @@
 namespace trinix {
 
 // NW * 32 / KS query rows of one sequence and head (the list's block).
-template <class E, int D, int BN, int NW, int OCC, int KS, bool ALIBI>
+template <class E, int D, int BN, int NW, int OCC, int KS, int ALIBI>
 __global__ __launch_bounds__(NW * 64, OCC) void packed_fwd16(const PackedParams p) {
   constexpr int BM = NW * 32 / KS, DB = D / 32;
   TRINIX_TILE16_LDS(D, BN, KS);
@@ -58,8 +58,11 @@ __global__ __launch_bounds__(NW * 64, OCC) void packed_fwd16(const PackedParams 
 template <class E, int D, int BN, int NW, int OCC, int KS>
 hipError_t launch_packed_fwd16(const PackedParams& p, int grid, hipStream_t st) {
   const dim3 g((unsigned)grid), b(NW * 64);
-  if (p.alibi) return launch_kernel(&packed_fwd16<E, D, BN, NW, OCC, KS, true>, g, b, 0, st, p);
-  return launch_kernel(&packed_fwd16<E, D, BN, NW, OCC, KS, false>, g, b, 0, st, p);
+  if (!p.alibi) return launch_kernel(&packed_fwd16<E, D, BN, NW, OCC, KS, 0>, g, b, 0, st, p);
+  // (a causal row sees no key behind it; 128-key tiles and head_dim 256 have no registers for 2)
+  if constexpr (BN <= 64 && D <= 128)
+    if (p.causal) return launch_kernel(&packed_fwd16<E, D, BN, NW, OCC, KS, 2>, g, b, 0, st, p);
+  return launch_kernel(&packed_fwd16<E, D, BN, NW, OCC, KS, 1>, g, b, 0, st, p);
 }
 
 // 64-key tiles of 4 wavefronts, two per SIMD (head_dim 256: one); kPair at

@@ -50,7 +50,13 @@ struct KeyRun {
   int pos;
 };
 
-template <class E, int D, int BN, int NW, int KS, bool ALIBI>
+// ALIBI: 0 none; 1 -slope * |distance|, three instructions per score; 2 the same where
+// no key of a full tile lies behind a row (causal runs): linear in the key there, so
+// that the accumulators start at its part within the tile, which stays in registers (an
+// operand of the first product, no instruction of its own), and its part of the whole
+// tile joins the maximum in the exponential's FMA (32 heads of 128, ten ragged prompts of
+// 8326 rows: 144 us with 1, 135 with 2, 126 without ALiBi).
+template <class E, int D, int BN, int NW, int KS, int ALIBI>
 struct Tile16 {
   static constexpr int DS = D / 16;    // MFMA k-steps over head_dim
   static constexpr int NB = BN / 32;   // 32-key blocks per tile
@@ -59,9 +65,10 @@ struct Tile16 {
   static constexpr int LPW = BN * UPR / (64 * NW);  // copies per wavefront and tile (K or V)
   static constexpr float TAU = 8.f;
   static_assert(D % 64 == 0 && BN % 32 == 0 && BN * UPR % (64 * NW) == 0, "tile shape");
+  static constexpr int NQK = NB * DS, NPV = DB * NB * 2;  // MFMAs of a tile
   // operand reads ahead of their MFMA
-  static constexpr int KPF = D == 256 ? 2 : 6, VPF = D == 256 ? 2 : 4;
-  static constexpr int NQK = NB * DS, NPV = DB * NB * 2;
+  static constexpr int KPF = D == 256 ? 2 : (NQK < 6 ? NQK : 6), VPF = D == 256 ? 2 : 4;
+  static_assert(KPF <= NQK && VPF <= NPV, "reads ahead");
 
   uint16_t *k0, *k1, *v0, *v1;
   int lane, wave, r, g, kp;
@@ -70,6 +77,7 @@ struct Tile16 {
   u32x4_t qr[DS];
   f32x16_t acc[DB];  // O^T: element (db, 4 vq + e) is d = 32 db + 8 vq + 4 g + e of the lane's row
   float m_run, l_run, c, alibi_mul;
+  f32x16_t lin[ALIBI == 2 ? NB : 1];
 
   __device__ __forceinline__ Tile16(uint16_t* k0_, uint16_t* k1_, uint16_t* v0_, uint16_t* v1_)
       : k0(k0_), k1(k1_), v0(v0_), v1(v1_) {
@@ -98,7 +106,15 @@ struct Tile16 {
   __device__ __forceinline__ void load_q(const uint16_t* row, float scale_log2, float slope) {
     const bool neg = scale_log2 < 0.f, zero = scale_log2 == 0.f;
     c = neg ? -scale_log2 : (zero ? 1.f : scale_log2);
-    if constexpr (ALIBI) alibi_mul = -slope * kLog2e / c;
+    if constexpr (ALIBI != 0) alibi_mul = -slope * kLog2e / c;
+    if constexpr (ALIBI == 2) {
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v) lin[nb][v] = -alibi_mul * (float)(nb * 32 + (v >> 2) * 8 + (v & 3));
+        asm volatile("" : "+v"(lin[nb]));
+      }
+    }
     const uint32_t flip = neg ? 0x80008000u : 0u, keep = zero ? 0u : 0xffffffffu;
 #pragma unroll
     for (int ds = 0; ds < DS; ++ds) {
@@ -178,7 +194,8 @@ struct Tile16 {
     };
 
     // S^T of one tile; ALiBi starts the accumulators at bias / c
-    auto qk = [&](const uint16_t* kt, int n0, f32x16_t(&s)[NB]) __attribute__((always_inline)) {
+    auto qk = [&](auto edge, const uint16_t* kt, int n0, f32x16_t(&s)[NB]) __attribute__((always_inline)) {
+      constexpr bool LIN = ALIBI == 2 && !decltype(edge)::value;
       u32x4_t kf[NQK];
 #pragma unroll
       for (int k = 0; k < KPF; ++k) kf[k] = kread(kt, k);
@@ -187,11 +204,11 @@ struct Tile16 {
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
         for (int v = 0; v < 16; ++v)
-          s[nb][v] = ALIBI ? fabsf(fi - (float)(nb * 32 + (v >> 2) * 8 + (v & 3))) * alibi_mul : 0.f;
+          if constexpr (!LIN) s[nb][v] = ALIBI ? fabsf(fi - (float)(nb * 32 + (v >> 2) * 8 + (v & 3))) * alibi_mul : 0.f;
 #pragma unroll
       for (int k = 0; k < NQK; ++k) {
         if (k + KPF < NQK) kf[k + KPF] = kread(kt, k + KPF);
-        s[k / DS] = E::mfma(kf[k], qr[k % DS], s[k / DS]);
+        s[k / DS] = E::mfma(kf[k], qr[k % DS], LIN && k % DS == 0 ? lin[ALIBI == 2 ? k / DS : 0] : s[k / DS]);
       }
       __builtin_amdgcn_sched_group_barrier(0x100, KPF, 0);
 #pragma unroll
@@ -215,7 +232,9 @@ struct Tile16 {
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
         for (int v = 0; v < 16; ++v) mx = fmaxf(mx, s[nb][v]);
-      mx = xlane_max(mx) * c;
+      constexpr bool LIN = ALIBI == 2 && !decltype(edge)::value;
+      const float tile_bias = LIN ? alibi_mul * (float)(kr.pos - n0 - 4 * g) : 0.f;
+      mx = xlane_max(mx + tile_bias) * c;
       pin_acc();
       if (__builtin_expect(wave_any(mx > m_run + TAU), 0)) {
         const float m_new = fmaxf(m_run, mx);
@@ -227,7 +246,7 @@ struct Tile16 {
       }
       pin_acc();
       // a row that has seen no key yet: exp2(-inf) = 0
-      const float mneg = m_run == -INFINITY ? 0.f : -m_run;
+      const float mneg = __builtin_fmaf(tile_bias, c, m_run == -INFINITY ? 0.f : -m_run);
       float sum[2] = {0.f, 0.f};
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
@@ -285,7 +304,7 @@ struct Tile16 {
         // matrix sections at raised priority: the other wavefront of the SIMD
         // fills the gaps with its softmax
         __builtin_amdgcn_s_setprio(1);
-        qk(kt, n0, sc);
+        qk(edge, kt, n0, sc);
 #pragma unroll
         for (int m = 0; m < VPF; ++m) vpre[m] = vread(vt, m);
         __builtin_amdgcn_s_setprio(0);
