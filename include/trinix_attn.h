@@ -503,7 +503,7 @@ typedef struct trinix_packed_args {
   const int32_t* plan;  /* from trinix_packed_plan */
   int64_t plan_bytes;
   int64_t n_seqs, total_q, total_k;
-  int64_t nheads_q, nheads_kv, head_dim; /* head_dim 64, 128 or 256 */
+  int64_t nheads_q, nheads_kv, head_dim; /* head_dim to 256: multiples of 8, fp32 of 4 */
   int32_t dtype;        /* TRINIX_F32, TRINIX_F16 or TRINIX_BF16 */
   float softmax_scale;
   int32_t causal;
@@ -535,7 +535,7 @@ int trinix_packed_bwd(const trinix_packed_args* args, void* stream);
  * when the kernels run; clamped into [0, capacity]) may be NULL: len = capacity.
  * Cache rows at and behind len are not read.  A row without any key has out 0
  * and lse -inf.  prefix_len or capacity may be 0 (their pointers then are not
- * read).  head_dim 64, 128 or 256; 16-bit rows 16-byte aligned, fp32 rows too.
+ * read).  head_dim to 256, multiples of 8 (fp32: of 4); rows 16-byte aligned.
  *
  * trinix_shared_prefix_workspace: bytes of fp32 workspace that a call takes
  * (host only).  trinix_shared_prefix_fwd: the forward on `stream`; workspace

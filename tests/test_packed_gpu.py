@@ -54,7 +54,7 @@ RAGGED = [3, 1, 64, 130, 0, 65, 33, 257]
 
 
 @pytest.mark.parametrize("dtype", [BF, HF, F32])
-@pytest.mark.parametrize("D", [64, 128, 256, 80])
+@pytest.mark.parametrize("D", [64, 128, 256, 8, 30, 40, 80, 96, 129, 200])
 def test_ragged_causal(dtype, D):
     check(RAGGED, D=D, dtype=dtype, pad=5, seed=D)
 

@@ -56,7 +56,8 @@ def shared_args(**kw):
 
 @pytest.mark.parametrize("kw,code", [
     (dict(dtype=nat.TRINIX_U8), nat.TRINIX_ERR_BAD_DTYPE),
-    (dict(head_dim=80), nat.TRINIX_ERR_BAD_HEAD_DIM),
+    (dict(head_dim=84), nat.TRINIX_ERR_BAD_HEAD_DIM),
+    (dict(head_dim=264), nat.TRINIX_ERR_BAD_HEAD_DIM),
     (dict(batch=0), nat.TRINIX_ERR_BAD_SHAPE),
     (dict(seqlen_q=0), nat.TRINIX_ERR_BAD_SHAPE),
     (dict(prefix_len=-1), nat.TRINIX_ERR_BAD_SHAPE),
@@ -131,7 +132,9 @@ def args(lib, **kw):
 
 @pytest.mark.parametrize("kw,code", [
     (dict(dtype=nat.TRINIX_U8), nat.TRINIX_ERR_BAD_DTYPE),
-    (dict(head_dim=96), nat.TRINIX_ERR_BAD_HEAD_DIM),
+    (dict(head_dim=92), nat.TRINIX_ERR_BAD_HEAD_DIM),
+    (dict(head_dim=264), nat.TRINIX_ERR_BAD_HEAD_DIM),
+    (dict(head_dim=0), nat.TRINIX_ERR_BAD_HEAD_DIM),
     (dict(nheads_kv=3), nat.TRINIX_ERR_BAD_SHAPE),
     (dict(nheads_q=0), nat.TRINIX_ERR_BAD_SHAPE),
     (dict(nheads_kv=0), nat.TRINIX_ERR_BAD_SHAPE),
@@ -177,7 +180,7 @@ def test_packed_backward_workspace(lib):
         assert lib.trinix_packed_bwd(ctypes.byref(a), None) == nat.TRINIX_ERR_BAD_ARGUMENT
     assert lib.trinix_packed_bwd_workspace(None, ctypes.byref(n)) == nat.TRINIX_ERR_NULL_POINTER
     assert lib.trinix_packed_bwd_workspace(ctypes.byref(a), None) == nat.TRINIX_ERR_NULL_POINTER
-    for bad in (dict(nheads_kv=0), dict(nheads_kv=3), dict(head_dim=96), dict(total_k=-1), dict(n_seqs=0)):
+    for bad in (dict(nheads_kv=0), dict(nheads_kv=3), dict(head_dim=92), dict(total_k=-1), dict(n_seqs=0)):
         assert lib.trinix_packed_bwd_workspace(ctypes.byref(args(lib, **bad)), ctypes.byref(n)) == nat.TRINIX_ERR_BAD_SHAPE
 
 

@@ -68,7 +68,7 @@ def check(B, Sq, P, cap, lens, H=8, Hkv=2, D=64, dtype=BF, seed=0, layout="bhsd"
 
 
 @pytest.mark.parametrize("dtype", [BF, HF, F32])
-@pytest.mark.parametrize("D", [64, 128, 256, 80])
+@pytest.mark.parametrize("D", [64, 128, 256, 8, 30, 40, 80, 96, 129, 200])
 def test_decode(dtype, D):
     check(5, 1, 300, 200, [1, 200, 64, 17, 129], D=D, dtype=dtype, seed=D)
 

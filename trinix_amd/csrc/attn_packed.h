@@ -1,6 +1,7 @@
 // Attention over packed sequences: parameters, the work item of a workgroup and
 // the pieces that its kernels share (semantics: trinix_attn.h, trinix_packed_args).
 #pragma once
+#include "attn_ops.h"
 #include "attn_params.h"
 #include "lds_tile.h"
 #include "packed_map.h"
@@ -22,6 +23,7 @@ struct PackedParams {
   int64_t q_ss, q_sh, k_ss, k_sh, v_ss, v_sh, o_ss, o_sh;
   int64_t do_ss, do_sh, dq_ss, dq_sh, dk_ss, dk_sh, dv_ss, dv_sh;
   int Tq, Hq, Hkv, G;
+  int d;  // columns of every tensor: head_dim, at most the kernel's D
   float scale, scale_log2;
   int causal, has_window;
   int64_t wl, wr;  // clamped to +-2^30
@@ -84,6 +86,69 @@ struct PackedHeads {
 __device__ inline float* packed_partial(const PackedParams& p, int split, int which, int64_t row, int hkv, int D) {
   return p.part + ((((int64_t)split * 2 + which) * p.Tk + row) * p.Hkv + hkv) * D;
 }
+
+// Rows of d columns in kernels of D >= d: the operand in registers is zero from column
+// d on, so what the other one holds there (a copy of a real unit) adds nothing, and
+// output columns from d on are not written.
+template <class O>
+__device__ inline typename O::Frag load_frag_cols(const typename O::Store* row, int g, int d) {
+  typename O::Frag f;
+  constexpr int N = sizeof(f.r) / sizeof(f.r[0]), PER = O::kD / N, HALF = PER / 2;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int d0 = k * PER + g * HALF;
+    if constexpr (sizeof(typename O::Store) == 2) {
+      const u32x4_t x = *(const u32x4_t*)(row + min(d0, d - 8));
+      f.r[k] = d0 < d ? x : (u32x4_t){0u, 0u, 0u, 0u};
+    } else {
+      typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));  // any 4-byte aligned row
+      const f32x4_t x = *(const f32x4_any*)(row + min(d0, d - 4));
+      f.r[k] = d0 < d ? x : (f32x4_t){0.f, 0.f, 0.f, 0.f};
+    }
+  }
+  return f;
+}
+
+// TileCopy (attn_ops.h) of such rows: units from d on read the row's last one.
+template <class O, int NW>
+struct PackedCopy {
+  using Store = typename O::Store;
+  static constexpr int ESZ = (int)sizeof(Store), UPR = O::kD * ESZ / 16, PER = kTileRows * UPR / (64 * NW);
+  static_assert(PER >= 1 && kTileRows * UPR % (64 * NW) == 0, "tile shape");
+  int64_t ss;
+  int wave, lane, units;
+  uint32_t off[PER];
+  __device__ PackedCopy(int64_t ss_, int wave_, int lane_, int d) : ss(ss_), wave(wave_), lane(lane_), units(d * ESZ / 16) {
+#pragma unroll
+    for (int l = 0; l < PER; ++l) off[l] = offset(l, kTileRows - 1);
+  }
+  __device__ uint32_t offset(int l, int last) const {
+    const int row = tile_copy_row(wave, PER, l, lane, UPR);
+    return tile32_offset(row, last, ss, ESZ, min(O::swz(((wave * PER + l) * 64 + lane) % UPR, row), units - 1));
+  }
+  // rows [i0, i0 + 32) of n; `wide`: 16 bytes a lane from 32-bit offsets (always for 16-bit types)
+  __device__ void operator()(const Store* base, int i0, int n, char* lds_tile, bool wide) const {
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void_t*)lds_tile;
+    if (ESZ == 2 || wide) {
+      const uint64_t gb = uniform_ptr(base + (int64_t)i0 * ss);
+      if (i0 + kTileRows <= n) {
+#pragma unroll
+        for (int l = 0; l < PER; ++l) dma_16b_s(off[l], gb, __builtin_amdgcn_readfirstlane(lds0 + (wave * PER + l) * 1024));
+      } else {
+#pragma unroll 1
+        for (int l = 0; l < PER; ++l)
+          dma_16b_s(offset(l, n - 1 - i0), gb, __builtin_amdgcn_readfirstlane(lds0 + (wave * PER + l) * 1024));
+      }
+    } else {
+#pragma unroll 1
+      for (int l = 0; l < PER * 4; ++l) {
+        const int c = wave * PER * 4 + l, word = c * 64 + lane, unit = word / 4, row = unit / UPR;
+        dma_4b(base + (int64_t)min(i0 + row, n - 1) * ss + min(O::swz(unit % UPR, row), units - 1) * 4 + (word & 3),
+               __builtin_amdgcn_readfirstlane(lds0 + c * 256));
+      }
+    }
+  }
+};
 
 // fp16 keeps its output's rounding residue times 2^11 (half a step of the
 // largest fp16 number is 2^4; unscaled, the residue of 2^-10 would be denormal).

@@ -22,7 +22,7 @@ __global__ __launch_bounds__(256) void packed_delta_kernel(const PackedParams p,
   float acc = 0.f;
   const int64_t t = row / p.Hq;
   const int h = (int)(row % p.Hq);
-  if (row < rows) {
+  if (row < rows && c * VE < p.d) {
     const int64_t oo = t * p.o_ss + h * p.o_sh + c * VE, od = t * p.do_ss + h * p.do_sh + c * VE;
     if constexpr (F32) {
       const f32x4_t o = *(const f32x4_any*)((const float*)p.o + oo), d = *(const f32x4_any*)((const float*)p.dout + od);
@@ -52,7 +52,7 @@ __global__ __launch_bounds__(256) void packed_delta_kernel(const PackedParams p,
 template <class E, bool F32>
 __global__ __launch_bounds__(256) void packed_dkdv_sum(const PackedParams p, int D) {
   const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4, per = (int64_t)p.Tk * p.Hkv * D;
-  if (at >= per) return;
+  if (at >= per || at % D >= p.d) return;
   const int which = blockIdx.y;
   const float* x = p.part + which * per + at;
   f32x4_t s = *(const f32x4_t*)x;
@@ -108,6 +108,7 @@ PackedParams params(const trinix_packed_args* a) {
   p.Hq = (int)a->nheads_q;
   p.Hkv = (int)a->nheads_kv;
   p.G = p.Hq / p.Hkv;
+  p.d = (int)a->head_dim;
   p.scale = a->softmax_scale;
   p.scale_log2 = a->softmax_scale * kLog2e;
   p.causal = a->causal ? 1 : 0;
@@ -143,6 +144,7 @@ constexpr int kListOf[3] = {kRows64, kRows128, kRows256};  // of a PackedShape
 // TRINIX_PACKED_FWD = 0, 1, 2 forces pair, plain, wide (tuning and tests).
 PackedShape packed_shape(const trinix_packed_args* a) {
   const int64_t n = a->n_seqs, blocks = (a->total_q / 128 + lmin(n, a->total_q) / 2) * a->nheads_q;
+  const int D = packed_kernel_dim(a->head_dim);
   PackedShape s = PackedShape::kPlain;
   if (blocks <= 256 && a->total_k / n >= 256) s = PackedShape::kPair;
   else if (a->total_k / n >= 4096 && a->total_q * a->nheads_q / 256 >= 192) s = PackedShape::kWide;
@@ -150,7 +152,7 @@ PackedShape packed_shape(const trinix_packed_args* a) {
     const int want = atoi(env);
     if (want >= 0 && want <= 2) s = (PackedShape)want;
   }
-  if ((a->head_dim == 256 && s == PackedShape::kPair) || (a->head_dim != 128 && s == PackedShape::kWide)) s = PackedShape::kPlain;
+  if ((D == 256 && s == PackedShape::kPair) || (D != 128 && s == PackedShape::kWide)) s = PackedShape::kPlain;
   return s;
 }
 
@@ -166,7 +168,7 @@ PackedShape packed_shape(const trinix_packed_args* a) {
 //    3 x 1000 201 | 206, 9 x 300 111 | 129).
 // TRINIX_PACKED_PAIRS = 1, 2 forces either (tuning and tests).
 int two_per_group(const trinix_packed_args* a, int64_t total, int64_t heads, int64_t chain) {
-  if (a->dtype == TRINIX_F32 && a->head_dim == 256) return 1;
+  if (a->dtype == TRINIX_F32 && packed_kernel_dim(a->head_dim) == 256) return 1;
   if (const char* env = getenv("TRINIX_PACKED_PAIRS")) return atoi(env) == 1 ? 1 : 2;
   const int64_t blocks = (total / 128 + lmin(a->n_seqs, total) / 2) * heads, keys = a->total_k / a->n_seqs;
   if (a->dtype == TRINIX_F32) return blocks > 1536 && keys >= 1024 ? 1 : 2;
@@ -184,7 +186,7 @@ extern "C" int trinix_packed_fwd(const trinix_packed_args* a, void* stream) {
   if (a->total_q == 0) return TRINIX_OK;
   PackedParams p = params(a);
   hipStream_t st = (hipStream_t)stream;
-  const int D = (int)a->head_dim;
+  const int D = packed_kernel_dim(a->head_dim);
   hipError_t e;
   if (a->dtype == TRINIX_F32) {
     p.rows16 = rows16(a->k, a->k_stride) && rows16(a->v, a->v_stride);
@@ -203,7 +205,7 @@ extern "C" int trinix_packed_bwd(const trinix_packed_args* a, void* stream) {
   if (rc != TRINIX_OK) return rc;
   PackedParams p = params(a);
   hipStream_t st = (hipStream_t)stream;
-  const int D = (int)a->head_dim;
+  const int D = packed_kernel_dim(a->head_dim);
   const bool f32 = a->dtype == TRINIX_F32, bf = a->dtype == TRINIX_BF16;
   hipError_t e = hipSuccess;
   if (f32) p.rows16 = rows16(a->q, a->q_stride) && rows16(a->dout, a->dout_stride);

@@ -14,14 +14,14 @@ __global__ __launch_bounds__(NW * 64, OCC) void packed_fwd16(const PackedParams 
   if (w.blk < 0) return;
   Tile16<E, D, BN, NW, KS, ALIBI> T(lds_k0, lds_k1, lds_v0, lds_v1);
   const int hq = w.h, hkv = hq / p.G, m0 = w.blk * BM, iw0 = m0 + (T.wave / KS) * 32, i = iw0 + T.r;
-  T.load_q((const uint16_t*)p.q + (int64_t)(w.q0 + min(i, w.lq - 1)) * p.q_ss + hq * p.q_sh, p.scale_log2,
+  T.load_q((const uint16_t*)p.q + (int64_t)(w.q0 + min(i, w.lq - 1)) * p.q_ss + hq * p.q_sh, p.d, p.scale_log2,
            ALIBI ? p.alibi[hq * p.al_sh] : 0.f);
   const Span ks = w.keys_of(i);
   const int mlast = min(m0 + BM, w.lq) - 1;
   KeyRun kr;
   kr.k = (const uint16_t*)p.k + (int64_t)w.k0 * p.k_ss + hkv * p.k_sh;
   kr.v = (const uint16_t*)p.v + (int64_t)w.k0 * p.v_ss + hkv * p.v_sh;
-  kr.k_ss = p.k_ss, kr.v_ss = p.v_ss, kr.n = w.lk;
+  kr.k_ss = p.k_ss, kr.v_ss = p.v_ss, kr.n = w.lk, kr.d = p.d;
   bwd_key_tiles(m0, BM, w.lq, w.lk, w.dlo, w.dhi, BN, kr.t_lo, kr.t_hi);
   packed_full_tiles(m0, mlast, w.lk, w.dlo, w.dhi, BN, kr.t_lo, kr.t_hi, kr.t_flo, kr.t_fhi);
   kr.jlo = ks.lo, kr.jspan = ks.span;
@@ -40,6 +40,7 @@ __global__ __launch_bounds__(NW * 64, OCC) void packed_fwd16(const PackedParams 
 #pragma unroll
     for (int vq = 0; vq < 4; ++vq) {
       const int d0 = db * 32 + vq * 8 + T.g * 4;
+      if (db * 32 + vq * 8 >= p.d) continue;
       float x[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[e] = T.acc[db][vq * 4 + e] * inv;

@@ -84,7 +84,7 @@ __device__ __forceinline__ void packed_dkdv_body(const PackedParams& p, const Pa
 #pragma unroll
     for (int l = 0; l < LPW; ++l) {
       const int row = tile_copy_row(wave, LPW, l, lane, UPR);
-      dma_16b_s(tile_copy_offset((uint32_t)min(row, last), ss, (uint32_t)((lane % UPR) ^ swz_kt<D>(row))), gb,
+      dma_16b_s(tile_copy_offset((uint32_t)min(row, last), ss, (uint32_t)min((lane % UPR) ^ swz_kt<D>(row), p.d / 8 - 1)), gb,
                 __builtin_amdgcn_readfirstlane(lds0 + l * 1024));
     }
   };
@@ -121,8 +121,8 @@ __device__ __forceinline__ void packed_dkdv_body(const PackedParams& p, const Pa
   auto run = [&](auto second_c) __attribute__((always_inline)) {
     constexpr bool SB = decltype(second_c)::value;  // dK
     const typename O::Frag br =
-        SB ? O::load_frag((const uint16_t*)p.v + (int64_t)(w.k0 + jc) * p.v_ss + hkv * p.v_sh, g)
-           : O::load_frag((const uint16_t*)p.k + (int64_t)(w.k0 + jc) * p.k_ss + hkv * p.k_sh, g);
+        SB ? load_frag_cols<O>((const uint16_t*)p.v + (int64_t)(w.k0 + jc) * p.v_ss + hkv * p.v_sh, g, p.d)
+           : load_frag_cols<O>((const uint16_t*)p.k + (int64_t)(w.k0 + jc) * p.k_ss + hkv * p.k_sh, g, p.d);
     f32x16_t acc[DB];
 #pragma unroll
     for (int db = 0; db < DB; ++db) acc[db] = (f32x16_t){};
@@ -283,7 +283,7 @@ __device__ __forceinline__ void packed_dkdv_body(const PackedParams& p, const Pa
     for (int db = 0; db < DB; ++db)
 #pragma unroll
       for (int vq = 0; vq < 4; ++vq)
-        O::store4(row, db * 32 + vq * 8 + g * 4, acc[db][vq * 4] * f, acc[db][vq * 4 + 1] * f, acc[db][vq * 4 + 2] * f,
+        if (db * 32 + vq * 8 < p.d) O::store4(row, db * 32 + vq * 8 + g * 4, acc[db][vq * 4] * f, acc[db][vq * 4 + 1] * f, acc[db][vq * 4 + 2] * f,
                   acc[db][vq * 4 + 3] * f);
   };
   if (wave >= NG) run(std::true_type{});
@@ -303,8 +303,8 @@ __device__ __forceinline__ void packed_dq_body(const PackedParams& p, const Pack
   const int off = w.lk - w.lq;
 
   const O ops(lane, 0);
-  const typename O::Frag qf = O::load_frag((const uint16_t*)p.q + (int64_t)(w.q0 + ic) * p.q_ss + hq * p.q_sh, g);
-  const typename O::Frag of = O::load_frag((const uint16_t*)p.dout + (int64_t)(w.q0 + ic) * p.do_ss + hq * p.do_sh, g);
+  const typename O::Frag qf = load_frag_cols<O>((const uint16_t*)p.q + (int64_t)(w.q0 + ic) * p.q_ss + hq * p.q_sh, g, p.d);
+  const typename O::Frag of = load_frag_cols<O>((const uint16_t*)p.dout + (int64_t)(w.q0 + ic) * p.do_ss + hq * p.do_sh, g, p.d);
   const int64_t ro = (int64_t)hq * p.Tq + w.q0 + ic;
   const float lse2 = fmaxf(p.lse[ro] * kLog2e, -0.5f * FLT_MAX), dlt = p.delta[ro];  // (finite: see write_rows)
   const float slope_l2 = p.alibi ? -p.alibi[hq * p.al_sh] * kLog2e : 0.f;
@@ -321,7 +321,7 @@ __device__ __forceinline__ void packed_dq_body(const PackedParams& p, const Pack
   const int64_t css = cv ? p.v_ss : p.k_ss;
   const uint16_t* cbase = cv ? (const uint16_t*)p.v + (int64_t)w.k0 * p.v_ss + hkv * p.v_sh
                              : (const uint16_t*)p.k + (int64_t)w.k0 * p.k_ss + hkv * p.k_sh;
-  const TileCopy<O, NG> copy(css, wave % NG, lane);
+  const PackedCopy<O, NG> copy(css, wave % NG, lane, p.d);
   auto load = [&](int t, int slot) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < NT; ++u)
@@ -378,7 +378,7 @@ __device__ __forceinline__ void packed_dq_body(const PackedParams& p, const Pack
   for (int db = 0; db < DB; ++db)
 #pragma unroll
     for (int vq = 0; vq < 4; ++vq)
-      O::store4(row, db * 32 + vq * 8 + g * 4, acc[db][vq * 4] * f, acc[db][vq * 4 + 1] * f, acc[db][vq * 4 + 2] * f,
+      if (db * 32 + vq * 8 < p.d) O::store4(row, db * 32 + vq * 8 + g * 4, acc[db][vq * 4] * f, acc[db][vq * 4 + 1] * f, acc[db][vq * 4 + 2] * f,
                 acc[db][vq * 4 + 3] * f);
 }
 

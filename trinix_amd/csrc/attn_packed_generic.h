@@ -33,7 +33,7 @@ __global__ __launch_bounds__(256, OCC) void packed_fwd_f32(const PackedParams p)
   const bool wide = p.rows16 != 0;
 
   const O ops(lane, 0);
-  const typename O::Frag qf = O::load_frag((const Store*)p.q + (int64_t)(w.q0 + ic) * p.q_ss + hq * p.q_sh, g);
+  const typename O::Frag qf = load_frag_cols<O>((const Store*)p.q + (int64_t)(w.q0 + ic) * p.q_ss + hq * p.q_sh, g, p.d);
   const float slope_l2 = p.alibi ? -p.alibi[hq * p.al_sh] * kLog2e : 0.f;
   const int off = w.lk - w.lq;
   f32x16_t acc[DB];
@@ -45,7 +45,7 @@ __global__ __launch_bounds__(256, OCC) void packed_fwd_f32(const PackedParams p)
   bwd_key_tiles(m0, BM, w.lq, w.lk, w.dlo, w.dhi, kTileRows, t_lo, t_hi);
   const Store* kbase = (const Store*)p.k + (int64_t)w.k0 * p.k_ss + hkv * p.k_sh;
   const Store* vbase = (const Store*)p.v + (int64_t)w.k0 * p.v_ss + hkv * p.v_sh;
-  const TileCopy<O, NW> copy_k(p.k_ss, wave, lane), copy_v(p.v_ss, wave, lane);
+  const PackedCopy<O, NW> copy_k(p.k_ss, wave, lane, p.d), copy_v(p.v_ss, wave, lane, p.d);
   auto load = [&](int t, int slot) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < KS; ++u)
@@ -142,7 +142,7 @@ __global__ __launch_bounds__(256, OCC) void packed_fwd_f32(const PackedParams p)
   for (int db = 0; db < DB; ++db)
 #pragma unroll
     for (int vq = 0; vq < 4; ++vq)
-      O::store4(orow, db * 32 + vq * 8 + g * 4, acc[db][vq * 4] * inv, acc[db][vq * 4 + 1] * inv, acc[db][vq * 4 + 2] * inv,
+      if (db * 32 + vq * 8 + g * 4 < p.d) O::store4(orow, db * 32 + vq * 8 + g * 4, acc[db][vq * 4] * inv, acc[db][vq * 4 + 1] * inv, acc[db][vq * 4 + 2] * inv,
                 acc[db][vq * 4 + 3] * inv);
   if (p.lse && g == 0) p.lse[(int64_t)hq * p.Tq + row] = l > 0.f ? (m_run + log2f(l)) * kLn2 : -INFINITY;
 }
@@ -172,14 +172,14 @@ __global__ __launch_bounds__(256, OCC) void packed_dkdv_generic(const PackedPara
   const int n_items = nqt > 0 ? (hd.gh1 - hd.gh0) * nqt : 0;  // item = (q-head of the group, query tile)
 
   const O ops(lane, db0);
-  const typename O::Frag kf = O::load_frag((const Store*)p.k + (int64_t)(w.k0 + jc) * p.k_ss + hkv * p.k_sh, g);
-  const typename O::Frag vf = O::load_frag((const Store*)p.v + (int64_t)(w.k0 + jc) * p.v_ss + hkv * p.v_sh, g);
+  const typename O::Frag kf = load_frag_cols<O>((const Store*)p.k + (int64_t)(w.k0 + jc) * p.k_ss + hkv * p.k_sh, g, p.d);
+  const typename O::Frag vf = load_frag_cols<O>((const Store*)p.v + (int64_t)(w.k0 + jc) * p.v_ss + hkv * p.v_sh, g, p.d);
   f32x16_t dk[DB], dv[DB];
 #pragma unroll
   for (int db = 0; db < DB; ++db) dk[db] = dv[db] = (f32x16_t){};
   ZScale<O> zs;
 
-  const TileCopy<O, NW> copy_q(p.q_ss, wave, lane), copy_o(p.do_ss, wave, lane);
+  const PackedCopy<O, NW> copy_q(p.q_ss, wave, lane, p.d), copy_o(p.do_ss, wave, lane, p.d);
   float lse_next = 0.f, del_next = 0.f;
   auto load_step = [&](int it, int slot) __attribute__((always_inline)) {  // items it .. it + KS - 1
 #pragma unroll
@@ -287,6 +287,7 @@ __global__ __launch_bounds__(256, OCC) void packed_dkdv_generic(const PackedPara
 #pragma unroll
     for (int vq = 0; vq < 4; ++vq) {
       const int d0 = (db0 + db) * 32 + vq * 8 + g * 4;
+      if (d0 >= p.d) continue;
       O::store4(vrow, d0, dv[db][vq * 4] * fv, dv[db][vq * 4 + 1] * fv, dv[db][vq * 4 + 2] * fv, dv[db][vq * 4 + 3] * fv);
       O::store4(krow, d0, dk[db][vq * 4] * fk, dk[db][vq * 4 + 1] * fk, dk[db][vq * 4 + 2] * fk, dk[db][vq * 4 + 3] * fk);
     }
@@ -307,8 +308,8 @@ __global__ __launch_bounds__(256, OCC) void packed_dq_generic(const PackedParams
   const bool wide = p.rows16 != 0;
 
   const O ops(lane, db0);
-  const typename O::Frag qf = O::load_frag((const Store*)p.q + (int64_t)(w.q0 + ic) * p.q_ss + hq * p.q_sh, g);
-  const typename O::Frag of = O::load_frag((const Store*)p.dout + (int64_t)(w.q0 + ic) * p.do_ss + hq * p.do_sh, g);
+  const typename O::Frag qf = load_frag_cols<O>((const Store*)p.q + (int64_t)(w.q0 + ic) * p.q_ss + hq * p.q_sh, g, p.d);
+  const typename O::Frag of = load_frag_cols<O>((const Store*)p.dout + (int64_t)(w.q0 + ic) * p.do_ss + hq * p.do_sh, g, p.d);
   const int64_t ro = (int64_t)hq * p.Tq + w.q0 + ic;
   const float lse2 = fmaxf(p.lse[ro] * kLog2e, -0.5f * FLT_MAX), dlt = p.delta[ro];  // (finite: see above)
   const float slope_l2 = p.alibi ? -p.alibi[hq * p.al_sh] * kLog2e : 0.f;
@@ -321,7 +322,7 @@ __global__ __launch_bounds__(256, OCC) void packed_dq_generic(const PackedParams
   bwd_key_tiles(m0, BM, w.lq, w.lk, w.dlo, w.dhi, kTileRows, t_lo, t_hi);
   const Store* kbase = (const Store*)p.k + (int64_t)w.k0 * p.k_ss + hkv * p.k_sh;
   const Store* vbase = (const Store*)p.v + (int64_t)w.k0 * p.v_ss + hkv * p.v_sh;
-  const TileCopy<O, NW> copy_k(p.k_ss, wave, lane), copy_v(p.v_ss, wave, lane);
+  const PackedCopy<O, NW> copy_k(p.k_ss, wave, lane, p.d), copy_v(p.v_ss, wave, lane, p.d);
   auto load = [&](int t, int slot) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < KS; ++u)
@@ -382,7 +383,7 @@ __global__ __launch_bounds__(256, OCC) void packed_dq_generic(const PackedParams
 #pragma unroll
     for (int vq = 0; vq < 4; ++vq) {
       const int d0 = (db0 + db) * 32 + vq * 8 + g * 4;
-      O::store4(row, d0, acc[db][vq * 4] * f, acc[db][vq * 4 + 1] * f, acc[db][vq * 4 + 2] * f, acc[db][vq * 4 + 3] * f);
+      if (d0 < p.d) O::store4(row, d0, acc[db][vq * 4] * f, acc[db][vq * 4 + 1] * f, acc[db][vq * 4 + 2] * f, acc[db][vq * 4 + 3] * f);
     }
 }
 

@@ -39,11 +39,13 @@ constexpr int kTile16Words = KS * BN * D;
 // hold only pairs that every row of the workgroup may see.  A lane's row sees
 // keys jlo .. jlo + jspan (jlo = INT_MAX: none); keys outside [wlo, whi] are seen
 // by no row of the wavefront.  pos: position of the lane's row among the keys (ALiBi).
+// Rows hold d <= D columns (a multiple of 8): q is zero from there on in registers, and
+// K and V units from there on are copies of the row's last one.
 struct KeyRun {
   const uint16_t* k;
   const uint16_t* v;
   int64_t k_ss, v_ss;
-  int n, t_lo, t_hi, t_flo, t_fhi;
+  int n, d, t_lo, t_hi, t_flo, t_fhi;
   int jlo;
   uint32_t jspan;
   int wlo, whi;
@@ -103,7 +105,7 @@ struct Tile16 {
 
   // The lane's query row and the scale: the maximum of raw scores is that of the
   // scaled ones for a positive scale, so a negative one negates q, a zero one clears it.
-  __device__ __forceinline__ void load_q(const uint16_t* row, float scale_log2, float slope) {
+  __device__ __forceinline__ void load_q(const uint16_t* row, int d, float scale_log2, float slope) {
     const bool neg = scale_log2 < 0.f, zero = scale_log2 == 0.f;
     c = neg ? -scale_log2 : (zero ? 1.f : scale_log2);
     if constexpr (ALIBI != 0) alibi_mul = -slope * kLog2e / c;
@@ -118,9 +120,11 @@ struct Tile16 {
     const uint32_t flip = neg ? 0x80008000u : 0u, keep = zero ? 0u : 0xffffffffu;
 #pragma unroll
     for (int ds = 0; ds < DS; ++ds) {
-      qr[ds] = *(const u32x4_t*)(row + ds * 16 + g * 8);
+      const int d0 = ds * 16 + g * 8;
+      qr[ds] = *(const u32x4_t*)(row + min(d0, d - 8));
+      const uint32_t mask = d0 < d ? keep : 0u;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) qr[ds][e] = (qr[ds][e] ^ flip) & keep;
+      for (int e = 0; e < 4; ++e) qr[ds][e] = (qr[ds][e] ^ flip) & mask;
     }
   }
 
@@ -158,8 +162,8 @@ struct Tile16 {
     // (uniform by construction; 64-bit comparisons leave them in vector registers)
     for (int* x : {&kr.n, &kr.t_lo, &kr.t_hi, &kr.t_flo, &kr.t_fhi, &kr.wlo, &kr.whi}) *x = __builtin_amdgcn_readfirstlane(*x);
     auto ld_row = [&](int l) __attribute__((always_inline)) { return tile_copy_row(wave, LPW, l, lane, UPR); };
-    auto ld_unit_k = [&](int l) __attribute__((always_inline)) { return (lane % UPR) ^ swz_k<D>(ld_row(l)); };
-    auto ld_unit_v = [&](int l) __attribute__((always_inline)) { return (lane % UPR) ^ swz_v<D>(ld_row(l)); };
+    auto ld_unit_k = [&](int l) __attribute__((always_inline)) { return min((lane % UPR) ^ swz_k<D>(ld_row(l)), kr.d / 8 - 1); };
+    auto ld_unit_v = [&](int l) __attribute__((always_inline)) { return min((lane % UPR) ^ swz_v<D>(ld_row(l)), kr.d / 8 - 1); };
     uint32_t ld_koff[LPW], ld_voff[LPW];
 #pragma unroll
     for (int l = 0; l < LPW; ++l) {

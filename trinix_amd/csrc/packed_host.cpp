@@ -28,7 +28,7 @@ int check_rows(const void* ptr, const int64_t st[3], int64_t rows, bool f32) {
 int validate_packed(const trinix_packed_args* a, bool backward) {
   if (!a || !a->plan) return TRINIX_ERR_NULL_POINTER;
   if (a->dtype != TRINIX_F32 && a->dtype != TRINIX_F16 && a->dtype != TRINIX_BF16) return TRINIX_ERR_BAD_DTYPE;
-  if (a->head_dim != 64 && a->head_dim != 128 && a->head_dim != 256) return TRINIX_ERR_BAD_HEAD_DIM;
+  if (!packed_head_dim_ok(a->head_dim, a->dtype)) return TRINIX_ERR_BAD_HEAD_DIM;
   int64_t need = 0;
   const int prc = trinix_packed_plan_bytes(a->n_seqs, a->total_q, a->total_k, &need);
   if (prc != TRINIX_OK) return prc;
@@ -79,7 +79,7 @@ int packed_head_splits(const trinix_packed_args* a) {
 }
 int64_t packed_partial_bytes(const trinix_packed_args* a) {
   const int n = packed_head_splits(a);
-  return n > 1 ? 2ll * n * a->total_k * a->nheads_kv * a->head_dim * 4 : 0;
+  return n > 1 ? 2ll * n * a->total_k * a->nheads_kv * packed_kernel_dim(a->head_dim) * 4 : 0;
 }
 
 namespace {
@@ -100,7 +100,7 @@ int check_vec(const void* ptr, const int64_t* st, int dims, int esize) {
 int validate_shared(const trinix_shared_prefix_args* a) {
   if (!a) return TRINIX_ERR_NULL_POINTER;
   if (a->dtype != TRINIX_F32 && a->dtype != TRINIX_F16 && a->dtype != TRINIX_BF16) return TRINIX_ERR_BAD_DTYPE;
-  if (a->head_dim != 64 && a->head_dim != 128 && a->head_dim != 256) return TRINIX_ERR_BAD_HEAD_DIM;
+  if (!packed_head_dim_ok(a->head_dim, a->dtype)) return TRINIX_ERR_BAD_HEAD_DIM;
   constexpr int64_t kMax = 1ll << 30;
   if (a->batch <= 0 || a->seqlen_q <= 0 || a->prefix_len < 0 || a->capacity < 0 || a->nheads_q <= 0 || a->nheads_kv <= 0 ||
       a->batch >= (1ll << 24) || a->seqlen_q >= (1ll << 24) || a->prefix_len >= kMax || a->capacity >= kMax ||
@@ -132,7 +132,7 @@ int plan_shared(const trinix_shared_prefix_args* a, SharedPlan* pl) {
   const bool f32 = a->dtype == TRINIX_F32;
   const auto blocks = [](int64_t n, int64_t per) { return (n + per - 1) / per; };
   pl->rows = (int)rows;
-  const bool d256 = a->head_dim == 256;
+  const bool d256 = packed_kernel_dim(a->head_dim) == 256;
   pl->kind = f32 ? SharedKind::kRows16 : SharedKind::kSplit;
   if (!f32 && !d256 && own >= 32 && own <= 64 && a->batch * kv >= kSharedWhole) pl->kind = SharedKind::kWhole64;
   else if (!f32 && own > 64 && a->batch * blocks(own, 128) * kv >= kSharedWhole) pl->kind = SharedKind::kWhole128;
@@ -167,7 +167,7 @@ int plan_shared(const trinix_shared_prefix_args* a, SharedPlan* pl) {
   pl->wg_p = gp * pl->n_p;
   pl->wg_s = gs * pl->n_s;
   if (pl->wg_p + pl->wg_s > INT32_MAX) return TRINIX_ERR_BAD_SHAPE;
-  pl->ws_bytes = kv * rows * (pl->n_p + pl->n_s) * (a->head_dim + 1) * 4;
+  pl->ws_bytes = kv * rows * (pl->n_p + pl->n_s) * (packed_kernel_dim(a->head_dim) + 1) * 4;
   return TRINIX_OK;
 }
 
@@ -178,7 +178,7 @@ using namespace trinix;
 extern "C" int trinix_packed_bwd_workspace(const trinix_packed_args* a, int64_t* bytes) {
   if (!a || !bytes) return TRINIX_ERR_NULL_POINTER;
   if (a->nheads_q <= 0 || a->nheads_kv <= 0 || a->nheads_q > (1 << 20) || a->nheads_q % a->nheads_kv != 0 || a->n_seqs < 1 ||
-      a->total_k < 0 || a->total_k >= (1ll << 30) || (a->head_dim != 64 && a->head_dim != 128 && a->head_dim != 256))
+      a->total_k < 0 || a->total_k >= (1ll << 30) || !packed_head_dim_ok(a->head_dim, a->dtype))
     return TRINIX_ERR_BAD_SHAPE;
   *bytes = packed_partial_bytes(a);
   return TRINIX_OK;

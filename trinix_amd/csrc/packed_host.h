@@ -6,6 +6,13 @@
 
 namespace trinix {
 
+// head_dim that a call's kernels are built for (at least the tensors'), and whether
+// they take it: multiples of 8, fp32 of 4, up to 256.
+inline int packed_kernel_dim(int64_t head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
+inline bool packed_head_dim_ok(int64_t head_dim, int32_t dtype) {
+  return head_dim > 0 && head_dim <= 256 && head_dim % (dtype == TRINIX_F32 ? 4 : 8) == 0;
+}
+
 // TRINIX_OK or the status to return; no launch.  `backward`: the gradient
 // pointers and strides too.
 int validate_packed(const trinix_packed_args* a, bool backward);

@@ -35,6 +35,7 @@ struct SharedParams {
   const int32_t* lens;
   int64_t q_sb, q_ss, q_sh, pk_ss, pk_sh, pv_ss, pv_sh, k_sb, k_ss, k_sh, v_sb, v_ss, v_sh, o_sb, o_ss, o_sh;
   int B, Sq, P, cap, Hq, Hkv, G;
+  int d;  // columns of every tensor: head_dim, at most the kernel's D
   int rows, n_p, chunk_p, n_s, chunk_s, wg_p;
   float scale_log2;
   float* part_o;    // (Hkv, rows, n_p + n_s, D) normalised O of a chunk
@@ -131,13 +132,16 @@ __device__ __forceinline__ void rows16_body(const SharedParams& p, const Item it
   struct V4 {
     f32x4_t w[4][VC / 4];
   };
-  auto load_row = [&](const float* row) {
+  auto load_row = [&](const float* row) {  // (columns from d on: the last ones again)
     Seg x;
 #pragma unroll
-    for (int t = 0; t < VC; ++t) x.w[t] = *(const f32x4_t*)(row + t * 16 + lg * 4);
+    for (int t = 0; t < VC; ++t) x.w[t] = *(const f32x4_t*)(row + min(t * 16 + lg * 4, p.d - 4));
     return x;
   };
-  const Seg qv = load_row((const float*)p.q + rb * p.q_sb + (int64_t)ri * p.q_ss + hq * p.q_sh);
+  Seg qv = load_row((const float*)p.q + rb * p.q_sb + (int64_t)ri * p.q_ss + hq * p.q_sh);
+#pragma unroll
+  for (int t = 0; t < VC; ++t)
+    if (t * 16 + lg * 4 >= p.d) qv.w[t] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
   const int64_t kss = prefix ? p.pk_ss : p.k_ss, vss = prefix ? p.pv_ss : p.v_ss;
   const float* kbase = prefix ? (const float*)p.pk + hkv * p.pk_sh : (const float*)p.k + b * p.k_sb + hkv * p.k_sh;
   const float* vbase = prefix ? (const float*)p.pv + hkv * p.pv_sh : (const float*)p.v + b * p.v_sb + hkv * p.v_sh;
@@ -148,7 +152,7 @@ __device__ __forceinline__ void rows16_body(const SharedParams& p, const Item it
     for (int u = 0; u < 4; ++u)
 #pragma unroll
       for (int k = 0; k < VC / 4; ++k)
-        x.w[u][k] = *(const f32x4_t*)(vbase + (int64_t)min(j0 + lg * 4 + u, c1 - 1) * vss + lr * VC + k * 4);
+        x.w[u][k] = *(const f32x4_t*)(vbase + (int64_t)min(j0 + lg * 4 + u, c1 - 1) * vss + min(lr * VC + k * 4, p.d - 4));
     return x;
   };
 
@@ -281,7 +285,7 @@ __device__ inline KeyRun prefix_run(const SharedParams& p, int hkv, int c0, int 
   kr.k_ss = p.pk_ss, kr.v_ss = p.pv_ss;
   kr.k = (const uint16_t*)p.pk + hkv * p.pk_sh + (int64_t)c0 * p.pk_ss;
   kr.v = (const uint16_t*)p.pv + hkv * p.pv_sh + (int64_t)c0 * p.pv_ss;
-  kr.n = c1 - c0;
+  kr.n = c1 - c0, kr.d = p.d;
   kr.t_lo = kr.t_flo = 0;
   kr.t_hi = (kr.n + BN - 1) / BN;
   kr.t_fhi = kr.n / BN;
@@ -301,7 +305,7 @@ __device__ inline KeyRun own_run(const SharedParams& p, int b, int hkv, int c0, 
   kr.k_ss = p.k_ss, kr.v_ss = p.v_ss;
   kr.k = (const uint16_t*)p.k + b * p.k_sb + hkv * p.k_sh + (int64_t)c0 * p.k_ss;
   kr.v = (const uint16_t*)p.v + b * p.v_sb + hkv * p.v_sh + (int64_t)c0 * p.v_ss;
-  kr.n = c1 - c0;
+  kr.n = c1 - c0, kr.d = p.d;
   const int at0 = len - p.Sq - c0;  // last key of query 0, from c0
   kr.t_lo = kr.t_flo = 0;
   kr.t_hi = (min(kr.n, max(at0 + ie + 1, 0)) + BN - 1) / BN;
@@ -329,7 +333,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void shared_split(const Shar
   Tile16<E, D, BN, 4, KS, 0> T(lds_k0, lds_k1, lds_v0, lds_v1);
   const int rw = it.r0 + (T.wave / KS) * 32;
   const TileRow row(p, rw, it.r1, T.lane, it.hkv);
-  T.load_q(row.q(p), p.scale_log2, 0.f);
+  T.load_q(row.q(p), p.d, p.scale_log2, 0.f);
   if (it.prefix) {
     T.run(prefix_run<BN>(p, it.hkv, it.c0, it.c1, row.ok, rw < it.r1));
   } else {
@@ -363,7 +367,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void shared_whole(const Shar
   Tile16<E, D, BN, 4, KS, 0> T(lds_k0, lds_k1, lds_v0, lds_v1);
   const int rw = r0 + (T.wave / KS) * 32;
   const TileRow row(p, rw, r1, T.lane, hkv);
-  T.load_q(row.q(p), p.scale_log2, 0.f);
+  T.load_q(row.q(p), p.d, p.scale_log2, 0.f);
   if (p.P > 0) {
     T.run(prefix_run<BN>(p, hkv, 0, p.P, row.ok, rw < r1));
     __syncthreads();  // the buffers are free for the second run
@@ -381,7 +385,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void shared_whole(const Shar
   for (int db = 0; db < D / 32; ++db)
 #pragma unroll
     for (int vq = 0; vq < 4; ++vq)
-      Row<E>::store4(o + db * 32 + vq * 8 + T.g * 4, T.acc[db][vq * 4] * inv, T.acc[db][vq * 4 + 1] * inv,
+      if (db * 32 + vq * 8 < p.d) Row<E>::store4(o + db * 32 + vq * 8 + T.g * 4, T.acc[db][vq * 4] * inv, T.acc[db][vq * 4 + 1] * inv,
                         T.acc[db][vq * 4 + 2] * inv, T.acc[db][vq * 4 + 3] * inv);
   if (p.lse && T.g == 0)
     p.lse[((int64_t)b * p.Hq + row.h) * p.Sq + row.i] = l > 0.f ? (T.m_run + __log2f(l)) * kLn2 : -INFINITY;
@@ -447,7 +451,7 @@ __global__ __launch_bounds__(256) void shared_merge(const SharedParams p) {
     oo += w * s_o[k][t];
   }
   const float inv = LL > 0.f ? 1.f / LL : 0.f;  // a row that sees no key: 0
-  Row<E>::store4((Store*)p.o + b * p.o_sb + (int64_t)i * p.o_ss + hq * p.o_sh + t * 4, oo[0] * inv, oo[1] * inv, oo[2] * inv,
+  if (t * 4 < p.d) Row<E>::store4((Store*)p.o + b * p.o_sb + (int64_t)i * p.o_ss + hq * p.o_sh + t * 4, oo[0] * inv, oo[1] * inv, oo[2] * inv,
             oo[3] * inv);
   if (p.lse && t == 0) p.lse[((int64_t)b * p.Hq + hq) * p.Sq + i] = LL > 0.f ? (mm + __log2f(LL)) * kLn2 : -INFINITY;
 }
@@ -497,13 +501,14 @@ extern "C" int trinix_shared_prefix_fwd(const trinix_shared_prefix_args* a, void
   p.o_sb = a->out_stride[0], p.o_ss = a->out_stride[1], p.o_sh = a->out_stride[2];
   p.B = (int)a->batch, p.Sq = (int)a->seqlen_q, p.P = (int)a->prefix_len, p.cap = (int)a->capacity;
   p.Hq = (int)a->nheads_q, p.Hkv = (int)a->nheads_kv, p.G = p.Hq / p.Hkv;
+  p.d = (int)a->head_dim;
   p.rows = pl.rows;
   p.n_p = pl.n_p, p.chunk_p = pl.chunk_p, p.n_s = pl.n_s, p.chunk_s = pl.chunk_s;
   p.wg_p = (int)pl.wg_p;
   p.scale_log2 = a->softmax_scale * kLog2e;
   p.part_o = (float*)workspace;
-  p.part_lse = p.part_o + (int64_t)p.Hkv * p.rows * (p.n_p + p.n_s) * a->head_dim;
-  const int D = (int)a->head_dim;
+  p.part_lse = p.part_o + (int64_t)p.Hkv * p.rows * (p.n_p + p.n_s) * packed_kernel_dim(a->head_dim);
+  const int D = packed_kernel_dim(a->head_dim);
   hipStream_t st = (hipStream_t)stream;
   const hipError_t e = a->dtype == TRINIX_F32 ? launch<F32>(p, D, pl, st)
                        : a->dtype == TRINIX_BF16 ? launch<BF16>(p, D, pl, st) : launch<F16>(p, D, pl, st);

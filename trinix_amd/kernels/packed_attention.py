@@ -129,9 +129,15 @@ def _ready(t: torch.Tensor) -> bool:
     return t.element_size() == 4 or (t.data_ptr() % 16 == 0 and s % 8 == 0 and h % 8 == 0 and s < 1 << 22)
 
 
-def _operand(t: torch.Tensor, d_kernel: int) -> torch.Tensor:
-    if t.shape[-1] != d_kernel:
-        t = torch.nn.functional.pad(t, (0, d_kernel - t.shape[-1]))
+def _columns(t: torch.Tensor) -> int:
+    """Columns that the kernels take t at: its head_dim rounded up to 16 bytes."""
+    per = 16 // t.element_size()
+    return -(-t.shape[-1] // per) * per
+
+
+def _operand(t: torch.Tensor, d: int) -> torch.Tensor:
+    if t.shape[-1] != d:
+        t = torch.nn.functional.pad(t, (0, d - t.shape[-1]))
     if not _ready(t):
         t = t.contiguous()
         if not _ready(t):
@@ -331,7 +337,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sequence
         a = nat.PackedArgs.from_buffer_copy(ent.fwd)
         a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
     else:
-        d_kernel = kernel_head_dim(q.shape[-1])
+        d_kernel = _columns(q)
         a = _args(q, k, sequences, scale, causal, window_size, slopes, d_kernel)
         if d_kernel == q.shape[-1] and _ready(q) and _ready(k) and _ready(v):
             _set_operands(a, q, k, v, d_kernel)

@@ -101,8 +101,9 @@ def _full(key, ts, seq_lens, scale, return_lse):
         raise ValueError(f"shapes don't match: q, prefix_k, prefix_v, k, v are {[tuple(t.shape) for t in ts]}")
     if Hkv <= 0 or H <= 0 or D <= 0 or H % Hkv != 0:
         raise ValueError(f"num_heads ({H}) must be a multiple of the KV heads ({Hkv})")
-    d_kernel = kernel_head_dim(D)
-    if d_kernel is None:
+    per = 16 // q.element_size()
+    d_kernel = -(-D // per) * per  # rows of whole 16 bytes
+    if kernel_head_dim(D) is None:
         raise ValueError(f"head_dim {D} > {KERNEL_HEAD_DIMS[-1]} is not supported")
     if seq_lens is not None and (seq_lens.shape != (B,) or seq_lens.device != q.device
                                  or seq_lens.dtype not in (torch.int32, torch.int64)):
