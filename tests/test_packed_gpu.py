@@ -86,7 +86,7 @@ def test_windows_beside_the_diagonal(window):
 
 
 @pytest.mark.parametrize("shape", ["0", "1", "2"])
-@pytest.mark.parametrize("dtype,D", [(BF, 64), (HF, 128), (BF, 256)])
+@pytest.mark.parametrize("dtype,D", [(BF, 64), (HF, 128), (BF, 256), (BF, 96), (HF, 80)])
 def test_forced_tile_shapes(shape, dtype, D, monkeypatch):
     # 64, 128 and 256 rows per workgroup (where the head_dim has that shape)
     monkeypatch.setenv("TRINIX_PACKED_FWD", shape)
@@ -98,7 +98,7 @@ def test_forced_tile_shapes(shape, dtype, D, monkeypatch):
 
 
 @pytest.mark.parametrize("splits", ["1", "2", "3", "16"])
-@pytest.mark.parametrize("dtype,D", [(BF, 64), (HF, 128), (BF, 256), (F32, 64)])
+@pytest.mark.parametrize("dtype,D", [(BF, 64), (HF, 128), (BF, 256), (F32, 64), (BF, 80), (F32, 96)])
 def test_heads_shared_out(splits, dtype, D, monkeypatch):
     # the query heads of a KV head over several workgroups, summed in order
     monkeypatch.setenv("TRINIX_PACKED_SPLITS", splits)
@@ -106,7 +106,7 @@ def test_heads_shared_out(splits, dtype, D, monkeypatch):
 
 
 @pytest.mark.parametrize("pairs", ["1", "2"])
-@pytest.mark.parametrize("dtype,D", [(F32, 64), (F32, 128), (F32, 256), (BF, 256), (HF, 256)])
+@pytest.mark.parametrize("dtype,D", [(F32, 64), (F32, 128), (F32, 256), (BF, 256), (HF, 256), (F32, 80), (F32, 96)])
 def test_forced_pairs(pairs, dtype, D, monkeypatch):
     # one or two wavefronts per 32 rows
     monkeypatch.setenv("TRINIX_PACKED_PAIRS", pairs)

@@ -12,8 +12,9 @@
 //                        the lane's column;
 //   accum(acc, tile, x)  acc[k], k < NDB (row d = (db0 + k)*32 + (v/4)*8 + 4g +
 //                        v%4, column l % 32) += sum over tile rows of
-//                        tile[row][d] * x, for the NDB of the D/32 head_dim
+//                        tile[row][d] * x, for the NDB of the C/32 head_dim
 //                        blocks from db0 (a multiple of NDB).
+// Tile rows are D wide, of which the products take the first C columns.
 //
 //   Ops32  fp32 operands on v_mfma_f32_32x32x2f32 (exact products, fp32 sums);
 //          the coefficients keep all 24 bits; an operand element is 4 bytes,
@@ -62,10 +63,10 @@ struct Tile16Reader {
   }
 };
 
-template <class E, int D>
+template <class E, int D, int C = D>
 struct Ops16 {
   using Store = uint16_t;
-  static constexpr int kD = D, DS = D / 16, DB = D / 32;
+  static constexpr int kD = D, kC = C, DS = C / 16, DB = C / 32;
   // Held at 2^kPShift: fp16 terms have a fixed quantum of 2^-24, so P (at
   // most 1) is held times 2^11, and dZ at a power of two of its own (Scale).
   static constexpr bool kScaled = std::is_same<E, F16>::value;
@@ -141,10 +142,10 @@ struct Ops16 {
   }
 };
 
-template <int D>
+template <int D, int C = D>
 struct Ops32 {
   using Store = float;
-  static constexpr int kD = D, DB = D / 32, DT = D / 8;
+  static constexpr int kD = D, kC = C, DB = C / 32, DT = C / 8;
   static constexpr bool kScaled = false;
   static constexpr float kPShift = 0.f;
   struct Frag {

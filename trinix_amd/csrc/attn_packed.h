@@ -23,7 +23,7 @@ struct PackedParams {
   int64_t q_ss, q_sh, k_ss, k_sh, v_ss, v_sh, o_ss, o_sh;
   int64_t do_ss, do_sh, dq_ss, dq_sh, dk_ss, dk_sh, dv_ss, dv_sh;
   int Tq, Hq, Hkv, G;
-  int d;  // columns of every tensor: head_dim, at most the kernel's D
+  int d;  // columns of every tensor: head_dim, at most the kernel's C
   float scale, scale_log2;
   int causal, has_window;
   int64_t wl, wr;  // clamped to +-2^30
@@ -87,13 +87,13 @@ __device__ inline float* packed_partial(const PackedParams& p, int split, int wh
   return p.part + ((((int64_t)split * 2 + which) * p.Tk + row) * p.Hkv + hkv) * D;
 }
 
-// Rows of d columns in kernels of D >= d: the operand in registers is zero from column
+// Rows of d columns in kernels of C >= d: the operand in registers is zero from column
 // d on, so what the other one holds there (a copy of a real unit) adds nothing, and
 // output columns from d on are not written.
 template <class O>
 __device__ inline typename O::Frag load_frag_cols(const typename O::Store* row, int g, int d) {
   typename O::Frag f;
-  constexpr int N = sizeof(f.r) / sizeof(f.r[0]), PER = O::kD / N, HALF = PER / 2;
+  constexpr int N = sizeof(f.r) / sizeof(f.r[0]), PER = O::kC / N, HALF = PER / 2;
 #pragma unroll
   for (int k = 0; k < N; ++k) {
     const int d0 = k * PER + g * HALF;
@@ -159,19 +159,23 @@ constexpr float kLoScale = std::is_same<E, F16>::value ? 2048.f : 1.f;
 // taking alternate key tiles; kPlain 128 rows; kWide 256 rows (head_dim 128).
 enum class PackedShape { kPair, kPlain, kWide };
 
-// Launchers, one translation unit per type (attn_packed_*.hip).  rows: block
-// size of the item list that p.items points at.
-hipError_t launch_packed_fwd_bf16(const PackedParams& p, int D, PackedShape shape, int grid, hipStream_t st);
-hipError_t launch_packed_fwd_f16(const PackedParams& p, int D, PackedShape shape, int grid, hipStream_t st);
-hipError_t launch_packed_fwd_f32(const PackedParams& p, int D, int ks, int grid, hipStream_t st);
+// Columns C that a kernel computes, 64, 96, 128 or 256, and its rows in LDS: those of
+// 96 are 128 wide (the swizzles permute the units of a power of two).
+constexpr int packed_lds_dim(int C) { return C == 96 ? 128 : C; }
+
+// Launchers, one translation unit per type (attn_packed_*.hip); grid: the items of the
+// list at p.items times the heads.  ks: wavefronts per 32 rows or keys.
+hipError_t launch_packed_fwd_bf16(const PackedParams& p, int C, PackedShape shape, int grid, hipStream_t st);
+hipError_t launch_packed_fwd_f16(const PackedParams& p, int C, PackedShape shape, int grid, hipStream_t st);
+hipError_t launch_packed_fwd_f32(const PackedParams& p, int C, int ks, int grid, hipStream_t st);
 // dK and dV, and dQ (16-bit: head_dim 256; 64 and 128 run both in one launch).
 hipError_t launch_packed_dkdv_bf16(const PackedParams& p, int ks, int grid, hipStream_t st);
 hipError_t launch_packed_dkdv_f16(const PackedParams& p, int ks, int grid, hipStream_t st);
-hipError_t launch_packed_dkdv_f32(const PackedParams& p, int D, int ks, int grid, hipStream_t st);
+hipError_t launch_packed_dkdv_f32(const PackedParams& p, int C, int ks, int grid, hipStream_t st);
 hipError_t launch_packed_dq_bf16(const PackedParams& p, int ks, int grid, hipStream_t st);
 hipError_t launch_packed_dq_f16(const PackedParams& p, int ks, int grid, hipStream_t st);
-hipError_t launch_packed_dq_f32(const PackedParams& p, int D, int ks, int grid, hipStream_t st);
-hipError_t launch_packed_bwd_bf16(const PackedParams& p, int D, int n_kv, int n_q, hipStream_t st);
-hipError_t launch_packed_bwd_f16(const PackedParams& p, int D, int n_kv, int n_q, hipStream_t st);
+hipError_t launch_packed_dq_f32(const PackedParams& p, int C, int ks, int grid, hipStream_t st);
+hipError_t launch_packed_bwd_bf16(const PackedParams& p, int C, int n_kv, int n_q, hipStream_t st);
+hipError_t launch_packed_bwd_f16(const PackedParams& p, int C, int n_kv, int n_q, hipStream_t st);
 
 }  // namespace trinix

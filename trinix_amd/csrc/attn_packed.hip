@@ -186,16 +186,16 @@ extern "C" int trinix_packed_fwd(const trinix_packed_args* a, void* stream) {
   if (a->total_q == 0) return TRINIX_OK;
   PackedParams p = params(a);
   hipStream_t st = (hipStream_t)stream;
-  const int D = packed_kernel_dim(a->head_dim);
+  const int C = packed_columns(a->head_dim);
   hipError_t e;
   if (a->dtype == TRINIX_F32) {
     p.rows16 = rows16(a->k, a->k_stride) && rows16(a->v, a->v_stride);
     const int ks = two_per_group(a, a->total_q, a->nheads_q, 1);
-    e = launch_packed_fwd_f32(p, D, ks, (int)(use_list(p, a, ks == 2 ? kRows64 : kRows128) * p.Hq), st);
+    e = launch_packed_fwd_f32(p, C, ks, (int)(use_list(p, a, ks == 2 ? kRows64 : kRows128) * p.Hq), st);
   } else {
     const PackedShape shape = packed_shape(a);
     const int grid = (int)(use_list(p, a, kListOf[(int)shape]) * p.Hq);
-    e = a->dtype == TRINIX_BF16 ? launch_packed_fwd_bf16(p, D, shape, grid, st) : launch_packed_fwd_f16(p, D, shape, grid, st);
+    e = a->dtype == TRINIX_BF16 ? launch_packed_fwd_bf16(p, C, shape, grid, st) : launch_packed_fwd_f16(p, C, shape, grid, st);
   }
   return e == hipSuccess ? TRINIX_OK : TRINIX_ERR_LAUNCH;
 }
@@ -205,7 +205,7 @@ extern "C" int trinix_packed_bwd(const trinix_packed_args* a, void* stream) {
   if (rc != TRINIX_OK) return rc;
   PackedParams p = params(a);
   hipStream_t st = (hipStream_t)stream;
-  const int D = packed_kernel_dim(a->head_dim);
+  const int C = packed_columns(a->head_dim), D = packed_lds_dim(C);
   const bool f32 = a->dtype == TRINIX_F32, bf = a->dtype == TRINIX_BF16;
   hipError_t e = hipSuccess;
   if (f32) p.rows16 = rows16(a->q, a->q_stride) && rows16(a->dout, a->dout_stride);
@@ -216,24 +216,24 @@ extern "C" int trinix_packed_bwd(const trinix_packed_args* a, void* stream) {
   p.Tk = (int)a->total_k;
   p.n_split = packed_head_splits(a);
   p.part = (float*)a->workspace;
-  if (!f32 && D != 256) {
+  if (!f32 && C != 256) {
     const int n_q = (int)(use_list(p, a, kRows128) * p.Hq);
     p.items_q = p.items;
     const int n_kv = (int)(use_list(p, a, kKeys64) * p.Hkv * p.n_split);
     if (n_kv + n_q > 0)
-      e = bf ? launch_packed_bwd_bf16(p, D, n_kv, n_q, st) : launch_packed_bwd_f16(p, D, n_kv, n_q, st);
+      e = bf ? launch_packed_bwd_bf16(p, C, n_kv, n_q, st) : launch_packed_bwd_f16(p, C, n_kv, n_q, st);
   } else {
     if (a->total_k > 0) {
       const int ks = two_per_group(a, a->total_k, a->nheads_kv * p.n_split, p.G / p.n_split);
       const int grid = (int)(use_list(p, a, ks == 2 ? kKeys64 : kKeys128) * p.Hkv * p.n_split);
-      e = f32 ? launch_packed_dkdv_f32(p, D, ks, grid, st) : bf ? launch_packed_dkdv_bf16(p, ks, grid, st) : launch_packed_dkdv_f16(p, ks, grid, st);
+      e = f32 ? launch_packed_dkdv_f32(p, C, ks, grid, st) : bf ? launch_packed_dkdv_bf16(p, ks, grid, st) : launch_packed_dkdv_f16(p, ks, grid, st);
       if (e != hipSuccess) return TRINIX_ERR_LAUNCH;
     }
     if (a->total_q > 0) {
       if (f32) p.rows16 = rows16(a->k, a->k_stride) && rows16(a->v, a->v_stride);
       const int ks = two_per_group(a, a->total_q, a->nheads_q, 1);
       const int grid = (int)(use_list(p, a, ks == 2 ? kRows64 : kRows128) * p.Hq);
-      e = f32 ? launch_packed_dq_f32(p, D, ks, grid, st) : bf ? launch_packed_dq_bf16(p, ks, grid, st) : launch_packed_dq_f16(p, ks, grid, st);
+      e = f32 ? launch_packed_dq_f32(p, C, ks, grid, st) : bf ? launch_packed_dq_bf16(p, ks, grid, st) : launch_packed_dq_f16(p, ks, grid, st);
     }
   }
   if (e == hipSuccess && p.n_split > 1 && a->total_k > 0)

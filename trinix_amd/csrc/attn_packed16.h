@@ -6,13 +6,13 @@
 namespace trinix {
 
 // NW * 32 / KS query rows of one sequence and head (the list's block).
-template <class E, int D, int BN, int NW, int OCC, int KS, int ALIBI>
+template <class E, int C, int BN, int NW, int OCC, int KS, int ALIBI>
 __global__ __launch_bounds__(NW * 64, OCC) void packed_fwd16(const PackedParams p) {
-  constexpr int BM = NW * 32 / KS, DB = D / 32;
+  constexpr int BM = NW * 32 / KS, D = packed_lds_dim(C), DB = C / 32;
   TRINIX_TILE16_LDS(D, BN, KS);
   const PackedBlock w(p, p.items, (int)blockIdx.x, p.Hkv, p.G);
   if (w.blk < 0) return;
-  Tile16<E, D, BN, NW, KS, ALIBI> T(lds_k0, lds_k1, lds_v0, lds_v1);
+  Tile16<E, D, C, BN, NW, KS, ALIBI> T(lds_k0, lds_k1, lds_v0, lds_v1);
   const int hq = w.h, hkv = hq / p.G, m0 = w.blk * BM, iw0 = m0 + (T.wave / KS) * 32, i = iw0 + T.r;
   T.load_q((const uint16_t*)p.q + (int64_t)(w.q0 + min(i, w.lq - 1)) * p.q_ss + hq * p.q_sh, p.d, p.scale_log2,
            ALIBI ? p.alibi[hq * p.al_sh] : 0.f);
@@ -56,27 +56,36 @@ __global__ __launch_bounds__(NW * 64, OCC) void packed_fwd16(const PackedParams 
   if (p.lse && T.g == 0) p.lse[(int64_t)hq * p.Tq + row] = l > 0.f ? (T.m_run + __log2f(l)) * kLn2 : -INFINITY;
 }
 
-template <class E, int D, int BN, int NW, int OCC, int KS>
+template <class E, int C, int BN, int NW, int OCC, int KS>
 hipError_t launch_packed_fwd16(const PackedParams& p, int grid, hipStream_t st) {
   const dim3 g((unsigned)grid), b(NW * 64);
-  if (!p.alibi) return launch_kernel(&packed_fwd16<E, D, BN, NW, OCC, KS, 0>, g, b, 0, st, p);
+  if (!p.alibi) return launch_kernel(&packed_fwd16<E, C, BN, NW, OCC, KS, 0>, g, b, 0, st, p);
   // (a causal row sees no key behind it; 128-key tiles and head_dim 256 have no registers for 2)
-  if constexpr (BN <= 64 && D <= 128)
-    if (p.causal) return launch_kernel(&packed_fwd16<E, D, BN, NW, OCC, KS, 2>, g, b, 0, st, p);
-  return launch_kernel(&packed_fwd16<E, D, BN, NW, OCC, KS, 1>, g, b, 0, st, p);
+  if constexpr (BN <= 64 && C <= 128)
+    if (p.causal) return launch_kernel(&packed_fwd16<E, C, BN, NW, OCC, KS, 2>, g, b, 0, st, p);
+  return launch_kernel(&packed_fwd16<E, C, BN, NW, OCC, KS, 1>, g, b, 0, st, p);
+}
+
+template <class E, int C>
+hipError_t launch_packed_fwd16_128(const PackedParams& p, PackedShape shape, int grid, hipStream_t st) {
+  switch (shape) {
+    case PackedShape::kPair: return launch_packed_fwd16<E, C, 32, 4, 2, 2>(p, grid, st);
+    case PackedShape::kPlain: return launch_packed_fwd16<E, C, 64, 4, 2, 1>(p, grid, st);
+    case PackedShape::kWide: return launch_packed_fwd16<E, C, 128, 8, 2, 1>(p, grid, st);
+  }
+  return hipErrorNotSupported;
 }
 
 // 64-key tiles of 4 wavefronts, two per SIMD (head_dim 256: one); kPair at
 // head_dim 128 on 32-key tiles, in the same LDS (at 256 it would spill); kWide
 // 128-key tiles of 8.
 template <class E>
-hipError_t launch_packed_fwd16(const PackedParams& p, int D, PackedShape shape, int grid, hipStream_t st) {
+hipError_t launch_packed_fwd16(const PackedParams& p, int C, PackedShape shape, int grid, hipStream_t st) {
   const bool pair = shape == PackedShape::kPair;
-  switch (D) {
+  switch (C) {
     case 64: return pair ? launch_packed_fwd16<E, 64, 64, 4, 2, 2>(p, grid, st) : launch_packed_fwd16<E, 64, 64, 4, 2, 1>(p, grid, st);
-    case 128:
-      if (shape == PackedShape::kWide) return launch_packed_fwd16<E, 128, 128, 8, 2, 1>(p, grid, st);
-      return pair ? launch_packed_fwd16<E, 128, 32, 4, 2, 2>(p, grid, st) : launch_packed_fwd16<E, 128, 64, 4, 2, 1>(p, grid, st);
+    case 96: return launch_packed_fwd16_128<E, 96>(p, shape, grid, st);
+    case 128: return launch_packed_fwd16_128<E, 128>(p, shape, grid, st);
     case 256: return launch_packed_fwd16<E, 256, 64, 4, 1, 1>(p, grid, st);
   }
   return hipErrorNotSupported;

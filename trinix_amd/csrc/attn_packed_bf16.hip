@@ -5,11 +5,11 @@
 
 namespace trinix {
 
-hipError_t launch_packed_fwd_bf16(const PackedParams& p, int D, PackedShape shape, int grid, hipStream_t st) {
-  return launch_packed_fwd16<BF16>(p, D, shape, grid, st);
+hipError_t launch_packed_fwd_bf16(const PackedParams& p, int C, PackedShape shape, int grid, hipStream_t st) {
+  return launch_packed_fwd16<BF16>(p, C, shape, grid, st);
 }
-hipError_t launch_packed_bwd_bf16(const PackedParams& p, int D, int n_kv, int n_q, hipStream_t st) {
-  return launch_packed_bwd16<BF16>(p, D, n_kv, n_q, st);
+hipError_t launch_packed_bwd_bf16(const PackedParams& p, int C, int n_kv, int n_q, hipStream_t st) {
+  return launch_packed_bwd16<BF16>(p, C, n_kv, n_q, st);
 }
 hipError_t launch_packed_dkdv_bf16(const PackedParams& p, int ks, int grid, hipStream_t st) {
   using O = Ops16<BF16, 256>;

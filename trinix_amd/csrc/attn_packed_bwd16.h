@@ -42,12 +42,12 @@ struct PackedBwdLds {
   static constexpr int kBytes = kKv > kDq ? kKv : kDq;
 };
 
-template <class E, int D>
+template <class E, int D, int C>
 __device__ __forceinline__ void packed_dkdv_body(const PackedParams& p, const PackedBlock& w, char* pool) {
-  using O = Ops16<E, D>;
+  using O = Ops16<E, D, C>;
   using L = PackedBwdLds<D>;
   constexpr int NG = L::NG, NW = 2 * NG, BK = NG * 32, BQ = kTileRows, NSL = L::NSL;
-  constexpr int DS = D / 16, DB = D / 32, UPR = D / 8, LPW = BQ * UPR / (64 * NW);
+  constexpr int DS = C / 16, DB = C / 32, UPR = D / 8, LPW = BQ * UPR / (64 * NW);
   constexpr int RPF = 4, TPF = 2;  // row and transpose reads ahead of their MFMA
   static_assert(LPW >= 1 && BQ * UPR % (64 * NW) == 0, "tile shape");
   char* const lds_q = pool;
@@ -290,11 +290,11 @@ __device__ __forceinline__ void packed_dkdv_body(const PackedParams& p, const Pa
   else run(std::false_type{});
 }
 
-template <class E, int D>
+template <class E, int D, int C>
 __device__ __forceinline__ void packed_dq_body(const PackedParams& p, const PackedBlock& w, char* pool) {
-  using O = Ops16<E, D>;
+  using O = Ops16<E, D, C>;
   using L = PackedBwdLds<D>;
-  constexpr int NG = L::NG, BM = NG * 64, DB = D / 32, TILE = kTileRows * D * 2, NT = L::KT;  // tiles per step
+  constexpr int NG = L::NG, BM = NG * 64, DB = C / 32, TILE = kTileRows * D * 2, NT = L::KT;  // tiles per step
   char* const lds_k = pool;
   char* const lds_v = pool + 2 * NT * TILE;
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, g = lane >> 5;
@@ -383,24 +383,29 @@ __device__ __forceinline__ void packed_dq_body(const PackedParams& p, const Pack
 }
 
 // Workgroups [0, n_kv): dK and dV of p.items; behind them dQ of p.items_q.
-template <class E, int D>
+template <class E, int C>
 __global__ __launch_bounds__(256, 2) void packed_bwd16(const PackedParams p, int n_kv) {
+  constexpr int D = packed_lds_dim(C);
   __shared__ __attribute__((aligned(1024))) char pool[PackedBwdLds<D>::kBytes];
   const int wg = (int)blockIdx.x;
   if (wg < n_kv) {
     const PackedBlock w(p, p.items, wg, p.Hkv * p.n_split, 1);
-    if (w.blk >= 0) packed_dkdv_body<E, D>(p, w, pool);
+    if (w.blk >= 0) packed_dkdv_body<E, D, C>(p, w, pool);
   } else {
     const PackedBlock w(p, p.items_q, wg - n_kv, p.Hkv, p.G);
-    if (w.blk >= 0) packed_dq_body<E, D>(p, w, pool);
+    if (w.blk >= 0) packed_dq_body<E, D, C>(p, w, pool);
   }
 }
 
 template <class E>
-hipError_t launch_packed_bwd16(const PackedParams& p, int D, int n_kv, int n_q, hipStream_t st) {
+hipError_t launch_packed_bwd16(const PackedParams& p, int C, int n_kv, int n_q, hipStream_t st) {
   const dim3 grid((unsigned)(n_kv + n_q)), block(256);
-  return D == 64 ? launch_kernel(&packed_bwd16<E, 64>, grid, block, 0, st, p, n_kv)
-                 : launch_kernel(&packed_bwd16<E, 128>, grid, block, 0, st, p, n_kv);
+  switch (C) {
+    case 64: return launch_kernel(&packed_bwd16<E, 64>, grid, block, 0, st, p, n_kv);
+    case 96: return launch_kernel(&packed_bwd16<E, 96>, grid, block, 0, st, p, n_kv);
+    case 128: return launch_kernel(&packed_bwd16<E, 128>, grid, block, 0, st, p, n_kv);
+  }
+  return hipErrorNotSupported;
 }
 
 }  // namespace trinix

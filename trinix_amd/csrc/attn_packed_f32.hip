@@ -4,12 +4,15 @@
 namespace trinix {
 
 // ks: wavefronts per 32 rows (keys); head_dim 256 (registers, LDS): 1
-hipError_t launch_packed_fwd_f32(const PackedParams& p, int D, int ks, int grid, hipStream_t st) {
+hipError_t launch_packed_fwd_f32(const PackedParams& p, int C, int ks, int grid, hipStream_t st) {
   const dim3 g((unsigned)grid), b(256);
-  switch (D) {
+  switch (C) {
     case 64:
       return ks == 2 ? launch_kernel(&packed_fwd_f32<Ops32<64>, 2, 2>, g, b, 0, st, p)
                      : launch_kernel(&packed_fwd_f32<Ops32<64>, 2, 1>, g, b, 0, st, p);
+    case 96:
+      return ks == 2 ? launch_kernel(&packed_fwd_f32<Ops32<128, 96>, 1, 2>, g, b, 0, st, p)
+                     : launch_kernel(&packed_fwd_f32<Ops32<128, 96>, 1, 1>, g, b, 0, st, p);
     case 128:
       return ks == 2 ? launch_kernel(&packed_fwd_f32<Ops32<128>, 1, 2>, g, b, 0, st, p)
                      : launch_kernel(&packed_fwd_f32<Ops32<128>, 1, 1>, g, b, 0, st, p);
@@ -17,20 +20,24 @@ hipError_t launch_packed_fwd_f32(const PackedParams& p, int D, int ks, int grid,
   }
   return hipErrorNotSupported;
 }
-hipError_t launch_packed_dkdv_f32(const PackedParams& p, int D, int ks, int grid, hipStream_t st) {
-  switch (D) {
+hipError_t launch_packed_dkdv_f32(const PackedParams& p, int C, int ks, int grid, hipStream_t st) {
+  switch (C) {
     case 64:
       return ks == 2 ? launch_packed_dkdv_g<Ops32<64>, 2, 1, 2>(p, grid, st) : launch_packed_dkdv_g<Ops32<64>, 2, 1, 1>(p, grid, st);
+    case 96:
+      return ks == 2 ? launch_packed_dkdv_g<Ops32<128, 96>, 1, 1, 2>(p, grid, st) : launch_packed_dkdv_g<Ops32<128, 96>, 1, 1, 1>(p, grid, st);
     case 128:
       return ks == 2 ? launch_packed_dkdv_g<Ops32<128>, 1, 1, 2>(p, grid, st) : launch_packed_dkdv_g<Ops32<128>, 1, 1, 1>(p, grid, st);
     case 256: return launch_packed_dkdv_g<Ops32<256>, 1, 4, 1>(p, grid, st);  // K and V rows fill the registers
   }
   return hipErrorNotSupported;
 }
-hipError_t launch_packed_dq_f32(const PackedParams& p, int D, int ks, int grid, hipStream_t st) {
-  switch (D) {
+hipError_t launch_packed_dq_f32(const PackedParams& p, int C, int ks, int grid, hipStream_t st) {
+  switch (C) {
     case 64:
       return ks == 2 ? launch_packed_dq_g<Ops32<64>, 2, 1, 2>(p, grid, st) : launch_packed_dq_g<Ops32<64>, 2, 1, 1>(p, grid, st);
+    case 96:
+      return ks == 2 ? launch_packed_dq_g<Ops32<128, 96>, 1, 1, 2>(p, grid, st) : launch_packed_dq_g<Ops32<128, 96>, 1, 1, 1>(p, grid, st);
     case 128:
       return ks == 2 ? launch_packed_dq_g<Ops32<128>, 1, 1, 2>(p, grid, st) : launch_packed_dq_g<Ops32<128>, 1, 1, 1>(p, grid, st);
     case 256: return launch_packed_dq_g<Ops32<256>, 1, 2, 1>(p, grid, st);

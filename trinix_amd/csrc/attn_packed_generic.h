@@ -22,7 +22,7 @@ namespace trinix {
 template <class O, int OCC, int KS>
 __global__ __launch_bounds__(256, OCC) void packed_fwd_f32(const PackedParams p) {
   using Store = typename O::Store;
-  constexpr int NW = 4, BM = NW * 32 / KS, D = O::kD, DB = D / 32, TILE = kTileRows * D * (int)sizeof(Store);
+  constexpr int NW = 4, BM = NW * 32 / KS, D = O::kD, DB = O::DB, TILE = kTileRows * D * (int)sizeof(Store);
   __shared__ __attribute__((aligned(1024))) char lds_k[2][KS * TILE];
   __shared__ __attribute__((aligned(1024))) char lds_v[2][KS * TILE];
   const PackedBlock w(p, p.items, (int)blockIdx.x, p.Hkv, p.G);

@@ -39,7 +39,7 @@ constexpr int kTile16Words = KS * BN * D;
 // hold only pairs that every row of the workgroup may see.  A lane's row sees
 // keys jlo .. jlo + jspan (jlo = INT_MAX: none); keys outside [wlo, whi] are seen
 // by no row of the wavefront.  pos: position of the lane's row among the keys (ALiBi).
-// Rows hold d <= D columns (a multiple of 8): q is zero from there on in registers, and
+// Rows hold d <= C columns (a multiple of 8): q is zero from there on in registers, and
 // K and V units from there on are copies of the row's last one.
 struct KeyRun {
   const uint16_t* k;
@@ -58,11 +58,12 @@ struct KeyRun {
 // operand of the first product, no instruction of its own), and its part of the whole
 // tile joins the maximum in the exponential's FMA (32 heads of 128, ten ragged prompts of
 // 8326 rows: 144 us with 1, 135 with 2, 126 without ALiBi).
-template <class E, int D, int BN, int NW, int KS, int ALIBI>
+// The products take the first C of a tile's D columns.
+template <class E, int D, int C, int BN, int NW, int KS, int ALIBI>
 struct Tile16 {
-  static constexpr int DS = D / 16;    // MFMA k-steps over head_dim
+  static constexpr int DS = C / 16;    // MFMA k-steps over head_dim
   static constexpr int NB = BN / 32;   // 32-key blocks per tile
-  static constexpr int DB = D / 32;    // 32-wide head_dim blocks of O^T
+  static constexpr int DB = C / 32;    // 32-wide head_dim blocks of O^T
   static constexpr int UPR = D / 8;    // 16-byte units per row
   static constexpr int LPW = BN * UPR / (64 * NW);  // copies per wavefront and tile (K or V)
   static constexpr float TAU = 8.f;
@@ -345,7 +346,7 @@ struct Tile16 {
   // afterwards kp == 0 holds the row).  Every wavefront of the workgroup calls it.
   __device__ __forceinline__ float finish() {
     if constexpr (KS == 2) {
-      constexpr int HB = BN == 32 ? DB / 2 : DB;  // head_dim blocks per K buffer
+      constexpr int HB = BN == 32 ? (DB + 1) / 2 : DB;  // head_dim blocks per K buffer
       static_assert(NW / 2 * HB * 16 * 64 * 4 <= KS * BN * D * 2, "exchange fits the K buffers");
       const int rg = wave / 2;
       auto mo = [&](int db, int v) __attribute__((always_inline)) -> float* {

@@ -9,6 +9,11 @@ namespace trinix {
 // head_dim that a call's kernels are built for (at least the tensors'), and whether
 // they take it: multiples of 8, fp32 of 4, up to 256.
 inline int packed_kernel_dim(int64_t head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
+// Columns that the packed-sequence kernels compute: 96 of 128 where that is enough
+// (us, forward and forward with backward, all 128 | 96: 8 heads of 80, 1090 rows in five
+// documents, fp32 44 and 176 | 36 and 143; bf16 32/8 heads of 96, 8192 rows 500 and 2815 |
+// 426 and 2384; 12 heads of 96, 1024 rows 19.5 and 69.8 | 17.8 and 62.6).
+inline int packed_columns(int64_t head_dim) { return head_dim > 64 && head_dim <= 96 ? 96 : packed_kernel_dim(head_dim); }
 inline bool packed_head_dim_ok(int64_t head_dim, int32_t dtype) {
   return head_dim > 0 && head_dim <= 256 && head_dim % (dtype == TRINIX_F32 ? 4 : 8) == 0;
 }

@@ -330,7 +330,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void shared_split(const Shar
   const int blk = (int)blockIdx.x;
   const Item it = blk < p.wg_p ? prefix_item(p, blk, BM) : own_item(p, blk - p.wg_p, BM);
   if (it.c0 >= it.c1) return;
-  Tile16<E, D, BN, 4, KS, 0> T(lds_k0, lds_k1, lds_v0, lds_v1);
+  Tile16<E, D, D, BN, 4, KS, 0> T(lds_k0, lds_k1, lds_v0, lds_v1);
   const int rw = it.r0 + (T.wave / KS) * 32;
   const TileRow row(p, rw, it.r1, T.lane, it.hkv);
   T.load_q(row.q(p), p.d, p.scale_log2, 0.f);
@@ -364,7 +364,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void shared_whole(const Shar
   const int per = p.Sq * p.G, groups = (per + BM - 1) / BM;
   const int w = xcd_remap((int)blockIdx.x, p.Hkv * p.B * groups);
   const int hkv = w / (p.B * groups), b = w / groups % p.B, r0 = b * per + w % groups * BM, r1 = min(r0 + BM, (b + 1) * per);
-  Tile16<E, D, BN, 4, KS, 0> T(lds_k0, lds_k1, lds_v0, lds_v1);
+  Tile16<E, D, D, BN, 4, KS, 0> T(lds_k0, lds_k1, lds_v0, lds_v1);
   const int rw = r0 + (T.wave / KS) * 32;
   const TileRow row(p, rw, r1, T.lane, hkv);
   T.load_q(row.q(p), p.d, p.scale_log2, 0.f);
