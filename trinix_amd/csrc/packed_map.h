@@ -9,14 +9,14 @@
 
 namespace trinix {
 
-// A plan holds six lists of work items: blocks of 64, 128 and 256 query rows
-// (lists 0..2) and of 64, 128 and 256 keys (lists 3..5) of one sequence each,
-// the longest first.  An item is eight int32:
+// A plan holds five lists of work items: blocks of 64, 128 and 256 query rows
+// (lists 0..2) and of 64 and 128 keys (lists 3, 4) of one sequence each, the
+// longest first.  An item is eight int32:
 //   first query row, query rows, first key, keys of its sequence; block number
 //   (-1: no item); sequence; two zeros.
 // Rows behind the last sequence form a sequence of their own without keys
 // (their output is 0), keys behind it one without rows (their gradients are 0).
-constexpr int kPackedLists = 6;
+constexpr int kPackedLists = 5;
 constexpr int kPackedItemInts = 8;
 __host__ __device__ inline int packed_list_block(int list) { return 64 << (list % 3); }
 __host__ __device__ inline bool packed_list_is_keys(int list) { return list >= 3; }

@@ -8,7 +8,7 @@
 // item then finds its sequence by bisection and is placed by a counting sort on
 // its cost, 1024 classes, the longest first (items of one class in any order:
 // it changes when an item runs, not its result).
-// Latency bound: about 10 us for ten sequences of 8192 rows, once per batch.
+// Latency bound, once per batch: 11 us for ten sequences of 8326 rows, 44 us for 4000 of 3.
 #include "common.h"
 #include "packed_map.h"
 #include "trinix_attn.h"
@@ -25,23 +25,32 @@ struct PlanParams {
   int n_seqs, total_q, total_k;
 };
 
-// Inclusive scan over the workgroup; every thread calls it.
+// Inclusive scan over the workgroup, and the result of all of it; every thread calls
+// it.  Within the wavefronts first, then over their results.
 template <class F>
-__device__ inline int block_scan(int x, int* lds, F op) {
-  const int t = threadIdx.x;
-  lds[t] = x;
-  __syncthreads();
-  for (int d = 1; d < kPlanThreads; d <<= 1) {
-    const int y = t >= d ? op(lds[t - d], x) : x;
-    __syncthreads();
-    lds[t] = x = y;
-    __syncthreads();
+__device__ inline int block_scan(int x, int* lds, F op, int& all) {
+  constexpr int NW = kPlanThreads / 64;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int y = __shfl_up(x, d);
+    if (lane >= d) x = op(y, x);
   }
+  __syncthreads();  // the last call's results are read
+  if (lane == 63) lds[wave] = x;
+  __syncthreads();
+  int sum = lds[0];
+#pragma unroll
+  for (int w = 1; w < NW; ++w) {
+    if (w == wave) x = op(sum, x);
+    sum = op(sum, lds[w]);
+  }
+  all = sum;
   return x;
 }
 
 __global__ __launch_bounds__(kPlanThreads) void packed_plan_kernel(const PlanParams p) {
-  __shared__ int scan[kPlanThreads];
+  __shared__ int scan[kPlanThreads / 64];
   __shared__ int hist[kPlanThreads];
   __shared__ int most;
   const int list = blockIdx.x, t = threadIdx.x, n = p.n_seqs;
@@ -60,12 +69,8 @@ __global__ __launch_bounds__(kPlanThreads) void packed_plan_kernel(const PlanPar
       q = larger(q, imin(p.cu_q[i], p.total_q));
       k = larger(k, imin(p.cu_k[i], p.total_k));
     }
-    q = block_scan(q, scan, larger);
-    top_q = scan[kPlanThreads - 1];
-    __syncthreads();
-    k = block_scan(k, scan, larger);
-    top_k = scan[kPlanThreads - 1];
-    __syncthreads();
+    q = block_scan(q, scan, larger, top_q);
+    k = block_scan(k, scan, larger, top_k);
     if (i <= n) cq[i] = q, ck[i] = k;
   }
   __syncthreads();
@@ -74,9 +79,9 @@ __global__ __launch_bounds__(kPlanThreads) void packed_plan_kernel(const PlanPar
   for (int base = 0; base < n + 2; base += kPlanThreads) {
     const int s = base + t;
     const int nb = s < n + 2 ? packed_blocks(packed_seq(s, n, cq, ck, p.total_q, p.total_k), list) : 0;
-    const int end = count + block_scan(nb, scan, plus);
-    count += scan[kPlanThreads - 1];
-    __syncthreads();
+    int all;
+    const int end = count + block_scan(nb, scan, plus, all);
+    count += all;
     if (s < n + 2) first[s] = end - nb;
   }
   if (t == 0) most = 1;
@@ -111,7 +116,8 @@ __global__ __launch_bounds__(kPlanThreads) void packed_plan_kernel(const PlanPar
   }
   __syncthreads();
   const int mine = hist[t];
-  const int upto = block_scan(mine, scan, plus);
+  int all;
+  const int upto = block_scan(mine, scan, plus, all);
   hist[t] = upto - mine;
   __syncthreads();
   typedef int i32x4 __attribute__((ext_vector_type(4)));
