@@ -309,6 +309,21 @@ def test_rebuild_between_forward_and_backward_is_refused():
         out.sum().backward()
 
 
+def test_second_derivatives_and_gradients_of_slopes_are_refused():
+    q, k, v = (torch.randn(20, 2, 64, device=DEV).to(BF).requires_grad_(True) for _ in range(3))
+    seqs = tx.PackedSequences([0, 9, 20])
+    slopes = torch.tensor([0.5, 0.25], device=DEV, requires_grad=True)
+    for _ in range(2):  # (the second call finds the first one's arguments)
+        with pytest.raises(ValueError):
+            tx.packed_attn_func(q, k, v, seqs, causal=True, alibi_slopes=slopes)
+        tx.packed_attn_func(q, k, v, seqs, causal=True, alibi_slopes=slopes.detach())
+    with torch.no_grad():
+        tx.packed_attn_func(q, k, v, seqs, causal=True, alibi_slopes=slopes)
+    (dq,) = torch.autograd.grad(tx.packed_attn_func(q, k, v, seqs).float().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError):
+        dq.float().sum().backward()
+
+
 def test_refusals():
     x = torch.randn(20, 4, 64, device=DEV).to(BF)
     seqs = tx.PackedSequences([0, 9, 20])

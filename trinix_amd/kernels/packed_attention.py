@@ -14,6 +14,7 @@ import ctypes
 from typing import Optional, Sequence, Tuple, Union
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import _native as nat
 from .attention_kernel import _DTYPE_CODE, KERNEL_HEAD_DIMS, TritonAttentionKernel, current_stream_ptr, kernel_head_dim
@@ -172,24 +173,6 @@ def _check(q, k, v, seqs: PackedSequences, alibi_slopes) -> None:
         raise ValueError(f"alibi_slopes shape {tuple(alibi_slopes.shape)} must be (H,) or (1, H)")
 
 
-def _args(q, k, v, seqs, scale, causal, window_size, slopes) -> nat.PackedArgs:
-    a = nat.PackedArgs()
-    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    a.q_stride, a.k_stride, a.v_stride = (nat.Int64x3(*_strides(t)) for t in (q, k, v))
-    a.plan, a.plan_bytes = seqs.plan.data_ptr(), seqs._bytes
-    a.n_seqs, a.total_q, a.total_k = seqs.n_seqs, seqs.total_q, seqs.total_k
-    a.nheads_q, a.nheads_kv, a.head_dim = q.shape[1], k.shape[1], q.shape[2]
-    a.dtype = _DTYPE_CODE[q.dtype]
-    a.softmax_scale = scale
-    a.causal = 1 if causal else 0
-    if window_size is not None:
-        a.has_window = 1
-        a.window_left, a.window_right = int(window_size[0]), int(window_size[1])
-    if slopes is not None:
-        a.alibi_slopes, a.alibi_stride = slopes.data_ptr(), 1
-    return a
-
-
 # Launch cache (see attention_kernel.py), kept with the sequences: a call whose
 # operands the kernels read in place is described, apart from its pointers, by
 # shapes, strides, types and scalars.  The first one goes through every check and
@@ -216,11 +199,11 @@ def _launch(fn: str, a: nat.PackedArgs, device: torch.device) -> None:
 def _run(a, q, slopes, want_lse, keep):
     """Allocates the outputs of a forward (arguments a, operands set) and launches
     it: (out at the kernel's head_dim, out_lo, lse)."""
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     a.out = out.data_ptr()
     out_lo = lse = None
     if keep and q.dtype != torch.float32:
-        out_lo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out_lo = torch.empty_like(out)
         a.out_lo = out_lo.data_ptr()
     if want_lse or keep:
         lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device)
@@ -247,13 +230,14 @@ class _PackedAttention(torch.autograd.Function):
         return res
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout, *unused):
         q, k, v, out, out_lo, lse, slopes = ctx.saved_tensors
         ent, fwd, seqs, generation, D = ctx.call
         if seqs.generation != generation:
             raise RuntimeError("the packed sequences were rebuilt between the forward and its backward")
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        delta = torch.empty(lse.shape, dtype=torch.float32, device=lse.device)
+        dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
+        delta = torch.empty_like(lse)
         tpl = None
         if ent is not None and dout.dtype == q.dtype and not dout.data_ptr() % 16:
             tpl = ent.bwd.get(dout.stride())
@@ -320,6 +304,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sequence
     if window_size is not None:
         window_size = (int(window_size[0]), int(window_size[1]))
     grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
+    if alibi_slopes is not None and alibi_slopes.requires_grad and torch.is_grad_enabled():
+        raise ValueError("alibi_slopes are constants without a gradient; pass alibi_slopes.detach()")
     key = (q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), q.dtype, k.dtype, v.dtype, q.device, k.device,
            v.device, scale, bool(causal), window_size,
            None if alibi_slopes is None else (alibi_slopes.shape, alibi_slopes.dtype, alibi_slopes.stride(), alibi_slopes.device))

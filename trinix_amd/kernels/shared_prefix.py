@@ -47,10 +47,10 @@ def _operand(t: torch.Tensor, d_kernel: int) -> torch.Tensor:
 # in place is described, apart from its pointers, by shapes, strides, types and
 # scalars.  The first one goes through every check and leaves its arguments here.
 class _Launch:
-    __slots__ = ("args", "out_shape", "lse_shape", "ws_bytes")
+    __slots__ = ("args", "lse_shape", "ws_bytes")
 
-    def __init__(self, args, out_shape, lse_shape, ws_bytes):
-        self.args, self.out_shape, self.lse_shape, self.ws_bytes = args, out_shape, lse_shape, ws_bytes
+    def __init__(self, args, lse_shape, ws_bytes):
+        self.args, self.lse_shape, self.ws_bytes = args, lse_shape, ws_bytes
 
 
 _LAUNCHES: dict = {}
@@ -123,13 +123,13 @@ def _full(key, ts, seq_lens, scale, return_lse):
     a.batch, a.seqlen_q, a.prefix_len, a.capacity = B, Sq, prefix_k.shape[0], S
     a.nheads_q, a.nheads_kv, a.head_dim, a.dtype = H, Hkv, d_kernel, _DTYPE_CODE[q.dtype]
     a.softmax_scale = float(D ** -0.5 if scale is None else scale)
-    ent = _Launch(nat.SharedPrefixArgs.from_buffer_copy(a), (B, Sq, H, d_kernel), lse_shape, None)
+    ent = _Launch(nat.SharedPrefixArgs.from_buffer_copy(a), lse_shape, None)
     lens = None
     if seq_lens is not None:
         lens = seq_lens.to(torch.int32).contiguous()
         a.seq_lens = lens.data_ptr()
     a.q, a.prefix_k, a.prefix_v, a.k, a.v = (t.data_ptr() for t in ops)
-    res = _run(a, ent, q)
+    res = _run(a, ent, ops[0])
     if all(x is y for x, y in zip(ops, ts)) and lens is seq_lens:  # read in place
         if len(_LAUNCHES) >= _MAX_LAUNCHES:
             _LAUNCHES.clear()
@@ -142,13 +142,14 @@ def _full(key, ts, seq_lens, scale, return_lse):
 
 
 def _run(a: nat.SharedPrefixArgs, ent: _Launch, q: torch.Tensor):
-    """Allocates out, lse and the workspace and launches; ent.ws_bytes None: asks for it first."""
+    """Allocates out (shaped as q), lse and the workspace and launches; ent.ws_bytes None:
+    asks for it first."""
     device = q.device
     if torch.cuda.current_device() != device.index:
         with torch.cuda.device(device):
             return _run(a, ent, q)
     lib = nat.load_library()
-    out = torch.empty(ent.out_shape, dtype=q.dtype, device=device)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     a.out = out.data_ptr()
     lse = None
     if ent.lse_shape is not None:

@@ -126,7 +126,7 @@ def packed_attn_func(
             a chunk of a prompt attends to its cache and to itself.
         window_size: (left, right): keys with
             -left <= j - (i + Lk - Lq) <= right.
-        alibi_slopes: (H,) or (1, H); adds ``-slope * |i + Lk - Lq - j|``.
+        alibi_slopes: (H,) or (1, H) constants; adds ``-slope * |i + Lk - Lq - j|``.
         return_lse: also return the fp32 (num_heads, total_q) log-sum-exp.
 
     Returns:
@@ -136,10 +136,16 @@ def packed_attn_func(
         log-sum-exp of -inf, where ``triton_attn_func`` gives NaN: packed
         batches hold such rows by design.
 
+    A graph captured around the forward and its backward takes q, k and v that
+    no living eager autograd graph holds as leaves (``detach()`` makes such), as
+    any captured backward does.
+
     Raises:
-        ValueError: non-GPU tensors, inconsistent shapes, types or devices.
-        RuntimeError: the HIP kernel library or a gfx950 GPU is unavailable, or
-            the sequences were rebuilt between a forward and its backward.
+        ValueError: non-GPU tensors, inconsistent shapes, types or devices,
+            slopes that require a gradient.
+        RuntimeError: the HIP kernel library or a gfx950 GPU is unavailable,
+            the sequences were rebuilt between a forward and its backward, or a
+            second derivative is asked for.
     """
     return packed_attention(q, k, v, sequences, softmax_scale, causal, window_size, alibi_slopes, return_lse)
 
