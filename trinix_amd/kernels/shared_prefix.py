@@ -69,7 +69,8 @@ def shared_prefix_attention(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: t
                             return_lse: bool = False):
     """``shared_prefix_attn_func`` (``layers/attention/functional.py``)."""
     ts = (q, prefix_k, prefix_v, k, v)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
+    if torch.is_grad_enabled() and (q.requires_grad or prefix_k.requires_grad or prefix_v.requires_grad or k.requires_grad
+                                    or v.requires_grad):
         raise ValueError("shared_prefix_attention has no backward; call it under torch.no_grad()")
     key = _key(*ts, seq_lens, scale, return_lse)
     ent = _LAUNCHES.get(key)
