@@ -33,7 +33,8 @@ struct PackedParams {
   // and dK, key, KV head, head_dim), or 1 and null
   int n_split, Tk;
   float* part;
-  int rows16;             // fp32: q, k, v and dout take 16-byte copies
+  int rows16;             // fp32: the tiles' tensors take 16-byte copies (of dK, dV: q and dout)
+  int rows16_q;           // the same of the backward's dQ: k and v
   const int32_t* items;   // of the launch's list
   const int32_t* items_q; // of its second one (packed_bwd16)
 };
@@ -164,17 +165,12 @@ enum class PackedShape { kPair, kPlain, kWide };
 constexpr int packed_lds_dim(int C) { return C == 96 ? 128 : C; }
 
 // Launchers, one translation unit per type (attn_packed_*.hip); grid: the items of the
-// list at p.items times the heads.  ks: wavefronts per 32 rows or keys.
+// list at p.items times the heads.  ks: wavefronts per 32 rows (keys).
 hipError_t launch_packed_fwd_bf16(const PackedParams& p, int C, PackedShape shape, int grid, hipStream_t st);
 hipError_t launch_packed_fwd_f16(const PackedParams& p, int C, PackedShape shape, int grid, hipStream_t st);
 hipError_t launch_packed_fwd_f32(const PackedParams& p, int C, int ks, int grid, hipStream_t st);
-// dK and dV, and dQ (16-bit: head_dim 256; 64 and 128 run both in one launch).
-hipError_t launch_packed_dkdv_bf16(const PackedParams& p, int ks, int grid, hipStream_t st);
-hipError_t launch_packed_dkdv_f16(const PackedParams& p, int ks, int grid, hipStream_t st);
-hipError_t launch_packed_dkdv_f32(const PackedParams& p, int C, int ks, int grid, hipStream_t st);
-hipError_t launch_packed_dq_bf16(const PackedParams& p, int ks, int grid, hipStream_t st);
-hipError_t launch_packed_dq_f16(const PackedParams& p, int ks, int grid, hipStream_t st);
-hipError_t launch_packed_dq_f32(const PackedParams& p, int C, int ks, int grid, hipStream_t st);
+// Backward, one launch: n_kv workgroups of dK and dV, n_q of dQ.
+hipError_t launch_packed_bwd_f32(const PackedParams& p, int C, int ks, int n_kv, int n_q, hipStream_t st);
 hipError_t launch_packed_bwd_bf16(const PackedParams& p, int C, int n_kv, int n_q, hipStream_t st);
 hipError_t launch_packed_bwd_f16(const PackedParams& p, int C, int n_kv, int n_q, hipStream_t st);
 

@@ -156,23 +156,18 @@ PackedShape packed_shape(const trinix_packed_args* a) {
   return s;
 }
 
-// Wavefronts per 32 rows (or keys) of the fp32 kernels and of the gradients at
-// head_dim 256; `chain`: heads that a block walks one after the other.  Measured,
-// forward and backward, us one | two:
-//  - fp32: two wins wherever blocks are few or sequences short (D=128 8 heads 1090 rows 321
-//    | 183; D=64 12 heads 4 x 1024 459 | 316, 24 x 100 99 | 82; 16/4 heads of 128 200 x 40 674
-//    | 482) and loses where long sequences fill the chip (D=64 16 heads 8 x 2048, 2112
-//    blocks, 2471 | 2541; even at 1560);
-//  - bf16 D=256, whose workgroup fills a CU either way: only chains worth halving (8/4
-//    heads 2048 + 1000 340 | 294; 16/4 4 x 1000: dK, dV in two 413 | 352, dQ as well 372; 8/4
-//    3 x 1000 201 | 206, 9 x 300 111 | 129).
+// Wavefronts per 32 rows (keys) of the fp32 kernels.  Measured, forward | forward with
+// backward, us one, two: two wins wherever blocks are few or sequences short (8 heads of
+// 128, 1090 rows 78, 44 | 219, 131; 12 heads of 64, 4 x 1024 109, 73 | 354, 302, 24 x 100
+// 23, 18 | 83, 72; 16/4 heads of 128, 200 x 40 160, 124 | 616, 441) and loses where long
+// sequences fill the chip (8 x 2048, 2112 blocks, 16 heads of 64 555, 580 | 2491, 2601, 16/4
+// of 96 886, 1072 | 3928, 4289; even at 1560).
 // TRINIX_PACKED_PAIRS = 1, 2 forces either (tuning and tests).
-int two_per_group(const trinix_packed_args* a, int64_t total, int64_t heads, int64_t chain) {
-  if (a->dtype == TRINIX_F32 && packed_kernel_dim(a->head_dim) == 256) return 1;
+int fp32_wavefronts(const trinix_packed_args* a) {
+  if (packed_kernel_dim(a->head_dim) == 256) return 1;
   if (const char* env = getenv("TRINIX_PACKED_PAIRS")) return atoi(env) == 1 ? 1 : 2;
-  const int64_t blocks = (total / 128 + lmin(a->n_seqs, total) / 2) * heads, keys = a->total_k / a->n_seqs;
-  if (a->dtype == TRINIX_F32) return blocks > 1536 && keys >= 1024 ? 1 : 2;
-  return blocks <= 384 && chain * keys >= 2500 ? 2 : 1;
+  const int64_t blocks = (a->total_q / 128 + lmin(a->n_seqs, a->total_q) / 2) * a->nheads_q;
+  return blocks > 1536 && a->total_k / a->n_seqs >= 1024 ? 1 : 2;
 }
 
 }  // namespace
@@ -190,7 +185,7 @@ extern "C" int trinix_packed_fwd(const trinix_packed_args* a, void* stream) {
   hipError_t e;
   if (a->dtype == TRINIX_F32) {
     p.rows16 = rows16(a->k, a->k_stride) && rows16(a->v, a->v_stride);
-    const int ks = two_per_group(a, a->total_q, a->nheads_q, 1);
+    const int ks = fp32_wavefronts(a);
     e = launch_packed_fwd_f32(p, C, ks, (int)(use_list(p, a, ks == 2 ? kRows64 : kRows128) * p.Hq), st);
   } else {
     const PackedShape shape = packed_shape(a);
@@ -208,7 +203,8 @@ extern "C" int trinix_packed_bwd(const trinix_packed_args* a, void* stream) {
   const int C = packed_columns(a->head_dim), D = packed_lds_dim(C);
   const bool f32 = a->dtype == TRINIX_F32, bf = a->dtype == TRINIX_BF16;
   hipError_t e = hipSuccess;
-  if (f32) p.rows16 = rows16(a->q, a->q_stride) && rows16(a->dout, a->dout_stride);
+  p.rows16 = f32 && rows16(a->q, a->q_stride) && rows16(a->dout, a->dout_stride);
+  p.rows16_q = f32 && rows16(a->k, a->k_stride) && rows16(a->v, a->v_stride);
   if (a->total_q > 0) {
     e = f32 ? launch_delta<BF16, true>(p, D, st) : bf ? launch_delta<BF16, false>(p, D, st) : launch_delta<F16, false>(p, D, st);
     if (e != hipSuccess) return TRINIX_ERR_LAUNCH;
@@ -216,26 +212,15 @@ extern "C" int trinix_packed_bwd(const trinix_packed_args* a, void* stream) {
   p.Tk = (int)a->total_k;
   p.n_split = packed_head_splits(a);
   p.part = (float*)a->workspace;
-  if (!f32 && C != 256) {
-    const int n_q = (int)(use_list(p, a, kRows128) * p.Hq);
-    p.items_q = p.items;
-    const int n_kv = (int)(use_list(p, a, kKeys64) * p.Hkv * p.n_split);
-    if (n_kv + n_q > 0)
-      e = bf ? launch_packed_bwd_bf16(p, C, n_kv, n_q, st) : launch_packed_bwd_f16(p, C, n_kv, n_q, st);
-  } else {
-    if (a->total_k > 0) {
-      const int ks = two_per_group(a, a->total_k, a->nheads_kv * p.n_split, p.G / p.n_split);
-      const int grid = (int)(use_list(p, a, ks == 2 ? kKeys64 : kKeys128) * p.Hkv * p.n_split);
-      e = f32 ? launch_packed_dkdv_f32(p, C, ks, grid, st) : bf ? launch_packed_dkdv_bf16(p, ks, grid, st) : launch_packed_dkdv_f16(p, ks, grid, st);
-      if (e != hipSuccess) return TRINIX_ERR_LAUNCH;
-    }
-    if (a->total_q > 0) {
-      if (f32) p.rows16 = rows16(a->k, a->k_stride) && rows16(a->v, a->v_stride);
-      const int ks = two_per_group(a, a->total_q, a->nheads_q, 1);
-      const int grid = (int)(use_list(p, a, ks == 2 ? kRows64 : kRows128) * p.Hq);
-      e = f32 ? launch_packed_dq_f32(p, C, ks, grid, st) : bf ? launch_packed_dq_bf16(p, ks, grid, st) : launch_packed_dq_f16(p, ks, grid, st);
-    }
-  }
+  const int ks = f32 ? fp32_wavefronts(a) : 1;
+  const bool pairs = f32 ? ks == 2 : C != 256;  // (16-bit: of keys only)
+  const int n_q = (int)(use_list(p, a, ks == 2 ? kRows64 : kRows128) * p.Hq);
+  p.items_q = p.items;
+  const int n_kv = (int)(use_list(p, a, pairs ? kKeys64 : kKeys128) * p.Hkv * p.n_split);
+  if (n_kv + n_q > 0)
+    e = f32  ? launch_packed_bwd_f32(p, C, ks, n_kv, n_q, st)
+        : bf ? launch_packed_bwd_bf16(p, C, n_kv, n_q, st)
+             : launch_packed_bwd_f16(p, C, n_kv, n_q, st);
   if (e == hipSuccess && p.n_split > 1 && a->total_k > 0)
     e = f32 ? launch_sum<BF16, true>(p, D, st) : bf ? launch_sum<BF16, false>(p, D, st) : launch_sum<F16, false>(p, D, st);
   return e == hipSuccess ? TRINIX_OK : TRINIX_ERR_LAUNCH;

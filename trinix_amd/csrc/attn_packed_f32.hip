@@ -20,27 +20,18 @@ hipError_t launch_packed_fwd_f32(const PackedParams& p, int C, int ks, int grid,
   }
   return hipErrorNotSupported;
 }
-hipError_t launch_packed_dkdv_f32(const PackedParams& p, int C, int ks, int grid, hipStream_t st) {
+hipError_t launch_packed_bwd_f32(const PackedParams& p, int C, int ks, int n_kv, int n_q, hipStream_t st) {
   switch (C) {
     case 64:
-      return ks == 2 ? launch_packed_dkdv_g<Ops32<64>, 2, 1, 2>(p, grid, st) : launch_packed_dkdv_g<Ops32<64>, 2, 1, 1>(p, grid, st);
+      return ks == 2 ? launch_packed_bwd_g<Ops32<64>, 2, 1, 1, 2>(p, n_kv, n_q, st)
+                     : launch_packed_bwd_g<Ops32<64>, 2, 1, 1, 1>(p, n_kv, n_q, st);
     case 96:
-      return ks == 2 ? launch_packed_dkdv_g<Ops32<128, 96>, 1, 1, 2>(p, grid, st) : launch_packed_dkdv_g<Ops32<128, 96>, 1, 1, 1>(p, grid, st);
+      return ks == 2 ? launch_packed_bwd_g<Ops32<128, 96>, 1, 1, 1, 2>(p, n_kv, n_q, st)
+                     : launch_packed_bwd_g<Ops32<128, 96>, 1, 1, 1, 1>(p, n_kv, n_q, st);
     case 128:
-      return ks == 2 ? launch_packed_dkdv_g<Ops32<128>, 1, 1, 2>(p, grid, st) : launch_packed_dkdv_g<Ops32<128>, 1, 1, 1>(p, grid, st);
-    case 256: return launch_packed_dkdv_g<Ops32<256>, 1, 4, 1>(p, grid, st);  // K and V rows fill the registers
-  }
-  return hipErrorNotSupported;
-}
-hipError_t launch_packed_dq_f32(const PackedParams& p, int C, int ks, int grid, hipStream_t st) {
-  switch (C) {
-    case 64:
-      return ks == 2 ? launch_packed_dq_g<Ops32<64>, 2, 1, 2>(p, grid, st) : launch_packed_dq_g<Ops32<64>, 2, 1, 1>(p, grid, st);
-    case 96:
-      return ks == 2 ? launch_packed_dq_g<Ops32<128, 96>, 1, 1, 2>(p, grid, st) : launch_packed_dq_g<Ops32<128, 96>, 1, 1, 1>(p, grid, st);
-    case 128:
-      return ks == 2 ? launch_packed_dq_g<Ops32<128>, 1, 1, 2>(p, grid, st) : launch_packed_dq_g<Ops32<128>, 1, 1, 1>(p, grid, st);
-    case 256: return launch_packed_dq_g<Ops32<256>, 1, 2, 1>(p, grid, st);
+      return ks == 2 ? launch_packed_bwd_g<Ops32<128>, 1, 1, 1, 2>(p, n_kv, n_q, st)
+                     : launch_packed_bwd_g<Ops32<128>, 1, 1, 1, 1>(p, n_kv, n_q, st);
+    case 256: return launch_packed_bwd_g<Ops32<256>, 1, 4, 2, 1>(p, n_kv, n_q, st);  // K and V rows fill the registers
   }
   return hipErrorNotSupported;
 }

@@ -1,15 +1,23 @@
 // Packed-sequence attention on the operand policies of attn_ops.h: fp32 on fp32
 // matrix products, the gradients of 16-bit types at head_dim 256 with their
 // coefficients in two terms:
-//   packed_fwd_f32        128 query rows of one sequence and head, 32 per wavefront,
-//                         over 32-key tiles: S^T = K Q^T, online softmax, O^T += V^T P^T;
-//   packed_dkdv_generic   128 keys of one sequence and KV head, 32 per wavefront, over
-//                         32-row tiles of Q and dO of every head of the group:
-//                         dV += P^T dO, dZ = P (dO V^T - delta), dK += dZ^T Q;
-//   packed_dq_generic     128 query rows as in the forward: dQ += dZ K.
+//   packed_fwd_f32      128 query rows of one sequence and head, 32 per wavefront,
+//                       over 32-key tiles: S^T = K Q^T, online softmax, O^T += V^T P^T;
+//   packed_bwd_generic  in one launch (no atomics)
+//     dK, dV  128 keys of one sequence and KV head, 32 per wavefront, over 32-row
+//             tiles of Q and dO of every head of the group: dV += P^T dO,
+//             dZ = P (dO V^T - delta), dK += dZ^T Q;
+//     dQ      128 query rows as in the forward: dQ += dZ K.
 // KS = 2: 64 of them, two wavefronts per 32 taking alternate tiles, joined through LDS
-// at the end: half the chain of tiles, which bounds small batches.  Tiles go global ->
-// LDS asynchronously into two slots, one barrier per step.
+// at the end: half the chain of tiles, which bounds small batches.  The dQ items come
+// behind those of dK and dV and fill the CUs that these leave idle (us, forward with
+// backward, launches of their own | one: fp32, 8 heads of 80, 1090 rows 143 | 103, of 128
+// 183 | 131; bf16 of 256, 16/4 heads 4 x 1000 413 | 359, 8/4 2048 + 1000 340 | 294; two
+// wavefronts per 32 at 256 then give nothing).  Tiles go global -> LDS asynchronously
+// into two slots, one barrier per step.
+// What bounds it: the fp32 products, 64 cycles for each 32x32x2.  8 x 2048 rows, 16/4
+// heads of 96: forward 116, all 118 TFLOP/s of 2 and 2 + 7 products, where the library's
+// large fp32 product reaches 154 on the same card.
 #pragma once
 #include <cfloat>
 
@@ -147,21 +155,27 @@ __global__ __launch_bounds__(256, OCC) void packed_fwd_f32(const PackedParams p)
   if (p.lse && g == 0) p.lse[(int64_t)hq * p.Tq + row] = l > 0.f ? (m_run + log2f(l)) * kLn2 : -INFINITY;
 }
 
-template <class O, int OCC, int HS, int KS>
-__global__ __launch_bounds__(256, OCC) void packed_dkdv_generic(const PackedParams p) {
+// LDS of either part, in bytes: two slots of two KS-tile operands, and rows of two floats.
+template <class O, int KS>
+constexpr int kGenericTiles = KS * kTileRows * O::kD * (int)sizeof(typename O::Store);
+template <class O, int KS>
+constexpr int kGenericLds = 4 * kGenericTiles<O, KS> + 4 * KS * kTileRows * 4;
+
+// dK and dV.  HS workgroups share a key block, each summing D / HS of the columns.
+template <class O, int HS, int KS>
+__device__ __forceinline__ void generic_dkdv_body(const PackedParams& p, int wg, char* pool) {
   using Store = typename O::Store;
   constexpr int NW = 4, BK = NW * 32 / KS, D = O::kD, DB = O::DB / HS, TILE = kTileRows * D * (int)sizeof(Store);
-  __shared__ __attribute__((aligned(1024))) char lds_q[2][KS * TILE];
-  __shared__ __attribute__((aligned(1024))) char lds_o[2][KS * TILE];
-  __shared__ __attribute__((aligned(128))) float lds_l[2][KS * kTileRows];
-  __shared__ __attribute__((aligned(128))) float lds_d[2][KS * kTileRows];
-  // HS workgroups share a key block, each summing D / HS of the columns
-  const PackedBlock w(p, p.items, (int)blockIdx.x / HS, p.Hkv * p.n_split, 1);
+  char(*const lds_q)[KS * TILE] = (char(*)[KS * TILE]) pool;
+  char(*const lds_o)[KS * TILE] = lds_q + 2;
+  float(*const lds_l)[KS * kTileRows] = (float(*)[KS * kTileRows])(lds_o + 2);
+  float(*const lds_d)[KS * kTileRows] = lds_l + 2;
+  const PackedBlock w(p, p.items, wg / HS, p.Hkv * p.n_split, 1);
   if (w.blk < 0) return;
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const PackedHeads hd(p, w.h);
-  const int hkv = hd.hkv, kb0 = w.blk * BK, db0 = ((int)blockIdx.x % HS) * DB;
+  const int hkv = hd.hkv, kb0 = w.blk * BK, db0 = (wg % HS) * DB;
   const int kp = wave % KS, j0 = kb0 + wave / KS * 32, j = j0 + (lane & 31), jc = min(j, w.lk - 1);
   const bool wide = p.rows16 != 0;
   const int off = w.lk - w.lq;
@@ -293,19 +307,19 @@ __global__ __launch_bounds__(256, OCC) void packed_dkdv_generic(const PackedPara
     }
 }
 
-template <class O, int OCC, int HS, int KS>
-__global__ __launch_bounds__(256, OCC) void packed_dq_generic(const PackedParams p) {
+template <class O, int HS, int KS>
+__device__ __forceinline__ void generic_dq_body(const PackedParams& p, int wg, char* pool) {
   using Store = typename O::Store;
   constexpr int NW = 4, BM = NW * 32 / KS, D = O::kD, DB = O::DB / HS, TILE = kTileRows * D * (int)sizeof(Store);
-  __shared__ __attribute__((aligned(1024))) char lds_k[2][KS * TILE];
-  __shared__ __attribute__((aligned(1024))) char lds_v[2][KS * TILE];
-  const PackedBlock w(p, p.items, (int)blockIdx.x / HS, p.Hkv, p.G);
+  char(*const lds_k)[KS * TILE] = (char(*)[KS * TILE]) pool;
+  char(*const lds_v)[KS * TILE] = lds_k + 2;
+  const PackedBlock w(p, p.items_q, wg / HS, p.Hkv, p.G);
   if (w.blk < 0) return;
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hq = w.h, hkv = hq / p.G, m0 = w.blk * BM, kp = wave % KS, iw0 = m0 + wave / KS * 32, i = iw0 + r, ic = min(i, w.lq - 1);
-  const int db0 = ((int)blockIdx.x % HS) * DB, off = w.lk - w.lq;
-  const bool wide = p.rows16 != 0;
+  const int db0 = (wg % HS) * DB, off = w.lk - w.lq;
+  const bool wide = p.rows16_q != 0;
 
   const O ops(lane, db0);
   const typename O::Frag qf = load_frag_cols<O>((const Store*)p.q + (int64_t)(w.q0 + ic) * p.q_ss + hq * p.q_sh, g, p.d);
@@ -387,13 +401,18 @@ __global__ __launch_bounds__(256, OCC) void packed_dq_generic(const PackedParams
     }
 }
 
-template <class O, int OCC, int HS, int KS>
-hipError_t launch_packed_dkdv_g(const PackedParams& p, int grid, hipStream_t st) {
-  return launch_kernel(&packed_dkdv_generic<O, OCC, HS, KS>, dim3((unsigned)(grid * HS)), dim3(256), 0, st, p);
+// Workgroups [0, n_kv * HSK): dK and dV of p.items; behind them dQ of p.items_q.
+template <class O, int OCC, int HSK, int HSQ, int KS>
+__global__ __launch_bounds__(256, OCC) void packed_bwd_generic(const PackedParams p, int n_kv) {
+  __shared__ __attribute__((aligned(1024))) char pool[kGenericLds<O, KS>];
+  const int wg = (int)blockIdx.x;
+  if (wg < n_kv * HSK) generic_dkdv_body<O, HSK, KS>(p, wg, pool);
+  else generic_dq_body<O, HSQ, KS>(p, wg - n_kv * HSK, pool);
 }
-template <class O, int OCC, int HS, int KS>
-hipError_t launch_packed_dq_g(const PackedParams& p, int grid, hipStream_t st) {
-  return launch_kernel(&packed_dq_generic<O, OCC, HS, KS>, dim3((unsigned)(grid * HS)), dim3(256), 0, st, p);
+template <class O, int OCC, int HSK, int HSQ, int KS>
+hipError_t launch_packed_bwd_g(const PackedParams& p, int n_kv, int n_q, hipStream_t st) {
+  return launch_kernel(&packed_bwd_generic<O, OCC, HSK, HSQ, KS>, dim3((unsigned)(n_kv * HSK + n_q * HSQ)), dim3(256), 0, st, p,
+                       n_kv);
 }
 
 }  // namespace trinix

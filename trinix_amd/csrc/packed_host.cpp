@@ -35,9 +35,10 @@ int validate_packed(const trinix_packed_args* a, bool backward) {
   if (a->nheads_q <= 0 || a->nheads_kv <= 0 || a->nheads_q > (1 << 20) || a->nheads_q % a->nheads_kv != 0)
     return TRINIX_ERR_BAD_SHAPE;
   if (a->plan_bytes < need || ((uintptr_t)a->plan & 15) != 0) return TRINIX_ERR_BAD_ARGUMENT;
-  // the largest grid: one workgroup per item of the finest list and head
+  // the largest grid: the backward at head_dim 256, four workgroups per item of the
+  // finest key list and head and two per one of the finest row list
   const int64_t most = lmax(packed_list_cap(a->total_q, a->n_seqs, 64), packed_list_cap(a->total_k, a->n_seqs, 64));
-  if (most > INT32_MAX / (4 * a->nheads_q)) return TRINIX_ERR_BAD_SHAPE;
+  if (most > INT32_MAX / (6 * a->nheads_q)) return TRINIX_ERR_BAD_SHAPE;
   const bool f32 = a->dtype == TRINIX_F32;
   const struct {
     const void* ptr;
