@@ -462,7 +462,8 @@ int trinix_abi_version(void);
  *   out_i = softmax_j(s[i,:]) @ v,  lse_i = log(sum_j exp(s[i,j]))
  * A row that sees no key has out 0 and lse -inf, and takes no part in any
  * gradient.  Rows behind the last sequence are such rows; keys behind it get
- * gradients of 0.
+ * gradients of 0.  What such rows, and keys that no row sees, hold reaches no
+ * result.
  *
  * The plan is a table of work items built on the GPU from cu_q and cu_k
  * (nothing is read back); boundaries are clamped into the tensors and made

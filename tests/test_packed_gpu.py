@@ -147,6 +147,38 @@ def test_padding_rows_are_zero_and_poison_there_is_not_read():
         assert bool(torch.isfinite(t[:200]).all()) and bool((t[200:] == 0).all())
 
 
+@pytest.mark.parametrize("dtype,D", [(BF, 64), (HF, 128), (F32, 96), (BF, 256), (F32, 64), (BF, 96)])
+@pytest.mark.parametrize("causal,window", [(True, (40, 0)), (False, (30, -5)), (True, None), (False, (-20, 60))])
+def test_what_no_row_sees_holds_anything(dtype, D, causal, window):
+    """Keys before every row's window, keys behind, and rows that see no key: NaN there changes no bit."""
+    lens_q, lens_k, H, Hkv = [50, 200, 3, 140, 1], [300, 70, 500, 140, 33], 4, 2
+    cu_q, cu_k = cumulative(lens_q), cumulative(lens_k)
+    q, k, v, do = (t.to(DEV) for t in make(cu_q[-1], cu_k[-1], H, Hkv, D, dtype, 5))
+    seqs = tx.PackedSequences(cu_q, cu_k)
+
+    def run(*ts):
+        a, b, c, do = ts
+        a, b, c = (t.detach().clone().requires_grad_(True) for t in (a, b, c))
+        out, lse = tx.packed_attn_func(a, b, c, seqs, causal=causal, window_size=window, return_lse=True)
+        return (out.detach(), lse, *torch.autograd.grad(out, (a, b, c), do))
+
+    want = run(q, k, v, do)
+    for s, (lq, lk) in enumerate(zip(lens_q, lens_k)):
+        i, j = torch.arange(lq)[:, None] + (lk - lq), torch.arange(lk)[None]
+        ok = torch.ones(lq, lk, dtype=torch.bool)
+        if causal:
+            ok &= j <= i
+        if window is not None:
+            ok &= (j - i >= -window[0]) & (j - i <= window[1])
+        rows, keys = (~ok.any(1)).to(DEV), (~ok.any(0)).to(DEV)
+        for t in (q, do):
+            t[cu_q[s]:cu_q[s + 1]][rows] = float("nan")
+        k[cu_k[s]:cu_k[s + 1]][keys] = float("nan")
+        v[cu_k[s]:cu_k[s + 1]][keys] = float("inf")
+    for name, a, b in zip(("out", "lse", "dq", "dk", "dv"), run(q, k, v, do), want):
+        assert torch.equal(a, b), name
+
+
 def test_strided_operands():
     # q, k and v as slices of one projection, a KV head expanded without a copy, dout with a stride of 0
     g = torch.Generator().manual_seed(4)

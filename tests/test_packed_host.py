@@ -260,6 +260,20 @@ int main() {
       int dlo, dhi;
       packed_band(lq, lk, causal, win, wl, wr, dlo, dhi);
       const int off = lk - lq;
+      // keys that any row sees, rows that see any key, and what a tile reads of them
+      int k_lo = lk, k_hi = -1, r_lo = lq, r_hi = -1;
+      for (int i = 0; i < lq; ++i) for (int j = std::max(0, i + dlo); j <= std::min(lk - 1, i + dhi); ++j) {
+        k_lo = std::min(k_lo, j), k_hi = std::max(k_hi, j), r_lo = std::min(r_lo, i), r_hi = std::max(r_hi, i);
+      }
+      const PackedRange ks = packed_seen_keys(lq, lk, dlo, dhi), rs = packed_seeing_rows(lq, lk, dlo, dhi);
+      EXPECT(0 <= ks.lo && ks.lo <= ks.hi && ks.hi < lk && 0 <= rs.lo && rs.lo <= rs.hi && rs.hi < lq);
+      if (k_hi >= 0) EXPECT(ks.lo == k_lo && ks.hi == k_hi && rs.lo == r_lo && rs.hi == r_hi);
+      for (int n0 = 0; n0 < lk; n0 += 32) {
+        const PackedRange t = packed_tile_range(ks, n0);
+        EXPECT(0 <= t.lo && t.lo <= t.hi && n0 + t.hi < lk);
+        if (n0 <= ks.hi && n0 + 32 > ks.lo)
+          for (int r = 0; r < 32; ++r) EXPECT(n0 + std::min(std::max(r, t.lo), t.hi) == std::min(std::max(n0 + r, ks.lo), ks.hi));
+      }
       for (int BM : {64, 128}) for (int m0 = 0; m0 < lq; m0 += BM) {
         int lo, hi;
         bwd_key_tiles(m0, BM, lq, lk, dlo, dhi, 32, lo, hi);

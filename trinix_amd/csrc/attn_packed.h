@@ -63,6 +63,8 @@ struct PackedBlock {
   __device__ Span rows_of(int j) const {
     return j < lk ? Span(max((int64_t)0, (int64_t)j - dhi), min((int64_t)lq - 1, (int64_t)j - dlo)) : Span(1, 0);
   }
+  __device__ PackedRange keys() const { return packed_seen_keys(lq, lk, dlo, dhi); }
+  __device__ PackedRange rows() const { return packed_seeing_rows(lq, lk, dlo, dhi); }
   // Block of rows [ia, ia + ni) and keys [ja, ja + nj): does it hold allowed
   // pairs; are all of its pairs allowed?
   __device__ bool live(int ia, int ni, int ja, int nj) const {
@@ -121,30 +123,32 @@ struct PackedCopy {
   uint32_t off[PER];
   __device__ PackedCopy(int64_t ss_, int wave_, int lane_, int d) : ss(ss_), wave(wave_), lane(lane_), units(d * ESZ / 16) {
 #pragma unroll
-    for (int l = 0; l < PER; ++l) off[l] = offset(l, kTileRows - 1);
+    for (int l = 0; l < PER; ++l) off[l] = offset(l, PackedRange{0, kTileRows - 1});
   }
-  __device__ uint32_t offset(int l, int last) const {
+  __device__ uint32_t offset(int l, const PackedRange& t) const {
     const int row = tile_copy_row(wave, PER, l, lane, UPR);
-    return tile32_offset(row, last, ss, ESZ, min(O::swz(((wave * PER + l) * 64 + lane) % UPR, row), units - 1));
+    return tile32_offset(max(row, t.lo), t.hi, ss, ESZ, min(O::swz(((wave * PER + l) * 64 + lane) % UPR, row), units - 1));
   }
-  // rows [i0, i0 + 32) of n; `wide`: 16 bytes a lane from 32-bit offsets (always for 16-bit types)
-  __device__ void operator()(const Store* base, int i0, int n, char* lds_tile, bool wide) const {
+  // rows [i0, i0 + 32), those outside [of.lo, of.hi] as the nearest within; `wide`: 16
+  // bytes a lane from 32-bit offsets (always for 16-bit types)
+  __device__ void operator()(const Store* base, int i0, const PackedRange& of, char* lds_tile, bool wide) const {
     const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void_t*)lds_tile;
+    const PackedRange t = packed_tile_range(of, i0);
     if (ESZ == 2 || wide) {
       const uint64_t gb = uniform_ptr(base + (int64_t)i0 * ss);
-      if (i0 + kTileRows <= n) {
+      if (t.lo == 0 && t.hi >= kTileRows - 1) {
 #pragma unroll
         for (int l = 0; l < PER; ++l) dma_16b_s(off[l], gb, __builtin_amdgcn_readfirstlane(lds0 + (wave * PER + l) * 1024));
       } else {
 #pragma unroll 1
         for (int l = 0; l < PER; ++l)
-          dma_16b_s(offset(l, n - 1 - i0), gb, __builtin_amdgcn_readfirstlane(lds0 + (wave * PER + l) * 1024));
+          dma_16b_s(offset(l, t), gb, __builtin_amdgcn_readfirstlane(lds0 + (wave * PER + l) * 1024));
       }
     } else {
 #pragma unroll 1
       for (int l = 0; l < PER * 4; ++l) {
         const int c = wave * PER * 4 + l, word = c * 64 + lane, unit = word / 4, row = unit / UPR;
-        dma_4b(base + (int64_t)min(i0 + row, n - 1) * ss + min(O::swz(unit % UPR, row), units - 1) * 4 + (word & 3),
+        dma_4b(base + (int64_t)(i0 + min(max(row, t.lo), t.hi)) * ss + min(O::swz(unit % UPR, row), units - 1) * 4 + (word & 3),
                __builtin_amdgcn_readfirstlane(lds0 + c * 256));
       }
     }

@@ -21,7 +21,8 @@ __global__ __launch_bounds__(NW * 64, OCC) void packed_fwd16(const PackedParams 
   KeyRun kr;
   kr.k = (const uint16_t*)p.k + (int64_t)w.k0 * p.k_ss + hkv * p.k_sh;
   kr.v = (const uint16_t*)p.v + (int64_t)w.k0 * p.v_ss + hkv * p.v_sh;
-  kr.k_ss = p.k_ss, kr.v_ss = p.v_ss, kr.n = w.lk, kr.d = p.d;
+  const PackedRange seen = w.keys();
+  kr.k_ss = p.k_ss, kr.v_ss = p.v_ss, kr.lo = seen.lo, kr.n = seen.hi + 1, kr.d = p.d;
   bwd_key_tiles(m0, BM, w.lq, w.lk, w.dlo, w.dhi, BN, kr.t_lo, kr.t_hi);
   packed_full_tiles(m0, mlast, w.lk, w.dlo, w.dhi, BN, kr.t_lo, kr.t_hi, kr.t_flo, kr.t_fhi);
   kr.jlo = ks.lo, kr.jspan = ks.span;

@@ -1,4 +1,4 @@
-// Gradients of packed-sequence attention, 16-bit types at head_dim 64 and 128, in one
+// Gradients of packed-sequence attention, 16-bit types at head_dims up to 128, in one
 // launch (no atomics) of 4-wavefront workgroups, two per CU:
 //   dK, dV  64 keys of one sequence and KV head, a pair of wavefronts per 32 keys: the
 //           first computes S = Q K^T, P = exp(scale S - lse) and dV^T += dO^T P, hands P in
@@ -59,7 +59,9 @@ __device__ __forceinline__ void packed_dkdv_body(const PackedParams& p, const Pa
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kg = wave % NG;
   const PackedHeads hd(p, w.h);
-  const int hkv = hd.hkv, kb0 = w.blk * BK, j0 = kb0 + kg * 32, j = j0 + (lane & 31), jc = min(j, w.lk - 1);
+  const int hkv = hd.hkv, kb0 = w.blk * BK, j0 = kb0 + kg * 32, j = j0 + (lane & 31);
+  const PackedRange kseen = w.keys(), qseen = w.rows();
+  const int jc = min(max(j, kseen.lo), kseen.hi);
   const int off = w.lk - w.lq;
   const Span qspan = w.rows_of(j);
 
@@ -80,11 +82,11 @@ __device__ __forceinline__ void packed_dkdv_body(const PackedParams& p, const Pa
   auto load_rows = [&](const uint16_t* base, int64_t ss, char* tile, int i0) __attribute__((always_inline)) {
     const uint64_t gb = uniform_ptr((const char*)base + (int64_t)i0 * ss * 2);
     const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void_t*)tile + wave_lds;
-    const int last = w.lq - 1 - i0;  // rows past the sequence read its last one
+    const PackedRange t = packed_tile_range(qseen, i0);
 #pragma unroll
     for (int l = 0; l < LPW; ++l) {
       const int row = tile_copy_row(wave, LPW, l, lane, UPR);
-      dma_16b_s(tile_copy_offset((uint32_t)min(row, last), ss, (uint32_t)min((lane % UPR) ^ swz_kt<D>(row), p.d / 8 - 1)), gb,
+      dma_16b_s(tile_copy_offset((uint32_t)min(max(row, t.lo), t.hi), ss, (uint32_t)min((lane % UPR) ^ swz_kt<D>(row), p.d / 8 - 1)), gb,
                 __builtin_amdgcn_readfirstlane(lds0 + l * 1024));
     }
   };
@@ -299,13 +301,15 @@ __device__ __forceinline__ void packed_dq_body(const PackedParams& p, const Pack
   char* const lds_v = pool + 2 * NT * TILE;
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int hq = w.h, hkv = hq / p.G, m0 = w.blk * BM, iw0 = m0 + wave * 32, i = iw0 + r, ic = min(i, w.lq - 1);
+  const int hq = w.h, hkv = hq / p.G, m0 = w.blk * BM, iw0 = m0 + wave * 32, i = iw0 + r;
+  const PackedRange kseen = w.keys(), qseen = w.rows();
+  const int ic = min(max(i, qseen.lo), qseen.hi);
   const int off = w.lk - w.lq;
 
   const O ops(lane, 0);
   const typename O::Frag qf = load_frag_cols<O>((const uint16_t*)p.q + (int64_t)(w.q0 + ic) * p.q_ss + hq * p.q_sh, g, p.d);
   const typename O::Frag of = load_frag_cols<O>((const uint16_t*)p.dout + (int64_t)(w.q0 + ic) * p.do_ss + hq * p.do_sh, g, p.d);
-  const int64_t ro = (int64_t)hq * p.Tq + w.q0 + ic;
+  const int64_t ro = (int64_t)hq * p.Tq + w.q0 + min(i, w.lq - 1);
   const float lse2 = fmaxf(p.lse[ro] * kLog2e, -0.5f * FLT_MAX), dlt = p.delta[ro];  // (finite: see write_rows)
   const float slope_l2 = p.alibi ? -p.alibi[hq * p.al_sh] * kLog2e : 0.f;
   f32x16_t acc[DB];
@@ -325,7 +329,7 @@ __device__ __forceinline__ void packed_dq_body(const PackedParams& p, const Pack
   auto load = [&](int t, int slot) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < NT; ++u)
-      if (t + u < t_hi) copy(cbase, (t + u) * kTileRows, w.lk, (cv ? lds_v : lds_k) + (slot * NT + u) * TILE, true);
+      if (t + u < t_hi) copy(cbase, (t + u) * kTileRows, kseen, (cv ? lds_v : lds_k) + (slot * NT + u) * TILE, true);
   };
   auto block = [&](int t, const char* kt, const char* vt) __attribute__((always_inline)) {
     const int n0 = t * kTileRows;

@@ -38,6 +38,7 @@ __global__ __launch_bounds__(256, OCC) void packed_fwd_f32(const PackedParams p)
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hq = w.h, hkv = hq / p.G, m0 = w.blk * BM, kp = wave % KS, iw0 = m0 + wave / KS * 32, i = iw0 + r, ic = min(i, w.lq - 1);
+  const PackedRange kseen = w.keys();
   const bool wide = p.rows16 != 0;
 
   const O ops(lane, 0);
@@ -58,8 +59,8 @@ __global__ __launch_bounds__(256, OCC) void packed_fwd_f32(const PackedParams p)
 #pragma unroll
     for (int u = 0; u < KS; ++u)
       if (t + u < t_hi) {
-        copy_k(kbase, (t + u) * kTileRows, w.lk, lds_k[slot] + u * TILE, wide);
-        copy_v(vbase, (t + u) * kTileRows, w.lk, lds_v[slot] + u * TILE, wide);
+        copy_k(kbase, (t + u) * kTileRows, kseen, lds_k[slot] + u * TILE, wide);
+        copy_v(vbase, (t + u) * kTileRows, kseen, lds_v[slot] + u * TILE, wide);
       }
   };
   auto block = [&](int t, int slot) __attribute__((always_inline)) {
@@ -176,7 +177,9 @@ __device__ __forceinline__ void generic_dkdv_body(const PackedParams& p, int wg,
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const PackedHeads hd(p, w.h);
   const int hkv = hd.hkv, kb0 = w.blk * BK, db0 = (wg % HS) * DB;
-  const int kp = wave % KS, j0 = kb0 + wave / KS * 32, j = j0 + (lane & 31), jc = min(j, w.lk - 1);
+  const int kp = wave % KS, j0 = kb0 + wave / KS * 32, j = j0 + (lane & 31);
+  const PackedRange kseen = w.keys(), qseen = w.rows();
+  const int jc = min(max(j, kseen.lo), kseen.hi);
   const bool wide = p.rows16 != 0;
   const int off = w.lk - w.lq;
 
@@ -200,8 +203,8 @@ __device__ __forceinline__ void generic_dkdv_body(const PackedParams& p, int wg,
     for (int u = 0; u < KS; ++u) {
       if (it + u >= n_items) break;
       const int hq = hkv * p.G + hd.gh0 + (it + u) / nqt, i0 = (qt_lo + (it + u) % nqt) * kTileRows;
-      copy_q((const Store*)p.q + (int64_t)w.q0 * p.q_ss + hq * p.q_sh, i0, w.lq, lds_q[slot] + u * TILE, wide);
-      copy_o((const Store*)p.dout + (int64_t)w.q0 * p.do_ss + hq * p.do_sh, i0, w.lq, lds_o[slot] + u * TILE, wide);
+      copy_q((const Store*)p.q + (int64_t)w.q0 * p.q_ss + hq * p.q_sh, i0, qseen, lds_q[slot] + u * TILE, wide);
+      copy_o((const Store*)p.dout + (int64_t)w.q0 * p.do_ss + hq * p.do_sh, i0, qseen, lds_o[slot] + u * TILE, wide);
       if (tid / kTileRows == u) {
         const int64_t ro = (int64_t)hq * p.Tq + w.q0 + min(i0 + tid % kTileRows, w.lq - 1);
         lse_next = p.lse[ro];
@@ -317,14 +320,16 @@ __device__ __forceinline__ void generic_dq_body(const PackedParams& p, int wg, c
   if (w.blk < 0) return;
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int hq = w.h, hkv = hq / p.G, m0 = w.blk * BM, kp = wave % KS, iw0 = m0 + wave / KS * 32, i = iw0 + r, ic = min(i, w.lq - 1);
+  const int hq = w.h, hkv = hq / p.G, m0 = w.blk * BM, kp = wave % KS, iw0 = m0 + wave / KS * 32, i = iw0 + r;
+  const PackedRange kseen = w.keys(), qseen = w.rows();
+  const int ic = min(max(i, qseen.lo), qseen.hi);
   const int db0 = (wg % HS) * DB, off = w.lk - w.lq;
   const bool wide = p.rows16_q != 0;
 
   const O ops(lane, db0);
   const typename O::Frag qf = load_frag_cols<O>((const Store*)p.q + (int64_t)(w.q0 + ic) * p.q_ss + hq * p.q_sh, g, p.d);
   const typename O::Frag of = load_frag_cols<O>((const Store*)p.dout + (int64_t)(w.q0 + ic) * p.do_ss + hq * p.do_sh, g, p.d);
-  const int64_t ro = (int64_t)hq * p.Tq + w.q0 + ic;
+  const int64_t ro = (int64_t)hq * p.Tq + w.q0 + min(i, w.lq - 1);
   const float lse2 = fmaxf(p.lse[ro] * kLog2e, -0.5f * FLT_MAX), dlt = p.delta[ro];  // (finite: see above)
   const float slope_l2 = p.alibi ? -p.alibi[hq * p.al_sh] * kLog2e : 0.f;
   f32x16_t acc[DB];
@@ -341,8 +346,8 @@ __device__ __forceinline__ void generic_dq_body(const PackedParams& p, int wg, c
 #pragma unroll
     for (int u = 0; u < KS; ++u)
       if (t + u < t_hi) {
-        copy_k(kbase, (t + u) * kTileRows, w.lk, lds_k[slot] + u * TILE, wide);
-        copy_v(vbase, (t + u) * kTileRows, w.lk, lds_v[slot] + u * TILE, wide);
+        copy_k(kbase, (t + u) * kTileRows, kseen, lds_k[slot] + u * TILE, wide);
+        copy_v(vbase, (t + u) * kTileRows, kseen, lds_v[slot] + u * TILE, wide);
       }
   };
   auto block = [&](int t, int slot) __attribute__((always_inline)) {

@@ -34,8 +34,8 @@ constexpr int kTile16Words = KS * BN * D;
   __shared__ __attribute__((aligned(1024))) uint16_t lds_v0[kTile16Words<D, BN, KS>]; \
   __shared__ __attribute__((aligned(1024))) uint16_t lds_v1[kTile16Words<D, BN, KS>]
 
-// A run of key tiles: keys [0, n) at k and v (row strides in elements; rows at
-// and past n are read as row n - 1), tiles [t_lo, t_hi) of which [t_flo, t_fhi)
+// A run of key tiles: keys [lo, n) at k and v (row strides in elements; rows outside
+// are read as the nearest of them), tiles [t_lo, t_hi) of which [t_flo, t_fhi)
 // hold only pairs that every row of the workgroup may see.  A lane's row sees
 // keys jlo .. jlo + jspan (jlo = INT_MAX: none); keys outside [wlo, whi] are seen
 // by no row of the wavefront.  pos: position of the lane's row among the keys (ALiBi).
@@ -45,7 +45,7 @@ struct KeyRun {
   const uint16_t* k;
   const uint16_t* v;
   int64_t k_ss, v_ss;
-  int n, d, t_lo, t_hi, t_flo, t_fhi;
+  int lo, n, d, t_lo, t_hi, t_flo, t_fhi;
   int jlo;
   uint32_t jspan;
   int wlo, whi;
@@ -161,7 +161,7 @@ struct Tile16 {
 
   __device__ __forceinline__ void run(KeyRun kr) {
     // (uniform by construction; 64-bit comparisons leave them in vector registers)
-    for (int* x : {&kr.n, &kr.t_lo, &kr.t_hi, &kr.t_flo, &kr.t_fhi, &kr.wlo, &kr.whi}) *x = __builtin_amdgcn_readfirstlane(*x);
+    for (int* x : {&kr.lo, &kr.n, &kr.t_lo, &kr.t_hi, &kr.t_flo, &kr.t_fhi, &kr.wlo, &kr.whi}) *x = __builtin_amdgcn_readfirstlane(*x);
     auto ld_row = [&](int l) __attribute__((always_inline)) { return tile_copy_row(wave, LPW, l, lane, UPR); };
     auto ld_unit_k = [&](int l) __attribute__((always_inline)) { return min((lane % UPR) ^ swz_k<D>(ld_row(l)), kr.d / 8 - 1); };
     auto ld_unit_v = [&](int l) __attribute__((always_inline)) { return min((lane % UPR) ^ swz_v<D>(ld_row(l)), kr.d / 8 - 1); };
@@ -178,14 +178,14 @@ struct Tile16 {
       const int n0 = tile * BN;
       const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void_t*)lds_tile + wave_lds;
       const uint64_t gb = base_s + (uint64_t)n0 * (uint64_t)(ss * 2);
-      if (n0 + BN <= kr.n) {
+      if (n0 >= kr.lo && n0 + BN <= kr.n) {
 #pragma unroll
         for (int l = 0; l < LPW; ++l) dma_16b_s(offs[l], gb, __builtin_amdgcn_readfirstlane(lds0 + l * 1024));
       } else {
-        const int last = kr.n - 1 - n0;  // >= 0: tiles start below n
+        const int last = kr.n - 1 - n0, first = max(kr.lo - n0, 0);  // last >= first: a tile holds keys of the run
 #pragma unroll
         for (int l = 0; l < LPW; ++l) {
-          const uint32_t row = (uint32_t)min(ld_row(l), last);
+          const uint32_t row = (uint32_t)min(max(ld_row(l), first), last);
           const uint32_t unit = (uint32_t)(decltype(is_k)::value ? ld_unit_k(l) : ld_unit_v(l));
           dma_16b_s(tile_copy_offset(row, ss, unit), gb, __builtin_amdgcn_readfirstlane(lds0 + l * 1024));
         }

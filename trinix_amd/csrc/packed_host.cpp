@@ -154,9 +154,10 @@ int plan_shared(const trinix_shared_prefix_args* a, SharedPlan* pl) {
   const int64_t gp = blocks(rows, bm) * kv, gs = a->batch * blocks(own, bm) * kv;
   // Chunks of whole 64 keys, at least 128, as many as give about `target`
   // workgroups.  16-bit: 256 for the prefix and 1024 for the own keys; targets of
-  // 128 / 256 / 512 / 1024 for the prefix: B=64 P=8192 40.8 | 38.9 | 49.3 | 58.7 us, B=1
-  // Sq=256 P=8192 114 | 68 | 60 | 67, B=64 Sq=4 117 | 72 | 79 | 85; of 256 / 512 / 1024 / 2048
-  // for the own keys: B=64 caches of 1024 41.5 | 41.1 | 38.9 | 42.9.
+  // 128 / 256 / 512 / 1024 for the prefix, caches warm: B=64 P=8192 40.8 | 38.9 | 49.3 |
+  // 58.7 us, B=1 Sq=256 P=8192 114 | 68 | 60 | 67, B=64 Sq=4 117 | 72 | 79 | 85; of 512 / 1024 /
+  // 2048 / 4096 for the own keys, caches read from memory: B=64 of 1024 54.0 | 50.2 | 52.4 |
+  // 57.5.  64 keys at least: B=32 of 200 behind 500 13.3 | 17.9, B=1 9.3 | 8.9.
   const auto split = [&](int64_t keys, int64_t groups, int64_t target, int* n, int* chunk) {
     const int64_t c = lmax(kDecodeMinChunk, blocks(blocks(keys, lmax(1, target / groups)), 64) * 64);
     *n = (int)blocks(keys, c);

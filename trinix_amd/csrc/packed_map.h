@@ -109,6 +109,32 @@ __host__ __device__ inline void packed_band(int lq, int lk, bool causal, bool ha
   dhi = (int)lmin(lmax(hi, -kFar), kFar);
 }
 
+// First and last key of a sequence that any of its rows sees, and row that sees any key
+// (inside the sequence; anything there where no pair is allowed).  Tiles read nothing
+// outside, so what the others hold, NaN too, reaches no result.
+struct PackedRange {
+  int lo, hi;
+};
+__host__ __device__ inline PackedRange packed_range(int64_t lo, int64_t hi, int n) {
+  PackedRange r;
+  r.hi = (int)lmin(lmax(hi, 0), (int64_t)n - 1);
+  r.lo = (int)lmin(lmax(lo, 0), (int64_t)r.hi);
+  return r;
+}
+__host__ __device__ inline PackedRange packed_seen_keys(int lq, int lk, int dlo, int dhi) {
+  return packed_range(dlo, (int64_t)lq - 1 + dhi, lk);
+}
+__host__ __device__ inline PackedRange packed_seeing_rows(int lq, int lk, int dlo, int dhi) {
+  return packed_range(-(int64_t)dhi, (int64_t)lk - 1 - dlo, lq);
+}
+// First and last row of the tile at n0 of such a range; the rows before and behind read these.
+__host__ __device__ inline PackedRange packed_tile_range(const PackedRange& r, int n0) {
+  PackedRange t;
+  t.hi = imax(r.hi - n0, 0);
+  t.lo = imin(imax(r.lo - n0, 0), t.hi);
+  return t;
+}
+
 // Tiles of BN keys, within [t_lo, t_hi), whose keys all of rows m0 .. mlast see.
 __host__ __device__ inline void packed_full_tiles(int m0, int mlast, int lk, int dlo, int dhi, int BN, int t_lo, int t_hi,
                                                   int& t_flo, int& t_fhi) {

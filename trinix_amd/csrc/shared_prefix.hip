@@ -8,9 +8,12 @@
 //    workgroup on Tile16, of the prefix (rows of any requests) or of one request's
 //    cache.  Leaves (O, lse) of each row and chunk in fp32 in the workspace;
 //    shared_merge adds them up, one workgroup per row.  64 requests behind 8192 keys,
-//    caches of 1..1024, 32/8 heads of 128: 39 us, 34 of them the 156 MB (4.6 TB/s);
-//    with the 16-row kernel below 95 (the prefix's products on fp32 matrix
-//    instructions), with it for the own keys alone 45;
+//    caches of 1..1024, 32/8 heads of 128, 156 MB: 49 us with caches read from memory
+//    (the copy rate gives 30; chunks that wait for a whole tile, the last items' tail
+//    and the merge, 5 us, the rest), 39 with caches that the last level still holds;
+//    there 95 with the 16-row kernel below (the prefix's products on fp32 matrix
+//    instructions), 45 with it for the own keys alone.  Own rows loaded straight into
+//    registers, three steps ahead: 54 from memory;
 //  - shared_whole, 16-bit types: 64 or 128 rows of one request by all its keys, where
 //    there are enough such blocks.  8 turns of 256 rows behind 6000 keys: 204 us
 //    (1060 TFLOP/s), 309 in chunks;
@@ -285,7 +288,7 @@ __device__ inline KeyRun prefix_run(const SharedParams& p, int hkv, int c0, int 
   kr.k_ss = p.pk_ss, kr.v_ss = p.pv_ss;
   kr.k = (const uint16_t*)p.pk + hkv * p.pk_sh + (int64_t)c0 * p.pk_ss;
   kr.v = (const uint16_t*)p.pv + hkv * p.pv_sh + (int64_t)c0 * p.pv_ss;
-  kr.n = c1 - c0, kr.d = p.d;
+  kr.lo = 0, kr.n = c1 - c0, kr.d = p.d;
   kr.t_lo = kr.t_flo = 0;
   kr.t_hi = (kr.n + BN - 1) / BN;
   kr.t_fhi = kr.n / BN;
@@ -305,7 +308,7 @@ __device__ inline KeyRun own_run(const SharedParams& p, int b, int hkv, int c0, 
   kr.k_ss = p.k_ss, kr.v_ss = p.v_ss;
   kr.k = (const uint16_t*)p.k + b * p.k_sb + hkv * p.k_sh + (int64_t)c0 * p.k_ss;
   kr.v = (const uint16_t*)p.v + b * p.v_sb + hkv * p.v_sh + (int64_t)c0 * p.v_ss;
-  kr.n = c1 - c0, kr.d = p.d;
+  kr.lo = 0, kr.n = c1 - c0, kr.d = p.d;
   const int at0 = len - p.Sq - c0;  // last key of query 0, from c0
   kr.t_lo = kr.t_flo = 0;
   kr.t_hi = (min(kr.n, max(at0 + ie + 1, 0)) + BN - 1) / BN;

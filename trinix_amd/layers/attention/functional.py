@@ -134,7 +134,10 @@ def packed_attn_func(
         and v.  A row that sees no key (a sequence without keys, a query before
         the first key, padding behind the last sequence) gives 0 and a
         log-sum-exp of -inf, where ``triton_attn_func`` gives NaN: packed
-        batches hold such rows by design.
+        batches hold such rows by design. Rows that see no key, and keys that no
+        row sees (before the window of a chunk's first query, say), may hold
+        anything; NaN or infinity in a key or value that one row sees may reach
+        the other rows of its sequence.
 
     A graph captured around the forward and its backward takes q, k and v that
     no living eager autograd graph holds as leaves (``detach()`` makes such), as
