@@ -294,6 +294,48 @@ def test_same_bits_every_run_and_other_streams():
         assert all(torch.equal(a, b) for a, b in zip(r, ref))
 
 
+def test_a_plan_and_its_calls_on_different_streams():
+    """Calls wait for the plan, and a rebuild waits for the calls, whichever streams they run on."""
+    q, k, v, _ = (t.to(DEV) for t in make(900, 900, 4, 2, 64, BF, 3))
+    bounds = [torch.tensor(b, dtype=torch.int32, device=DEV) for b in ([0, 500, 501, 900], [0, 0, 33, 700])]
+    want = [tx.packed_attn_func(q, k, v, tx.PackedSequences(b, total_q=900), causal=True) for b in bounds]
+    cu = bounds[0].clone()
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(a):
+        torch.cuda._sleep(20_000_000)
+        seqs = tx.PackedSequences(cu, total_q=900)
+    with torch.cuda.stream(b):
+        torch.cuda._sleep(20_000_000)
+        first = tx.packed_attn_func(q, k, v, seqs, causal=True)
+    with torch.cuda.stream(a):
+        cu.copy_(bounds[1])
+        seqs.rebuild()
+    second = tx.packed_attn_func(q, k, v, seqs, causal=True)
+    with torch.cuda.stream(b):
+        third = tx.packed_attn_func(q, k, v, seqs, causal=True)
+        del seqs
+    torch.cuda.synchronize()
+    for got, ref in zip((first, second, third), (want[0], want[1], want[1])):
+        assert torch.equal(got, ref)
+
+
+def test_a_scale_in_a_tensor_is_read_at_every_call():
+    q, k, v, _ = (t.to(DEV) for t in make(50, 50, 2, 2, 64, BF, 3))
+    seqs, scale = tx.PackedSequences([0, 50]), torch.tensor(0.125)
+    first = tx.packed_attn_func(q, k, v, seqs, scale)
+    scale.fill_(0.5)
+    assert torch.equal(tx.packed_attn_func(q, k, v, seqs, scale), tx.packed_attn_func(q, k, v, seqs, 0.5))
+    assert torch.equal(first, tx.packed_attn_func(q, k, v, seqs, 0.125))
+
+
+def test_window_bounds_beyond_64_bits():
+    q, k, v, _ = (t.to(DEV) for t in make(150, 150, 2, 2, 64, BF, 3))
+    seqs = tx.PackedSequences([0, 150])
+    for wide, same in (((1 << 70, 0), (150, 0)), ((3, 1 << 64), (3, 150)), ((-(1 << 70), 5), (-150, 5))):
+        assert torch.equal(tx.packed_attn_func(q, k, v, seqs, window_size=wide), tx.packed_attn_func(q, k, v, seqs, window_size=same))
+
+
 def test_captured_step_with_new_lengths():
     """Plan, forward and backward in one graph; the boundaries change between replays."""
     H, Hkv, D, T = 4, 2, 64, 400

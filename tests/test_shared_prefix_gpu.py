@@ -244,3 +244,14 @@ def test_refusals():
     assert f(z(0, 1, 4, 64), p, p, z(0, 7, 2, 64), z(0, 7, 2, 64)).shape == (0, 1, 4, 64)
     with torch.no_grad():
         assert f(q.requires_grad_(True), p, p, k, k).shape == q.shape
+
+
+def test_a_scale_in_a_tensor_is_read_at_every_call():
+    g = torch.Generator().manual_seed(1)
+    r = lambda *s: torch.randn(*s, generator=g).to(DEV, torch.bfloat16)
+    ts = (r(2, 1, 4, 64), r(70, 2, 64), r(70, 2, 64), r(2, 40, 2, 64), r(2, 40, 2, 64))
+    scale = torch.tensor(0.125)
+    first = tx.shared_prefix_attn_func(*ts, None, scale)
+    scale.fill_(0.5)
+    assert torch.equal(tx.shared_prefix_attn_func(*ts, None, scale), tx.shared_prefix_attn_func(*ts, None, 0.5))
+    assert torch.equal(first, tx.shared_prefix_attn_func(*ts, None, 0.125))

@@ -39,6 +39,10 @@ class PackedSequences:
             behind the last sequence are padding: their output is 0 and they
             take no part in any gradient.
         device: of the plan; by default the boundaries' GPU or the current one.
+
+    The plan is built on the stream that is current then.  Calls on another
+    stream wait for it, and ``rebuild`` waits for the calls, outside of graph
+    captures; inside one the order is the caller's.
     """
 
     def __init__(self, cu_seqlens_q: Boundaries, cu_seqlens_k: Optional[Boundaries] = None, *,
@@ -74,6 +78,8 @@ class PackedSequences:
         self._launches: dict = {}  # of calls with these sequences (_Launch)
         self.plan = torch.empty(n.value // 4, dtype=torch.int32, device=device)
         self.generation = 0
+        self._stream = self._built = None  # where the plan was built, and when
+        self._used: dict = {}  # calls on other streams since then
         self.rebuild()
 
     def _boundaries(self, cu, total, what) -> Tuple[torch.Tensor, int]:
@@ -104,12 +110,34 @@ class PackedSequences:
         the current stream: for boundaries that are written anew in place, and
         inside a captured graph."""
         with torch.cuda.device(self.device):
+            capturing = torch.cuda.is_current_stream_capturing()
+            stream = torch.cuda.current_stream(self.device)
+            if not capturing:
+                if self._built is not None and self._stream != stream:
+                    stream.wait_stream(self._stream)
+                for ev in self._used.values():
+                    stream.wait_event(ev)
             cq = self._source_q.to(torch.int32).contiguous()
             ck = cq if self._source_k is self._source_q else self._source_k.to(torch.int32).contiguous()
             nat.check(nat.load_library().trinix_packed_plan(
                 cq.data_ptr(), ck.data_ptr(), self.n_seqs, self.total_q, self.total_k, self.plan.data_ptr(), self._bytes,
                 current_stream_ptr(self.device)), "trinix_packed_plan")
+            self._used.clear()
+            self._stream, self._stream_ptr = stream, current_stream_ptr(self.device)
+            self._built = None if capturing else stream.record_event()
         self.generation += 1
+
+    def _enter(self, ptr: int) -> None:
+        """A call on another stream than the plan's: waits for the plan, and keeps its memory."""
+        stream = torch.cuda.current_stream(self.device)
+        if self._built is not None:
+            stream.wait_event(self._built)
+        if ptr not in self._used:
+            self._used[ptr] = torch.cuda.Event()
+            self.plan.record_stream(stream)
+
+    def _leave(self, ptr: int) -> None:
+        self._used[ptr].record(torch.cuda.current_stream(self.device))
 
 
 def _strides(t: torch.Tensor):
@@ -187,16 +215,21 @@ class _Launch:
 _MAX_LAUNCHES = 64
 
 
-def _launch(fn: str, a: nat.PackedArgs, device: torch.device) -> None:
-    lib = nat.load_library()
-    if torch.cuda.current_device() == device.index:
-        nat.check(getattr(lib, fn)(ctypes.byref(a), current_stream_ptr(device)), fn)
-    else:
+def _launch(fn: str, a: nat.PackedArgs, seqs: PackedSequences) -> None:
+    device = seqs.device
+    if torch.cuda.current_device() != device.index:
         with torch.cuda.device(device):
-            nat.check(getattr(lib, fn)(ctypes.byref(a), current_stream_ptr(device)), fn)
+            return _launch(fn, a, seqs)
+    stream = current_stream_ptr(device)
+    other = stream != seqs._stream_ptr and not torch.cuda.is_current_stream_capturing()
+    if other:
+        seqs._enter(stream)
+    nat.check(getattr(nat.load_library(), fn)(ctypes.byref(a), stream), fn)
+    if other:
+        seqs._leave(stream)
 
 
-def _run(a, q, slopes, want_lse, keep):
+def _run(a, q, seqs, slopes, want_lse, keep):
     """Allocates the outputs of a forward (arguments a, operands set) and launches
     it: (out at the kernel's head_dim, out_lo, lse)."""
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
@@ -210,7 +243,7 @@ def _run(a, q, slopes, want_lse, keep):
         a.lse = lse.data_ptr()
     if slopes is not None:
         a.alibi_slopes = slopes.data_ptr()
-    _launch("trinix_packed_fwd", a, q.device)
+    _launch("trinix_packed_fwd", a, seqs)
     return out, out_lo, lse
 
 
@@ -220,7 +253,7 @@ class _PackedAttention(torch.autograd.Function):
         D, d_kernel = q.shape[-1], int(a.head_dim)
         if ent is None:
             q, k, v = _set_operands(a, q, k, v, d_kernel)
-        out, out_lo, lse = _run(a, q, slopes, True, True)
+        out, out_lo, lse = _run(a, q, seqs, slopes, True, True)
         ctx.save_for_backward(q, k, v, out, out_lo, lse, slopes)
         ctx.call = (ent, a, seqs, seqs.generation, D)
         res = out if d_kernel == D else out[..., :D].contiguous()
@@ -261,7 +294,7 @@ class _PackedAttention(torch.autograd.Function):
         if n.value:
             ws = torch.empty(n.value, dtype=torch.uint8, device=q.device)
             a.workspace, a.workspace_bytes = ws.data_ptr(), n.value
-        _launch("trinix_packed_bwd", a, q.device)
+        _launch("trinix_packed_bwd", a, seqs)
         if q.shape[-1] != D:
             dq, dk, dv = dq[..., :D], dk[..., :D], dv[..., :D]
         return dq, dk, dv, None, None, None, None, None
@@ -287,7 +320,7 @@ def _args(q, k, seqs, scale, causal, window_size, slopes, d_kernel) -> nat.Packe
     a.causal = 1 if causal else 0
     if window_size is not None:
         a.has_window = 1
-        a.window_left, a.window_right = int(window_size[0]), int(window_size[1])
+        a.window_left, a.window_right = (min(max(w, -1 << 62), 1 << 62) for w in window_size)
     if slopes is not None:
         a.alibi_stride = 1
     return a
@@ -303,6 +336,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sequence
         raise ValueError(f"sequences must be PackedSequences, got {type(sequences)}")
     if window_size is not None:
         window_size = (int(window_size[0]), int(window_size[1]))
+    if scale is not None:
+        scale = float(scale)
     grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
     if alibi_slopes is not None and alibi_slopes.requires_grad and torch.is_grad_enabled():
         raise ValueError("alibi_slopes are constants without a gradient; pass alibi_slopes.detach()")
@@ -339,7 +374,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sequence
         return _PackedAttention.apply(q, k, v, ent, a, sequences, slopes, return_lse)
     D = q.shape[-1]
     ops = (q, k, v) if ent is not None else _set_operands(a, q, k, v, int(a.head_dim))  # held until the launch returns
-    out, _, lse = _run(a, ops[0], slopes, return_lse, False)
+    out, _, lse = _run(a, ops[0], sequences, slopes, return_lse, False)
     if out.shape[-1] != D:
         out = out[..., :D].contiguous()
     return (out, lse) if return_lse else out

@@ -72,6 +72,8 @@ def shared_prefix_attention(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: t
     if torch.is_grad_enabled() and (q.requires_grad or prefix_k.requires_grad or prefix_v.requires_grad or k.requires_grad
                                     or v.requires_grad):
         raise ValueError("shared_prefix_attention has no backward; call it under torch.no_grad()")
+    if scale is not None:
+        scale = float(scale)
     key = _key(*ts, seq_lens, scale, return_lse)
     ent = _LAUNCHES.get(key)
     if ent is not None:
