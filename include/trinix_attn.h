@@ -512,15 +512,20 @@ typedef struct trinix_packed_args {
   int64_t window_left, window_right;
   const float* alibi_slopes; /* (Hq) fp32, or NULL */
   int64_t alibi_stride;
-  void* workspace;      /* backward: trinix_packed_bwd_workspace bytes, 16-byte aligned */
+  void* workspace;      /* trinix_packed_fwd_workspace or trinix_packed_bwd_workspace
+                         * bytes, 16-byte aligned; forward: or NULL */
   int64_t workspace_bytes;
 } trinix_packed_args;
 
 /* Forward and backward on `stream`; 16-bit rows 16-byte aligned.  The backward
  * takes the forward's out, out_lo and lse.  No atomics: the same call gives the
  * same bits.
+ * trinix_packed_fwd_workspace: bytes of workspace with which the forward of these
+ * arguments shares a block's keys out over several workgroups (host only; 0
+ * where it would not; without it one workgroup walks them all).
  * trinix_packed_bwd_workspace: bytes of workspace that the backward of these
  * arguments takes (host only; 0 where the KV heads alone fill the GPU). */
+int trinix_packed_fwd_workspace(const trinix_packed_args* args, int64_t* bytes);
 int trinix_packed_fwd(const trinix_packed_args* args, void* stream);
 int trinix_packed_bwd_workspace(const trinix_packed_args* args, int64_t* bytes);
 int trinix_packed_bwd(const trinix_packed_args* args, void* stream);

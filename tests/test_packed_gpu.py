@@ -97,6 +97,24 @@ def test_forced_tile_shapes(shape, dtype, D, monkeypatch):
     check([100, 513], window=(-2, 40), causal=False, **kw)
 
 
+@pytest.mark.parametrize("chunks", ["1", "2", "3", "8"])
+@pytest.mark.parametrize("dtype,D", [(BF, 64), (HF, 128), (BF, 256), (HF, 40), (BF, 96)])
+def test_keys_shared_out(chunks, dtype, D, monkeypatch):
+    # the keys of a block of rows over several workgroups, joined by a second launch
+    monkeypatch.setenv("TRINIX_PACKED_CHUNKS", chunks)
+    kw = dict(D=D, dtype=dtype, pad=3)
+    check([1, 5, 0, 70, 3], [1500, 900, 300, 1100, 0], **kw)  # some blocks in one chunk, rows without keys
+    check([700, 1], causal=False, alibi=True, **kw)
+    check([40, 130], [2000, 1000], alibi=True, grad=False, **kw)
+    check([9, 300], [1700, 40], window=(700, 0), grad=False, **kw)
+    check([64, 1], [1200, 1], causal=False, window=(600, -20), grad=False, **kw)
+
+
+def test_single_tokens_behind_long_caches():
+    check([1] * 6, [9000, 1, 3000, 257, 256, 4100], H=8, Hkv=2, D=128, grad=False)
+    check([1, 2], [6000, 70], H=4, Hkv=1, D=64, dtype=HF, alibi=True, grad=False)
+
+
 @pytest.mark.parametrize("splits", ["1", "2", "3", "16"])
 @pytest.mark.parametrize("dtype,D", [(BF, 64), (HF, 128), (BF, 256), (F32, 64), (BF, 80), (F32, 96)])
 def test_heads_shared_out(splits, dtype, D, monkeypatch):

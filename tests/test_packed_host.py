@@ -168,6 +168,39 @@ def test_packed_backward_needs_its_tensors(lib, field):
     assert lib.trinix_packed_bwd(ctypes.byref(a), None) == nat.TRINIX_ERR_NULL_POINTER
 
 
+def test_packed_forward_workspace(lib, monkeypatch):
+    monkeypatch.delenv("TRINIX_PACKED_CHUNKS", raising=False)
+    n = ctypes.c_int64(0)
+
+    def need(**kw):
+        a = args(lib)
+        for k, v in kw.items():
+            setattr(a, k, v)
+        assert lib.trinix_packed_fwd_workspace(ctypes.byref(a), ctypes.byref(n)) == 0
+        return n.value
+
+    long = dict(total_q=8, total_k=16384, n_seqs=4, nheads_q=8, nheads_kv=2, head_dim=128, dtype=nat.TRINIX_BF16)
+    assert need(**long) == 8 * 8 * 8 * 129 * 4
+    assert need(**{**long, "dtype": nat.TRINIX_F32}) == 0  # one workgroup walks them all
+    assert need(**{**long, "total_k": 1000}) == 0
+    assert need(**{**long, "has_window": 1, "window_left": 500, "causal": 1}) == 0
+    assert need(**{**long, "has_window": 1, "window_left": 1 << 62, "window_right": 1 << 62}) == n.value > 0
+    assert need(**{**long, "total_q": 16384, "n_seqs": 64}) == 0  # the rows fill the GPU
+    assert need(**{**long, "total_q": 0}) == 0
+    monkeypatch.setenv("TRINIX_PACKED_CHUNKS", "3")
+    assert need(**long) == 3 * 8 * 8 * 129 * 4
+    monkeypatch.setenv("TRINIX_PACKED_CHUNKS", "-1")
+    assert need(**long) == 0
+    assert lib.trinix_packed_fwd_workspace(None, ctypes.byref(n)) == nat.TRINIX_ERR_NULL_POINTER
+    assert lib.trinix_packed_fwd_workspace(ctypes.byref(args(lib)), None) == nat.TRINIX_ERR_NULL_POINTER
+    for bad in (dict(nheads_q=0), dict(nheads_kv=3), dict(n_seqs=0), dict(total_q=-1), dict(total_q=1 << 30), dict(total_k=1 << 30),
+                dict(head_dim=12, dtype=nat.TRINIX_BF16), dict(head_dim=264)):
+        a = args(lib)
+        for k, v in bad.items():
+            setattr(a, k, v)
+        assert lib.trinix_packed_fwd_workspace(ctypes.byref(a), ctypes.byref(n)) == nat.TRINIX_ERR_BAD_SHAPE
+
+
 def test_packed_backward_workspace(lib):
     n = ctypes.c_int64(-1)
     a = args(lib)  # 8 heads of their own: no head to share out
@@ -252,6 +285,23 @@ int main() {
       }
     }
     EXPECT(packed_plan_ints(tq, tk, n) == end + kPackedLists * packed_scratch_ints(n));
+    // chunks of a run of tiles: every tile in one; which workgroup runs which block of which chunk
+    for (int t = 0; t < 50; ++t) {
+      const int tiles = std::rand() % 300, most = 1 + std::rand() % 8, BN = std::rand() % 2 ? 32 : 64;
+      const int total = std::rand() % 3 ? std::rand() % 4000 : INT32_MAX, heads = 1 + std::rand() % 64;
+      const PackedChunks c = packed_chunks(tiles, BN, most, total, heads, 512);
+      EXPECT(c.n >= 1 && c.n <= most && c.per * (int64_t)BN >= kPackedChunkKeys && (int64_t)c.n * c.per >= tiles);
+      EXPECT(c.n == 1 || (c.n - 1) * c.per < tiles);
+      // every block of every chunk once
+      const int per = kXcds * (1 + std::rand() % 20);
+      std::set<std::pair<int, int>> seen;
+      for (int b = 0; b < per * most; ++b) {
+        const int x = packed_chunk_block(b, b / per, per);
+        EXPECT(x >= 0 && x < per);
+        seen.insert({b / per, x});
+      }
+      EXPECT((int)seen.size() == per * most);
+    }
     // the band against its definition, tile ranges around it
     for (int t = 0; t < 20; ++t) {
       const int lq = 1 + std::rand() % 300, lk = 1 + std::rand() % 300;

@@ -270,6 +270,7 @@ SIGNATURES = {
     "trinix_packed_plan_bytes": (c_int32, [c_int64, c_int64, c_int64, POINTER(c_int64)]),
     "trinix_packed_plan": (c_int32, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p]),
     "trinix_packed_fwd": (c_int32, [POINTER(PackedArgs), c_void_p]),
+    "trinix_packed_fwd_workspace": (c_int32, [POINTER(PackedArgs), POINTER(c_int64)]),
     "trinix_packed_bwd_workspace": (c_int32, [POINTER(PackedArgs), POINTER(c_int64)]),
     "trinix_packed_bwd": (c_int32, [POINTER(PackedArgs), c_void_p]),
     "trinix_shared_prefix_workspace": (c_int32, [POINTER(SharedPrefixArgs), POINTER(c_int64)]),

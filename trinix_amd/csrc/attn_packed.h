@@ -33,6 +33,10 @@ struct PackedParams {
   // and dK, key, KV head, head_dim), or 1 and null
   int n_split, Tk;
   float* part;
+  // forward: at most n_chunks workgroups share the keys of a block of rows, each leaving
+  // its normalised O in part (chunk, head, row, D) and its log-sum-exp (log2) in part_lse
+  int n_chunks;
+  float* part_lse;
   int rows16;             // fp32: the tiles' tensors take 16-byte copies (of dK, dV: q and dout)
   int rows16_q;           // the same of the backward's dQ: k and v
   const int32_t* items;   // of the launch's list
@@ -43,6 +47,7 @@ struct PackedParams {
 // rows, first key and keys), block number (-1: none) and head, all wave-uniform.
 struct PackedBlock {
   int q0, lq, k0, lk, blk, h, dlo, dhi;
+  int total;  // of the list
   __device__ PackedBlock(const PackedParams& p, const int32_t* items, int wg, int heads_kv, int G) {
     typedef int i32x4 __attribute__((ext_vector_type(4)));
     const PackedWork w = packed_work(wg, heads_kv, G);
@@ -52,7 +57,9 @@ struct PackedBlock {
     lq = __builtin_amdgcn_readfirstlane(a[1]);
     k0 = __builtin_amdgcn_readfirstlane(a[2]);
     lk = __builtin_amdgcn_readfirstlane(a[3]);
-    blk = __builtin_amdgcn_readfirstlane(it[1][0]);
+    const i32x4 b = it[1];
+    blk = __builtin_amdgcn_readfirstlane(b[0]);
+    total = __builtin_amdgcn_readfirstlane(b[2]);
     h = w.h;
     packed_band(lq, lk, p.causal != 0, p.has_window != 0, p.wl, p.wr, dlo, dhi);
   }
@@ -172,6 +179,9 @@ constexpr int packed_lds_dim(int C) { return C == 96 ? 128 : C; }
 // list at p.items times the heads.  ks: wavefronts per 32 rows (keys).
 hipError_t launch_packed_fwd_bf16(const PackedParams& p, int C, PackedShape shape, int grid, hipStream_t st);
 hipError_t launch_packed_fwd_f16(const PackedParams& p, int C, PackedShape shape, int grid, hipStream_t st);
+// The same with the keys shared out (kPair; head_dim 256: kPlain), grid per chunk.
+hipError_t launch_packed_chunks_bf16(const PackedParams& p, int C, int grid, hipStream_t st);
+hipError_t launch_packed_chunks_f16(const PackedParams& p, int C, int grid, hipStream_t st);
 hipError_t launch_packed_fwd_f32(const PackedParams& p, int C, int ks, int grid, hipStream_t st);
 // Backward, one launch: n_kv workgroups of dK and dV, n_q of dQ.
 hipError_t launch_packed_bwd_f32(const PackedParams& p, int C, int ks, int n_kv, int n_q, hipStream_t st);

@@ -5,26 +5,38 @@
 
 namespace trinix {
 
-// NW * 32 / KS query rows of one sequence and head (the list's block).
-template <class E, int C, int BN, int NW, int OCC, int KS, int ALIBI>
+// NW * 32 / KS query rows of one sequence and head (the list's block).  SPLIT: p.n_chunks
+// workgroups share the block's keys (those of a short range leave at once), and
+// packed_fwd_merge joins what they leave; where one does it all it writes the result.
+template <class E, int C, int BN, int NW, int OCC, int KS, int ALIBI, bool SPLIT>
 __global__ __launch_bounds__(NW * 64, OCC) void packed_fwd16(const PackedParams p) {
   constexpr int BM = NW * 32 / KS, D = packed_lds_dim(C), DB = C / 32;
   TRINIX_TILE16_LDS(D, BN, KS);
-  const PackedBlock w(p, p.items, (int)blockIdx.x, p.Hkv, p.G);
+  const int per_chunk = SPLIT ? (int)gridDim.x / p.n_chunks : 1, chunk = SPLIT ? (int)blockIdx.x / per_chunk : 0;
+  const PackedBlock w(p, p.items, SPLIT ? packed_chunk_block((int)blockIdx.x, chunk, per_chunk) : (int)blockIdx.x, p.Hkv, p.G);
   if (w.blk < 0) return;
+  KeyRun kr;
+  PackedChunks chunks{0, 1};
+  const int m0 = w.blk * BM, mlast = min(m0 + BM, w.lq) - 1;
+  bwd_key_tiles(m0, BM, w.lq, w.lk, w.dlo, w.dhi, BN, kr.t_lo, kr.t_hi);
+  packed_full_tiles(m0, mlast, w.lk, w.dlo, w.dhi, BN, kr.t_lo, kr.t_hi, kr.t_flo, kr.t_fhi);
+  if constexpr (SPLIT) {
+    chunks = packed_chunks(kr.t_hi - kr.t_lo, BN, p.n_chunks, w.total, p.Hq, D == 256 ? 256 : 512);
+    if (chunk >= chunks.n) return;
+    kr.t_lo += chunk * chunks.per;
+    kr.t_hi = min(kr.t_hi, kr.t_lo + chunks.per);
+    kr.t_flo = min(max(kr.t_flo, kr.t_lo), kr.t_hi);
+    kr.t_fhi = min(max(kr.t_fhi, kr.t_flo), kr.t_hi);
+  }
   Tile16<E, D, C, BN, NW, KS, ALIBI> T(lds_k0, lds_k1, lds_v0, lds_v1);
-  const int hq = w.h, hkv = hq / p.G, m0 = w.blk * BM, iw0 = m0 + (T.wave / KS) * 32, i = iw0 + T.r;
+  const int hq = w.h, hkv = hq / p.G, iw0 = m0 + (T.wave / KS) * 32, i = iw0 + T.r;
   T.load_q((const uint16_t*)p.q + (int64_t)(w.q0 + min(i, w.lq - 1)) * p.q_ss + hq * p.q_sh, p.d, p.scale_log2,
            ALIBI ? p.alibi[hq * p.al_sh] : 0.f);
   const Span ks = w.keys_of(i);
-  const int mlast = min(m0 + BM, w.lq) - 1;
-  KeyRun kr;
   kr.k = (const uint16_t*)p.k + (int64_t)w.k0 * p.k_ss + hkv * p.k_sh;
   kr.v = (const uint16_t*)p.v + (int64_t)w.k0 * p.v_ss + hkv * p.v_sh;
   const PackedRange seen = w.keys();
   kr.k_ss = p.k_ss, kr.v_ss = p.v_ss, kr.lo = seen.lo, kr.n = seen.hi + 1, kr.d = p.d;
-  bwd_key_tiles(m0, BM, w.lq, w.lk, w.dlo, w.dhi, BN, kr.t_lo, kr.t_hi);
-  packed_full_tiles(m0, mlast, w.lk, w.dlo, w.dhi, BN, kr.t_lo, kr.t_hi, kr.t_flo, kr.t_fhi);
   kr.jlo = ks.lo, kr.jspan = ks.span;
   // (a wavefront whose rows all lie behind the sequence sees nothing)
   kr.wlo = iw0 < w.lq ? iw0 + w.dlo : INT_MAX;
@@ -35,6 +47,17 @@ __global__ __launch_bounds__(NW * 64, OCC) void packed_fwd16(const PackedParams 
   if (i >= w.lq || T.kp != 0) return;
   const float inv = l > 0.f ? 1.f / l : 0.f;  // a row that sees no key: 0
   const int64_t row = w.q0 + i;
+  if (SPLIT && chunks.n > 1) {
+    const int64_t at = ((int64_t)chunk * p.Hq + hq) * p.Tq + row;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int vq = 0; vq < 4; ++vq)
+        *(f32x4_t*)(p.part + at * D + db * 32 + vq * 8 + T.g * 4) =
+            (f32x4_t){T.acc[db][vq * 4] * inv, T.acc[db][vq * 4 + 1] * inv, T.acc[db][vq * 4 + 2] * inv, T.acc[db][vq * 4 + 3] * inv};
+    if (T.g == 0) p.part_lse[at] = l > 0.f ? T.m_run + __log2f(l) : -INFINITY;
+    return;
+  }
   uint16_t* orow = (uint16_t*)p.o + row * p.o_ss + hq * p.o_sh;
 #pragma unroll
   for (int db = 0; db < DB; ++db)
@@ -57,14 +80,14 @@ __global__ __launch_bounds__(NW * 64, OCC) void packed_fwd16(const PackedParams 
   if (p.lse && T.g == 0) p.lse[(int64_t)hq * p.Tq + row] = l > 0.f ? (T.m_run + __log2f(l)) * kLn2 : -INFINITY;
 }
 
-template <class E, int C, int BN, int NW, int OCC, int KS>
+template <class E, int C, int BN, int NW, int OCC, int KS, bool SPLIT = false>
 hipError_t launch_packed_fwd16(const PackedParams& p, int grid, hipStream_t st) {
   const dim3 g((unsigned)grid), b(NW * 64);
-  if (!p.alibi) return launch_kernel(&packed_fwd16<E, C, BN, NW, OCC, KS, 0>, g, b, 0, st, p);
+  if (!p.alibi) return launch_kernel(&packed_fwd16<E, C, BN, NW, OCC, KS, 0, SPLIT>, g, b, 0, st, p);
   // (a causal row sees no key behind it; 128-key tiles and head_dim 256 have no registers for 2)
   if constexpr (BN <= 64 && C <= 128)
-    if (p.causal) return launch_kernel(&packed_fwd16<E, C, BN, NW, OCC, KS, 2>, g, b, 0, st, p);
-  return launch_kernel(&packed_fwd16<E, C, BN, NW, OCC, KS, 1>, g, b, 0, st, p);
+    if (p.causal) return launch_kernel(&packed_fwd16<E, C, BN, NW, OCC, KS, 2, SPLIT>, g, b, 0, st, p);
+  return launch_kernel(&packed_fwd16<E, C, BN, NW, OCC, KS, 1, SPLIT>, g, b, 0, st, p);
 }
 
 template <class E, int C>
@@ -88,6 +111,80 @@ hipError_t launch_packed_fwd16(const PackedParams& p, int C, PackedShape shape, 
     case 96: return launch_packed_fwd16_128<E, 96>(p, shape, grid, st);
     case 128: return launch_packed_fwd16_128<E, 128>(p, shape, grid, st);
     case 256: return launch_packed_fwd16<E, 256, 64, 4, 1, 1>(p, grid, st);
+  }
+  return hipErrorNotSupported;
+}
+
+// Joins the chunks' results: the blocks of the launch before, D / 4 threads a row, four
+// columns each; blocks that one workgroup did leave at once.
+template <class E, int D, int BM, int BN>
+__global__ __launch_bounds__(256) void packed_fwd_merge(const PackedParams p) {
+  constexpr int TPR = D / 4, UNR = 4;
+  const PackedBlock w(p, p.items, (int)blockIdx.x, p.Hkv, p.G);
+  if (w.blk < 0) return;
+  const int m0 = w.blk * BM, hq = w.h, c = (int)threadIdx.x % TPR;
+  int t_lo, t_hi;
+  bwd_key_tiles(m0, BM, w.lq, w.lk, w.dlo, w.dhi, BN, t_lo, t_hi);
+  const int n = packed_chunks(t_hi - t_lo, BN, p.n_chunks, w.total, p.Hq, D == 256 ? 256 : 512).n;
+  if (n <= 1) return;
+  const int64_t step = (int64_t)p.Hq * p.Tq;
+  for (int i = m0 + (int)threadIdx.x / TPR; i < min(m0 + BM, w.lq); i += 256 / TPR) {
+    const int64_t row = w.q0 + i, at = hq * (int64_t)p.Tq + row;
+    const float* pl = p.part_lse + at;
+    const float* po = p.part + at * D + c * 4;
+    float m = -INFINITY, L = 0.f;
+    f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < n; s0 += UNR) {
+      float ls[UNR], mn = m;
+      f32x4_t ov[UNR];
+#pragma unroll
+      for (int u = 0; u < UNR; ++u) {
+        const int64_t s = min(s0 + u, n - 1) * step;
+        ls[u] = s0 + u < n ? pl[s] : -INFINITY;
+        ov[u] = *(const f32x4_t*)(po + s * D);
+        mn = fmaxf(mn, ls[u]);
+      }
+      const float m_use = mn == -INFINITY ? 0.f : mn, a = __builtin_amdgcn_exp2f(m - m_use);
+      L *= a;
+      o *= a;
+#pragma unroll
+      for (int u = 0; u < UNR; ++u) {
+        const float f = __builtin_amdgcn_exp2f(ls[u] - m_use);
+        L += f;
+        o += f * ov[u];
+      }
+      m = mn;
+    }
+    const float inv = L > 0.f ? 1.f / L : 0.f;  // a row that sees no key: 0
+    if (c * 4 < p.d) {
+      o *= inv;
+      const u32x2_t hi = {E::pack(o[0], o[1]), E::pack(o[2], o[3])};
+      const int64_t to = row * p.o_ss + hq * p.o_sh + c * 4;
+      *(u32x2_t*)((uint16_t*)p.o + to) = hi;
+      if (p.o_lo) {
+        constexpr float f = kLoScale<E>;
+        *(u32x2_t*)((uint16_t*)p.o_lo + to) = (u32x2_t){E::pack((o[0] - E::lo(hi[0])) * f, (o[1] - E::hi(hi[0])) * f),
+                                                        E::pack((o[2] - E::lo(hi[1])) * f, (o[3] - E::hi(hi[1])) * f)};
+      }
+    }
+    if (p.lse && c == 0) p.lse[at] = L > 0.f ? (m + __log2f(L)) * kLn2 : -INFINITY;
+  }
+}
+
+// grid: blocks times heads.
+template <class E, int C, int BN, int OCC, int KS>
+hipError_t launch_packed_chunks16(const PackedParams& p, int grid, hipStream_t st) {
+  const hipError_t e = launch_packed_fwd16<E, C, BN, 4, OCC, KS, true>(p, grid * p.n_chunks, st);
+  if (e != hipSuccess) return e;
+  return launch_kernel(&packed_fwd_merge<E, packed_lds_dim(C), 128 / KS, BN>, dim3((unsigned)grid), dim3(256), 0, st, p);
+}
+template <class E>
+hipError_t launch_packed_chunks16(const PackedParams& p, int C, int grid, hipStream_t st) {
+  switch (C) {
+    case 64: return launch_packed_chunks16<E, 64, 64, 2, 2>(p, grid, st);
+    case 96: return launch_packed_chunks16<E, 96, 32, 2, 2>(p, grid, st);
+    case 128: return launch_packed_chunks16<E, 128, 32, 2, 2>(p, grid, st);
+    case 256: return launch_packed_chunks16<E, 256, 64, 1, 1>(p, grid, st);
   }
   return hipErrorNotSupported;
 }

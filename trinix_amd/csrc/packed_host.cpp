@@ -83,6 +83,32 @@ int64_t packed_partial_bytes(const trinix_packed_args* a) {
   return n > 1 ? 2ll * n * a->total_k * a->nheads_kv * packed_kernel_dim(a->head_dim) * 4 : 0;
 }
 
+
+// A few rows behind long caches are a few long chains of tiles: their keys go over up to
+// eight workgroups each, as many as the lengths in the plan ask for (packed_chunks), and a
+// second launch joins them.  Measured, us whole | shared out: bf16 32/8 heads of 128, one
+// token behind 4000 keys 56 | 18, 4 behind 8000 106 | 44, 64 rows behind 8000 109 | 40, 512
+// 128 | 102; 12 chunks of 0 to 34 rows, two of them behind 5745 and 7929 keys, 16 heads 106 |
+// 31; 8 tokens behind 3000, 16/4 heads of 64 26 | 19, of 256 103 | 63.  It loses where the
+// chains are short (30 x 30 rows behind 300 18.6 | 21) or fill the GPU (64 tokens of 32
+// heads behind 600 62 | 65), and gains little on prompts (8192 rows of 4 heads 124 | 108, 2048
+// of 8 33 | 35, 6 x 600 14 | 23), so those stay whole.
+constexpr int kPackedChunksMost = 8;
+int packed_key_chunks(const trinix_packed_args* a) {
+  if (a->dtype == TRINIX_F32 || a->total_q == 0) return 1;
+  const char* env = getenv("TRINIX_PACKED_CHUNKS");  // (tuning and tests)
+  if (env) return (int)lmax(1, lmin(lmin(kPackedChunksMost, atoi(env)), INT32_MAX / (packed_list_cap(a->total_q, a->n_seqs, 64) * a->nheads_q)));
+  const int64_t block = packed_kernel_dim(a->head_dim) == 256 ? 128 : 64;
+  int64_t keys = a->total_k;  // of the longest chain, at most
+  if (a->has_window) keys = lmin(keys, lmax(0, clamp_window(a->window_left)) + lmax(0, a->causal ? 0 : clamp_window(a->window_right)) + block);
+  const int64_t wgs = (a->total_q / block + lmin(a->n_seqs, a->total_q)) * a->nheads_q;
+  return keys >= 2048 && a->total_k >= 2 * a->total_q && wgs <= 512 ? kPackedChunksMost : 1;
+}
+int64_t packed_chunk_bytes(const trinix_packed_args* a) {
+  const int n = packed_key_chunks(a);
+  return n > 1 ? (int64_t)n * a->nheads_q * a->total_q * (packed_kernel_dim(a->head_dim) + 1) * 4 : 0;
+}
+
 namespace {
 
 // (batch, rows, heads, head_dim) or, without a batch, (rows, heads, head_dim):
@@ -177,6 +203,15 @@ int plan_shared(const trinix_shared_prefix_args* a, SharedPlan* pl) {
 
 using namespace trinix;
 
+extern "C" int trinix_packed_fwd_workspace(const trinix_packed_args* a, int64_t* bytes) {
+  if (!a || !bytes) return TRINIX_ERR_NULL_POINTER;
+  if (a->nheads_q <= 0 || a->nheads_kv <= 0 || a->nheads_q > (1 << 20) || a->nheads_q % a->nheads_kv != 0 || a->n_seqs < 1 ||
+      a->total_q < 0 || a->total_q >= (1ll << 30) || a->total_k < 0 || a->total_k >= (1ll << 30) ||
+      !packed_head_dim_ok(a->head_dim, a->dtype))
+    return TRINIX_ERR_BAD_SHAPE;
+  *bytes = packed_chunk_bytes(a);
+  return TRINIX_OK;
+}
 extern "C" int trinix_packed_bwd_workspace(const trinix_packed_args* a, int64_t* bytes) {
   if (!a || !bytes) return TRINIX_ERR_NULL_POINTER;
   if (a->nheads_q <= 0 || a->nheads_kv <= 0 || a->nheads_q > (1 << 20) || a->nheads_q % a->nheads_kv != 0 || a->n_seqs < 1 ||

@@ -13,7 +13,8 @@ namespace trinix {
 // (lists 0..2) and of 64 and 128 keys (lists 3, 4) of one sequence each, the
 // longest first.  An item is eight int32:
 //   first query row, query rows, first key, keys of its sequence; block number
-//   (-1: no item); sequence; two zeros.
+//   (-1: no item); sequence; the sum of the costs (packed_cost) of the list's items, in
+//   64s; zero.
 // Rows behind the last sequence form a sequence of their own without keys
 // (their output is 0), keys behind it one without rows (their gradients are 0).
 constexpr int kPackedLists = 5;
@@ -133,6 +134,27 @@ __host__ __device__ inline PackedRange packed_tile_range(const PackedRange& r, i
   t.hi = imax(r.hi - n0, 0);
   t.lo = imin(imax(r.lo - n0, 0), t.hi);
   return t;
+}
+
+// A block's `tiles` tiles of BN keys over at most `most` workgroups: tiles per chunk and
+// chunks (1 for no tiles).  A chunk is at least kPackedChunkKeys keys and at least what
+// each of `slots` workgroups would take of all items' keys (`total`, in 64s) and heads.
+constexpr int kPackedChunkKeys = 512;
+struct PackedChunks {
+  int per, n;
+};
+__host__ __device__ inline PackedChunks packed_chunks(int tiles, int BN, int most, int total, int heads, int slots) {
+  const int64_t share = (int64_t)total * heads / slots * (64 / BN);
+  PackedChunks c;
+  c.per = (int)lmin(lmax(lmax(kPackedChunkKeys / BN, share), (tiles + most - 1) / most), INT32_MAX);
+  c.n = imax(1, (int)(((int64_t)tiles + c.per - 1) / c.per));
+  return c;
+}
+// Workgroup of a grid of `per_chunk` (whole rounds of the XCDs) per chunk: a block's
+// chunks on different XCDs.
+__host__ __device__ inline int packed_chunk_block(int blk, int chunk, int per_chunk) {
+  const int b = blk - chunk * per_chunk;
+  return b / kXcds * kXcds + (b + chunk * (kXcds - 1)) % kXcds;
 }
 
 // Tiles of BN keys, within [t_lo, t_hi), whose keys all of rows m0 .. mlast see.

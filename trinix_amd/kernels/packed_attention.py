@@ -206,10 +206,16 @@ def _check(q, k, v, seqs: PackedSequences, alibi_slopes) -> None:
 # shapes, strides, types and scalars.  The first one goes through every check and
 # leaves its arguments; the first backward leaves its own, per strides of dout.
 class _Launch:
-    __slots__ = ("fwd", "bwd", "slopes_as_given")
+    __slots__ = ("fwd", "bwd", "slopes_as_given", "ws_bytes")
 
-    def __init__(self, fwd, slopes_as_given):
-        self.fwd, self.bwd, self.slopes_as_given = fwd, {}, slopes_as_given
+    def __init__(self, fwd, slopes_as_given, ws_bytes):
+        self.fwd, self.bwd, self.slopes_as_given, self.ws_bytes = fwd, {}, slopes_as_given, ws_bytes
+
+
+def _fwd_workspace(a) -> int:
+    n = ctypes.c_int64(0)
+    nat.check(nat.load_library().trinix_packed_fwd_workspace(ctypes.byref(a), ctypes.byref(n)), "trinix_packed_fwd_workspace")
+    return n.value
 
 
 _MAX_LAUNCHES = 64
@@ -229,7 +235,7 @@ def _launch(fn: str, a: nat.PackedArgs, seqs: PackedSequences) -> None:
         seqs._leave(stream)
 
 
-def _run(a, q, seqs, slopes, want_lse, keep):
+def _run(a, ent, q, seqs, slopes, want_lse, keep):
     """Allocates the outputs of a forward (arguments a, operands set) and launches
     it: (out at the kernel's head_dim, out_lo, lse)."""
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
@@ -243,6 +249,10 @@ def _run(a, q, seqs, slopes, want_lse, keep):
         a.lse = lse.data_ptr()
     if slopes is not None:
         a.alibi_slopes = slopes.data_ptr()
+    n = _fwd_workspace(a) if ent is None else ent.ws_bytes
+    if n:
+        ws = torch.empty(n, dtype=torch.uint8, device=q.device)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), n
     _launch("trinix_packed_fwd", a, seqs)
     return out, out_lo, lse
 
@@ -253,7 +263,7 @@ class _PackedAttention(torch.autograd.Function):
         D, d_kernel = q.shape[-1], int(a.head_dim)
         if ent is None:
             q, k, v = _set_operands(a, q, k, v, d_kernel)
-        out, out_lo, lse = _run(a, q, seqs, slopes, True, True)
+        out, out_lo, lse = _run(a, ent, q, seqs, slopes, True, True)
         ctx.save_for_backward(q, k, v, out, out_lo, lse, slopes)
         ctx.call = (ent, a, seqs, seqs.generation, D)
         res = out if d_kernel == D else out[..., :D].contiguous()
@@ -288,6 +298,7 @@ class _PackedAttention(torch.autograd.Function):
         a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
         if slopes is not None:
             a.alibi_slopes = slopes.data_ptr()
+        a.workspace, a.workspace_bytes = None, 0  # (fwd may hold the forward's)
         n = ctypes.c_int64(0)
         nat.check(nat.load_library().trinix_packed_bwd_workspace(ctypes.byref(a), ctypes.byref(n)),
                   "trinix_packed_bwd_workspace")
@@ -364,7 +375,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sequence
             _set_operands(a, q, k, v, d_kernel)
             as_given = alibi_slopes is not None and (alibi_slopes.dim() == 1 and alibi_slopes.dtype == torch.float32
                                                      and alibi_slopes.device == q.device and alibi_slopes.is_contiguous())
-            ent = _Launch(nat.PackedArgs.from_buffer_copy(a), as_given)
+            ent = _Launch(nat.PackedArgs.from_buffer_copy(a), as_given, _fwd_workspace(a))
             ent.fwd.q = ent.fwd.k = ent.fwd.v = None
             if not (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16:
                 if len(sequences._launches) >= _MAX_LAUNCHES:
@@ -374,7 +385,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sequence
         return _PackedAttention.apply(q, k, v, ent, a, sequences, slopes, return_lse)
     D = q.shape[-1]
     ops = (q, k, v) if ent is not None else _set_operands(a, q, k, v, int(a.head_dim))  # held until the launch returns
-    out, _, lse = _run(a, ops[0], sequences, slopes, return_lse, False)
+    out, _, lse = _run(a, ent, ops[0], sequences, slopes, return_lse, False)
     if out.shape[-1] != D:
         out = out[..., :D].contiguous()
     return (out, lse) if return_lse else out
