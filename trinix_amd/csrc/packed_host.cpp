@@ -146,13 +146,21 @@ int validate_shared(const trinix_shared_prefix_args* a) {
   return TRINIX_OK;
 }
 
-// Blocks of whole rows that fill the chip: from 192 on one workgroup per block walks
-// all keys.  Measured, bf16, us split | whole 64 | whole 128: 256 blocks of 64 rows (B=32
-// Sq=16 G=4, P=4096) 85 | 66; 64 of them 30 | 62; 512 blocks of 32 rows (B=64 Sq=8 16/4
-// D=64, P=2048) 30 | 27; of 16 rows (Sq=4, P=8192) 76 | 149; 512 blocks of 128 rows (B=8
-// Sq=256 G=4, P=6000) 309 | 246 | 204; 256 of them (B=16 Sq=100 16/16 D=64) 51 | 22 | 22;
-// 56 (B=2 Sq=200 16/4) 41 | 63 | 78.
-constexpr int64_t kSharedWhole = 192;
+// Does one workgroup per block of `bm` whole rows walk all keys, or do workgroups share
+// them out?  Whole blocks read nothing twice and need no second launch; few of them are a
+// chain of all keys on few CUs, and blocks of one request's rows hold fewer than blocks of
+// the batch's do (`packed`, what the prefix takes shared out).  So: from `full` blocks on,
+// below that while keys are few, fewer the emptier the chip and the blocks.  Measured, us
+// shared out | whole 64 (head_dim 256: 128), bf16:
+//  - head_dim 128, Sq=95 16/4 heads, P=301, caches of 1001: B=15 53 | 30, 6 34 | 24, 3 29 | 23;
+//    P=3000: 90 | 70, 57 | 57, 32 | 49; Sq=72 16/16 B=2 P=5335 29 | 85; Sq=60 B=8 P=500 27 | 17;
+//    Sq=10 32/8 P=500 B=16 29 | 20, B=4 13 | 18; Sq=33 16/16 B=5 P=1500 21 | 30; Sq=200 32/8 B=2
+//    P=6000 100 | 88;
+//  - 256: Sq=95 16/4 P=301 B=15 97 | 56, 6 66 | 51, 3 42 | 47; P=3000 156 | 134, 84 | 126.
+// Blocks under 32 rows are shared out: of 16 (Sq=4, B=64, P=8192) 76 | 149.
+bool whole_blocks(int64_t keys, int64_t n, int64_t packed, int64_t full, int64_t limit) {
+  return n >= full || keys * (full - n) * n < limit * packed;
+}
 
 int plan_shared(const trinix_shared_prefix_args* a, SharedPlan* pl) {
   const int64_t G = a->nheads_q / a->nheads_kv, own = a->seqlen_q * G, rows = a->batch * own, kv = a->nheads_kv;
@@ -161,8 +169,12 @@ int plan_shared(const trinix_shared_prefix_args* a, SharedPlan* pl) {
   pl->rows = (int)rows;
   const bool d256 = packed_kernel_dim(a->head_dim) == 256;
   pl->kind = f32 ? SharedKind::kRows16 : SharedKind::kSplit;
-  if (!f32 && !d256 && own >= 32 && own <= 64 && a->batch * kv >= kSharedWhole) pl->kind = SharedKind::kWhole64;
-  else if (!f32 && own > 64 && a->batch * blocks(own, 128) * kv >= kSharedWhole) pl->kind = SharedKind::kWhole128;
+  // 128-row blocks where they fill the chip (B=8 Sq=256 G=4 P=6000 309 shared out, 246 in blocks
+  // of 64, 204 in blocks of 128); head_dim 256 has no others
+  const int64_t keys = a->prefix_len + a->capacity, b64 = a->batch * blocks(own, 64) * kv, b128 = a->batch * blocks(own, 128) * kv;
+  if (!f32 && own > 64 && b128 >= 192) pl->kind = SharedKind::kWhole128;
+  else if (!f32 && !d256 && own >= 32 && whole_blocks(keys, b64, blocks(rows, 64) * kv, 225, 210000)) pl->kind = SharedKind::kWhole64;
+  else if (!f32 && d256 && own >= 32 && whole_blocks(keys, b128, blocks(rows, 128) * kv, 192, 160000)) pl->kind = SharedKind::kWhole128;
   if (const char* env = getenv("TRINIX_SHARED_KIND")) {  // 1, 2, 3: split, whole 64, whole 128 (tuning and tests)
     const int want = atoi(env);
     if (!f32 && want >= 1 && want <= 3 && !(d256 && want == 2)) pl->kind = (SharedKind)want;
