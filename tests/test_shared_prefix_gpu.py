@@ -141,6 +141,29 @@ def test_forced_kinds(kind, dtype, D, monkeypatch):
     check(2, 7, 65, 0, [0, 0], H=6, Hkv=3, D=D, dtype=dtype)
 
 
+@pytest.mark.parametrize("kind", ["1", "2", "3"])
+def test_small_calls_by_every_kind(kind, monkeypatch):
+    # (the rule takes whole rows for most of these sizes)
+    monkeypatch.setenv("TRINIX_SHARED_KIND", kind)
+    for H, Hkv in ((1, 1), (16, 1), (6, 3), (40, 2)):
+        check(3, 2, 150, 90, [2, 90, 33], H=H, Hkv=Hkv, seed=H)
+    check(4, 3, 0, 40, [0, 2, 3, 40], D=64)
+    check(4, 3, 20, 40, [0, 1, 3, 40], D=64)
+    check(2, 1, 50, 0, [0, 0], D=64)
+    check(2, 2, 0, 0, [0, 0], D=128)
+    check(20, 3, 129, 70, [3 + 3 * b for b in range(20)], D=64)
+    check(3, 2, 100, 64, [64, 5, 33], layout="bshd", scale=-0.3, dtype=HF, D=80)
+    check(3, 2, 100, 64, None, poison=False, scale=0.0)
+    check(4, 1, 60, 64, [-5, 1000, 64, 0], poison=False)
+
+
+def test_another_kind_for_a_call_seen_before(monkeypatch):
+    # its workspace was sized for the first one
+    for kind in ("3", "1", "2", "1"):
+        monkeypatch.setenv("TRINIX_SHARED_KIND", kind)
+        check(3, 2, 150, 90, [2, 90, 33], seed=3)
+
+
 def test_lengths_outside_the_cache_are_clamped():
     check(4, 1, 60, 64, [-5, 1000, 64, 0], poison=False)
 

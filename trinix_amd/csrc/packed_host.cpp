@@ -157,7 +157,10 @@ int validate_shared(const trinix_shared_prefix_args* a) {
 //    Sq=10 32/8 P=500 B=16 29 | 20, B=4 13 | 18; Sq=33 16/16 B=5 P=1500 21 | 30; Sq=200 32/8 B=2
 //    P=6000 100 | 88;
 //  - 256: Sq=95 16/4 P=301 B=15 97 | 56, 6 66 | 51, 3 42 | 47; P=3000 156 | 134, 84 | 126.
-// Blocks under 32 rows are shared out: of 16 (Sq=4, B=64, P=8192) 76 | 149.
+// Blocks under 32 rows are shared out (of 16, Sq=4, B=64, P=8192, 76 | 149) but for a few
+// hundred keys, where one launch costs the host 4 us less and the GPU no more: 4 tokens of
+// 32/8 heads of 64 behind 400 keys 8.1 | 8.5, called in turn 13.1 | 9.2; of 128 behind 150 9.0
+// | 7.9, behind 400 9.4 | 11.2.
 bool whole_blocks(int64_t keys, int64_t n, int64_t packed, int64_t full, int64_t limit) {
   return n >= full || keys * (full - n) * n < limit * packed;
 }
@@ -174,6 +177,7 @@ int plan_shared(const trinix_shared_prefix_args* a, SharedPlan* pl) {
   const int64_t keys = a->prefix_len + a->capacity, b64 = a->batch * blocks(own, 64) * kv, b128 = a->batch * blocks(own, 128) * kv;
   if (!f32 && own > 64 && b128 >= 192) pl->kind = SharedKind::kWhole128;
   else if (!f32 && !d256 && own >= 32 && whole_blocks(keys, b64, blocks(rows, 64) * kv, 225, 210000)) pl->kind = SharedKind::kWhole64;
+  else if (!f32 && !d256 && own < 32 && keys * packed_kernel_dim(a->head_dim) <= 32768 && b64 <= 512) pl->kind = SharedKind::kWhole64;
   else if (!f32 && d256 && own >= 32 && whole_blocks(keys, b128, blocks(rows, 128) * kv, 192, 160000)) pl->kind = SharedKind::kWhole128;
   if (const char* env = getenv("TRINIX_SHARED_KIND")) {  // 1, 2, 3: split, whole 64, whole 128 (tuning and tests)
     const int want = atoi(env);

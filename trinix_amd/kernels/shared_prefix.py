@@ -6,7 +6,6 @@ whole batch instead of once per request; no counterpart in the reference.
 from __future__ import annotations
 
 import ctypes
-import os
 from typing import Optional
 
 import torch
@@ -60,8 +59,7 @@ _MAX_LAUNCHES = 256
 def _key(q, pk, pv, k, v, lens, scale, return_lse):
     return (q.shape, q.stride(), pk.shape, pk.stride(), pv.shape, pv.stride(), k.shape, k.stride(), v.shape, v.stride(),
             q.dtype, pk.dtype, pv.dtype, k.dtype, v.dtype, q.device, pk.device, pv.device, k.device, v.device,
-            None if lens is None else (lens.shape, lens.stride(), lens.dtype, lens.device), scale, return_lse,
-            os.environ.get("TRINIX_SHARED_KIND"))
+            None if lens is None else (lens.shape, lens.stride(), lens.dtype, lens.device), scale, return_lse)
 
 
 def shared_prefix_attention(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Tensor, k: torch.Tensor,
@@ -158,11 +156,16 @@ def _run(a: nat.SharedPrefixArgs, ent: _Launch, q: torch.Tensor):
     if ent.lse_shape is not None:
         lse = torch.empty(ent.lse_shape, dtype=torch.float32, device=device)
         a.lse = lse.data_ptr()
-    if ent.ws_bytes is None:
+    kept = ent.ws_bytes is not None
+    if not kept:
         n = ctypes.c_int64(0)
         nat.check(lib.trinix_shared_prefix_workspace(ctypes.byref(a), ctypes.byref(n)), "trinix_shared_prefix_workspace")
         ent.ws_bytes = n.value
     ws = torch.empty(ent.ws_bytes, dtype=torch.uint8, device=device) if ent.ws_bytes else None
-    nat.check(lib.trinix_shared_prefix_fwd(ctypes.byref(a), None if ws is None else ws.data_ptr(), ent.ws_bytes,
-                                           current_stream_ptr(device)), "trinix_shared_prefix_fwd")
+    rc = lib.trinix_shared_prefix_fwd(ctypes.byref(a), None if ws is None else ws.data_ptr(), ent.ws_bytes,
+                                      current_stream_ptr(device))
+    if rc == nat.TRINIX_ERR_BAD_ARGUMENT and kept:  # another kind than when the size was asked for (TRINIX_SHARED_KIND)
+        ent.ws_bytes = None
+        return _run(a, ent, q)
+    nat.check(rc, "trinix_shared_prefix_fwd")
     return out if lse is None else (out, lse)
