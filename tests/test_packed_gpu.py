@@ -217,6 +217,34 @@ def test_strided_operands():
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+def test_offsets_beyond_32_bits(dtype):
+    """Rows 8192 elements apart, the last ones more than 2^32 bytes and 2^31 elements behind the first: as a copy."""
+    n, D = 300_000, 64
+    cu_q, cu_k = [0, 1, 101, 164], [0, 298_500, 299_500, n]
+    g = torch.Generator(device=DEV).manual_seed(1)
+    r = lambda *s: torch.randn(s, generator=g, device=DEV).to(dtype)
+    wide = torch.empty(n, 2, 4096, dtype=dtype, device=DEV)
+    k, v = wide[:, :, :D], wide[:, :, 100 * 8:100 * 8 + D]
+    k.copy_(r(n, 2, D)), v.copy_(r(n, 2, D))
+    q, do = r(164, 4, D), r(164, 4, D)
+    seqs = tx.PackedSequences(cu_q, cu_k)
+
+    def run(k, v):
+        a, b, c = q.clone().requires_grad_(True), k.detach().requires_grad_(True), v.detach().requires_grad_(True)
+        out = tx.packed_attn_func(a, b, c, seqs, causal=True)
+        return (out.detach(), *torch.autograd.grad(out, (a, b, c), do))
+
+    for a, b in zip(run(k, v), run(k.contiguous(), v.contiguous())):
+        assert torch.equal(a, b)
+    # queries that far behind, of a few keys
+    wide[-164:, :, :D] = q.view(164, 2, 2, D)[:, :, 0]
+    few = tx.PackedSequences([0, n - 164, n], [0, 10, 40])
+    got = tx.packed_attn_func(wide[:, :, :D], k[:40], v[:40], few, causal=False)
+    want = tx.packed_attn_func(wide[-164:, :, :D].contiguous(), k[10:40], v[10:40], tx.PackedSequences([0, 164], [0, 30]))
+    assert torch.equal(got[-164:], want)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 def test_unaligned_operands(dtype):
     base = torch.randn(200 * 2 * 64 + 3, generator=torch.Generator().manual_seed(1)).to(dtype)
     t = base[3:].view(200, 2, 64)

@@ -107,6 +107,22 @@ def test_long_prefix_and_long_caches():
     check(2, 1, 20000, 9000, [9000, 4001], H=4, Hkv=1, D=128)
 
 
+@pytest.mark.parametrize("dtype,Sq", [(BF, 1), (BF, 70), (F32, 1)])
+def test_offsets_beyond_32_bits(dtype, Sq):
+    """Caches and a prefix that end more than 2^32 bytes and 2^31 elements behind their start: as copies."""
+    g = torch.Generator(device=DEV).manual_seed(1)
+    r = lambda *s: torch.randn(s, generator=g, device=DEV).to(dtype)
+    B, P, S, D = 3, 270_000, 90_000, 64
+    wide = torch.empty(B * S, 2, 4096, dtype=dtype, device=DEV)
+    wide[:, :, :2 * D] = r(B * S, 2, 2 * D)
+    cache = wide.view(B, S, 2, 4096)
+    args = (wide[:, :, :D], wide[:, :, D:2 * D], cache[..., :D], cache[..., D:2 * D])
+    q, lens = r(B, Sq, 4, D), torch.tensor([S, 100, S - 3], device=DEV)
+    assert args[0].shape[0] == P
+    got = tx.shared_prefix_attn_func(q, *args, lens)
+    assert torch.equal(got, tx.shared_prefix_attn_func(q, *(t.contiguous() for t in args), lens))
+
+
 def test_layouts_and_scales():
     check(3, 2, 100, 64, [64, 5, 33], layout="bshd")
     check(3, 2, 100, 64, None, poison=False)
