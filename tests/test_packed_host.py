@@ -193,8 +193,8 @@ def test_packed_forward_workspace(lib, monkeypatch):
     assert need(**long) == 0
     assert lib.trinix_packed_fwd_workspace(None, ctypes.byref(n)) == nat.TRINIX_ERR_NULL_POINTER
     assert lib.trinix_packed_fwd_workspace(ctypes.byref(args(lib)), None) == nat.TRINIX_ERR_NULL_POINTER
-    for bad in (dict(nheads_q=0), dict(nheads_kv=3), dict(n_seqs=0), dict(total_q=-1), dict(total_q=1 << 30), dict(total_k=1 << 30),
-                dict(head_dim=12, dtype=nat.TRINIX_BF16), dict(head_dim=264)):
+    for bad in (dict(nheads_q=0), dict(nheads_kv=3), dict(n_seqs=0), dict(n_seqs=(1 << 63) - 1), dict(total_q=-1),
+                dict(total_q=1 << 30), dict(total_k=1 << 30), dict(head_dim=12, dtype=nat.TRINIX_BF16), dict(head_dim=264)):
         a = args(lib)
         for k, v in bad.items():
             setattr(a, k, v)

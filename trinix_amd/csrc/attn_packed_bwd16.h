@@ -86,8 +86,8 @@ __device__ __forceinline__ void packed_dkdv_body(const PackedParams& p, const Pa
 #pragma unroll
     for (int l = 0; l < LPW; ++l) {
       const int row = tile_copy_row(wave, LPW, l, lane, UPR);
-      dma_16b_s(tile_copy_offset((uint32_t)min(max(row, t.lo), t.hi), ss, (uint32_t)min((lane % UPR) ^ swz_kt<D>(row), p.d / 8 - 1)), gb,
-                __builtin_amdgcn_readfirstlane(lds0 + l * 1024));
+      const uint32_t src = (uint32_t)min(max(row, t.lo), t.hi), unit = (uint32_t)min((lane % UPR) ^ swz_kt<D>(row), p.d / 8 - 1);
+      dma_16b_s(tile_copy_offset(src, ss, unit), gb, __builtin_amdgcn_readfirstlane(lds0 + l * 1024));
     }
   };
   float lse_pend = 0.f, del_pend = 0.f;
@@ -285,8 +285,9 @@ __device__ __forceinline__ void packed_dkdv_body(const PackedParams& p, const Pa
     for (int db = 0; db < DB; ++db)
 #pragma unroll
       for (int vq = 0; vq < 4; ++vq)
-        if (db * 32 + vq * 8 < p.d) O::store4(row, db * 32 + vq * 8 + g * 4, acc[db][vq * 4] * f, acc[db][vq * 4 + 1] * f, acc[db][vq * 4 + 2] * f,
-                  acc[db][vq * 4 + 3] * f);
+        if (db * 32 + vq * 8 < p.d)
+          O::store4(row, db * 32 + vq * 8 + g * 4, acc[db][vq * 4] * f, acc[db][vq * 4 + 1] * f, acc[db][vq * 4 + 2] * f,
+                    acc[db][vq * 4 + 3] * f);
   };
   if (wave >= NG) run(std::true_type{});
   else run(std::false_type{});
@@ -382,8 +383,9 @@ __device__ __forceinline__ void packed_dq_body(const PackedParams& p, const Pack
   for (int db = 0; db < DB; ++db)
 #pragma unroll
     for (int vq = 0; vq < 4; ++vq)
-      if (db * 32 + vq * 8 < p.d) O::store4(row, db * 32 + vq * 8 + g * 4, acc[db][vq * 4] * f, acc[db][vq * 4 + 1] * f, acc[db][vq * 4 + 2] * f,
-                acc[db][vq * 4 + 3] * f);
+      if (db * 32 + vq * 8 < p.d)
+        O::store4(row, db * 32 + vq * 8 + g * 4, acc[db][vq * 4] * f, acc[db][vq * 4 + 1] * f, acc[db][vq * 4 + 2] * f,
+                  acc[db][vq * 4 + 3] * f);
 }
 
 // Workgroups [0, n_kv): dK and dV of p.items; behind them dQ of p.items_q.

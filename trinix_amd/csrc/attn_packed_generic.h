@@ -151,8 +151,9 @@ __global__ __launch_bounds__(256, OCC) void packed_fwd_f32(const PackedParams p)
   for (int db = 0; db < DB; ++db)
 #pragma unroll
     for (int vq = 0; vq < 4; ++vq)
-      if (db * 32 + vq * 8 + g * 4 < p.d) O::store4(orow, db * 32 + vq * 8 + g * 4, acc[db][vq * 4] * inv, acc[db][vq * 4 + 1] * inv, acc[db][vq * 4 + 2] * inv,
-                acc[db][vq * 4 + 3] * inv);
+      if (db * 32 + vq * 8 + g * 4 < p.d)
+        O::store4(orow, db * 32 + vq * 8 + g * 4, acc[db][vq * 4] * inv, acc[db][vq * 4 + 1] * inv, acc[db][vq * 4 + 2] * inv,
+                  acc[db][vq * 4 + 3] * inv);
   if (p.lse && g == 0) p.lse[(int64_t)hq * p.Tq + row] = l > 0.f ? (m_run + log2f(l)) * kLn2 : -INFINITY;
 }
 
@@ -402,7 +403,8 @@ __device__ __forceinline__ void generic_dq_body(const PackedParams& p, int wg, c
 #pragma unroll
     for (int vq = 0; vq < 4; ++vq) {
       const int d0 = (db0 + db) * 32 + vq * 8 + g * 4;
-      if (d0 < p.d) O::store4(row, d0, acc[db][vq * 4] * f, acc[db][vq * 4 + 1] * f, acc[db][vq * 4 + 2] * f, acc[db][vq * 4 + 3] * f);
+      if (d0 < p.d)
+        O::store4(row, d0, acc[db][vq * 4] * f, acc[db][vq * 4 + 1] * f, acc[db][vq * 4 + 2] * f, acc[db][vq * 4 + 3] * f);
     }
 }
 

@@ -96,11 +96,16 @@ int64_t packed_partial_bytes(const trinix_packed_args* a) {
 constexpr int kPackedChunksMost = 8;
 int packed_key_chunks(const trinix_packed_args* a) {
   if (a->dtype == TRINIX_F32 || a->total_q == 0) return 1;
-  const char* env = getenv("TRINIX_PACKED_CHUNKS");  // (tuning and tests)
-  if (env) return (int)lmax(1, lmin(lmin(kPackedChunksMost, atoi(env)), INT32_MAX / (packed_list_cap(a->total_q, a->n_seqs, 64) * a->nheads_q)));
+  if (const char* env = getenv("TRINIX_PACKED_CHUNKS")) {  // (tuning and tests)
+    const int64_t grids = INT32_MAX / (packed_list_cap(a->total_q, a->n_seqs, 64) * a->nheads_q);
+    return (int)lmax(1, lmin(lmin(kPackedChunksMost, atoi(env)), grids));
+  }
   const int64_t block = packed_kernel_dim(a->head_dim) == 256 ? 128 : 64;
   int64_t keys = a->total_k;  // of the longest chain, at most
-  if (a->has_window) keys = lmin(keys, lmax(0, clamp_window(a->window_left)) + lmax(0, a->causal ? 0 : clamp_window(a->window_right)) + block);
+  if (a->has_window) {
+    const int64_t right = a->causal ? 0 : clamp_window(a->window_right);
+    keys = lmin(keys, lmax(0, clamp_window(a->window_left)) + lmax(0, right) + block);
+  }
   const int64_t wgs = (a->total_q / block + lmin(a->n_seqs, a->total_q)) * a->nheads_q;
   return keys >= 2048 && a->total_k >= 2 * a->total_q && wgs <= 512 ? kPackedChunksMost : 1;
 }
@@ -175,10 +180,12 @@ int plan_shared(const trinix_shared_prefix_args* a, SharedPlan* pl) {
   // 128-row blocks where they fill the chip (B=8 Sq=256 G=4 P=6000 309 shared out, 246 in blocks
   // of 64, 204 in blocks of 128); head_dim 256 has no others
   const int64_t keys = a->prefix_len + a->capacity, b64 = a->batch * blocks(own, 64) * kv, b128 = a->batch * blocks(own, 128) * kv;
-  if (!f32 && own > 64 && b128 >= 192) pl->kind = SharedKind::kWhole128;
-  else if (!f32 && !d256 && own >= 32 && whole_blocks(keys, b64, blocks(rows, 64) * kv, 225, 210000)) pl->kind = SharedKind::kWhole64;
-  else if (!f32 && !d256 && own < 32 && keys * packed_kernel_dim(a->head_dim) <= 32768 && b64 <= 512) pl->kind = SharedKind::kWhole64;
-  else if (!f32 && d256 && own >= 32 && whole_blocks(keys, b128, blocks(rows, 128) * kv, 192, 160000)) pl->kind = SharedKind::kWhole128;
+  if (!f32) {
+    const bool few = keys * packed_kernel_dim(a->head_dim) <= 32768 && b64 <= 512;
+    if (own > 64 && b128 >= 192) pl->kind = SharedKind::kWhole128;
+    else if (!d256 && (own >= 32 ? whole_blocks(keys, b64, blocks(rows, 64) * kv, 225, 210000) : few)) pl->kind = SharedKind::kWhole64;
+    else if (d256 && own >= 32 && whole_blocks(keys, b128, blocks(rows, 128) * kv, 192, 160000)) pl->kind = SharedKind::kWhole128;
+  }
   if (const char* env = getenv("TRINIX_SHARED_KIND")) {  // 1, 2, 3: split, whole 64, whole 128 (tuning and tests)
     const int want = atoi(env);
     if (!f32 && want >= 1 && want <= 3 && !(d256 && want == 2)) pl->kind = (SharedKind)want;
@@ -222,7 +229,7 @@ using namespace trinix;
 extern "C" int trinix_packed_fwd_workspace(const trinix_packed_args* a, int64_t* bytes) {
   if (!a || !bytes) return TRINIX_ERR_NULL_POINTER;
   if (a->nheads_q <= 0 || a->nheads_kv <= 0 || a->nheads_q > (1 << 20) || a->nheads_q % a->nheads_kv != 0 || a->n_seqs < 1 ||
-      a->total_q < 0 || a->total_q >= (1ll << 30) || a->total_k < 0 || a->total_k >= (1ll << 30) ||
+      a->n_seqs >= (1ll << 24) || a->total_q < 0 || a->total_q >= (1ll << 30) || a->total_k < 0 || a->total_k >= (1ll << 30) ||
       !packed_head_dim_ok(a->head_dim, a->dtype))
     return TRINIX_ERR_BAD_SHAPE;
   *bytes = packed_chunk_bytes(a);

@@ -388,8 +388,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void shared_whole(const Shar
   for (int db = 0; db < D / 32; ++db)
 #pragma unroll
     for (int vq = 0; vq < 4; ++vq)
-      if (db * 32 + vq * 8 < p.d) Row<E>::store4(o + db * 32 + vq * 8 + T.g * 4, T.acc[db][vq * 4] * inv, T.acc[db][vq * 4 + 1] * inv,
-                        T.acc[db][vq * 4 + 2] * inv, T.acc[db][vq * 4 + 3] * inv);
+      if (db * 32 + vq * 8 < p.d)
+        Row<E>::store4(o + db * 32 + vq * 8 + T.g * 4, T.acc[db][vq * 4] * inv, T.acc[db][vq * 4 + 1] * inv,
+                       T.acc[db][vq * 4 + 2] * inv, T.acc[db][vq * 4 + 3] * inv);
   if (p.lse && T.g == 0)
     p.lse[((int64_t)b * p.Hq + row.h) * p.Sq + row.i] = l > 0.f ? (T.m_run + __log2f(l)) * kLn2 : -INFINITY;
 }
@@ -454,8 +455,9 @@ __global__ __launch_bounds__(256) void shared_merge(const SharedParams p) {
     oo += w * s_o[k][t];
   }
   const float inv = LL > 0.f ? 1.f / LL : 0.f;  // a row that sees no key: 0
-  if (t * 4 < p.d) Row<E>::store4((Store*)p.o + b * p.o_sb + (int64_t)i * p.o_ss + hq * p.o_sh + t * 4, oo[0] * inv, oo[1] * inv, oo[2] * inv,
-            oo[3] * inv);
+  if (t * 4 < p.d)
+    Row<E>::store4((Store*)p.o + b * p.o_sb + (int64_t)i * p.o_ss + hq * p.o_sh + t * 4, oo[0] * inv, oo[1] * inv, oo[2] * inv,
+                   oo[3] * inv);
   if (p.lse && t == 0) p.lse[((int64_t)b * p.Hq + hq) * p.Sq + i] = LL > 0.f ? (mm + __log2f(LL)) * kLn2 : -INFINITY;
 }
 
