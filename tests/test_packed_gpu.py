@@ -98,7 +98,8 @@ def test_forced_tile_shapes(shape, dtype, D, monkeypatch):
 
 
 @pytest.mark.parametrize("chunks", ["1", "2", "3", "8"])
-@pytest.mark.parametrize("dtype,D", [(BF, 64), (HF, 128), (BF, 256), (HF, 40), (BF, 96)])
+@pytest.mark.parametrize("dtype,D", [(BF, 64), (HF, 128), (BF, 256), (HF, 40), (BF, 96), (F32, 64), (F32, 80), (F32, 128),
+                                     (F32, 256)])
 def test_keys_shared_out(chunks, dtype, D, monkeypatch):
     # the keys of a block of rows over several workgroups, joined by a second launch
     monkeypatch.setenv("TRINIX_PACKED_CHUNKS", chunks)
@@ -113,6 +114,7 @@ def test_keys_shared_out(chunks, dtype, D, monkeypatch):
 def test_single_tokens_behind_long_caches():
     check([1] * 6, [9000, 1, 3000, 257, 256, 4100], H=8, Hkv=2, D=128, grad=False)
     check([1, 2], [6000, 70], H=4, Hkv=1, D=64, dtype=HF, alibi=True, grad=False)
+    check([1, 2], [6000, 70], H=4, Hkv=1, D=64, dtype=F32, grad=False)
 
 
 @pytest.mark.parametrize("splits", ["1", "2", "3", "16"])

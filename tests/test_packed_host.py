@@ -181,7 +181,7 @@ def test_packed_forward_workspace(lib, monkeypatch):
 
     long = dict(total_q=8, total_k=16384, n_seqs=4, nheads_q=8, nheads_kv=2, head_dim=128, dtype=nat.TRINIX_BF16)
     assert need(**long) == 8 * 8 * 8 * 129 * 4
-    assert need(**{**long, "dtype": nat.TRINIX_F32}) == 0  # one workgroup walks them all
+    assert need(**{**long, "dtype": nat.TRINIX_F32, "head_dim": 40}) == 8 * 8 * 8 * 65 * 4
     assert need(**{**long, "total_k": 1000}) == 0
     assert need(**{**long, "has_window": 1, "window_left": 500, "causal": 1}) == 0
     assert need(**{**long, "has_window": 1, "window_left": 1 << 62, "window_right": 1 << 62}) == n.value > 0

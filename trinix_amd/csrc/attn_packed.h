@@ -162,6 +162,10 @@ struct PackedCopy {
   }
 };
 
+// Workgroups that the fp32 forward has on the GPU at once.
+template <int D>
+constexpr int kPackedF32Slots = D == 64 ? 512 : 256;
+
 // fp16 keeps its output's rounding residue times 2^11 (half a step of the
 // largest fp16 number is 2^4; unscaled, the residue of 2^-10 would be denormal).
 template <class E>
@@ -179,9 +183,10 @@ constexpr int packed_lds_dim(int C) { return C == 96 ? 128 : C; }
 // list at p.items times the heads.  ks: wavefronts per 32 rows (keys).
 hipError_t launch_packed_fwd_bf16(const PackedParams& p, int C, PackedShape shape, int grid, hipStream_t st);
 hipError_t launch_packed_fwd_f16(const PackedParams& p, int C, PackedShape shape, int grid, hipStream_t st);
-// The same with the keys shared out (kPair; head_dim 256: kPlain), grid per chunk.
+// The same with the keys shared out (blocks of 64 rows; head_dim 256: 128), grid per chunk.
 hipError_t launch_packed_chunks_bf16(const PackedParams& p, int C, int grid, hipStream_t st);
 hipError_t launch_packed_chunks_f16(const PackedParams& p, int C, int grid, hipStream_t st);
+hipError_t launch_packed_chunks_f32(const PackedParams& p, int C, int grid, hipStream_t st);
 hipError_t launch_packed_fwd_f32(const PackedParams& p, int C, int ks, int grid, hipStream_t st);
 // Backward, one launch: n_kv workgroups of dK and dV, n_q of dQ.
 hipError_t launch_packed_bwd_f32(const PackedParams& p, int C, int ks, int n_kv, int n_q, hipStream_t st);

@@ -183,17 +183,19 @@ extern "C" int trinix_packed_fwd(const trinix_packed_args* a, void* stream) {
   hipStream_t st = (hipStream_t)stream;
   const int C = packed_columns(a->head_dim);
   hipError_t e;
-  if (a->dtype == TRINIX_F32) {
-    p.rows16 = rows16(a->k, a->k_stride) && rows16(a->v, a->v_stride);
-    const int ks = fp32_wavefronts(a);
-    e = launch_packed_fwd_f32(p, C, ks, (int)(use_list(p, a, ks == 2 ? kRows64 : kRows128) * p.Hq), st);
-  } else if (const int64_t bytes = packed_chunk_bytes(a); bytes > 0 && a->workspace && a->workspace_bytes >= bytes &&
-                                                          ((uintptr_t)a->workspace & 15) == 0) {
+  p.rows16 = a->dtype == TRINIX_F32 && rows16(a->k, a->k_stride) && rows16(a->v, a->v_stride);
+  const int64_t bytes = packed_chunk_bytes(a);
+  if (bytes > 0 && a->workspace && a->workspace_bytes >= bytes && ((uintptr_t)a->workspace & 15) == 0) {
     p.n_chunks = packed_key_chunks(a);
     p.part = (float*)a->workspace;
     p.part_lse = p.part + (int64_t)p.n_chunks * p.Hq * p.Tq * packed_lds_dim(C);
     const int grid = (int)(use_list(p, a, C == 256 ? kRows128 : kRows64) * p.Hq);
-    e = a->dtype == TRINIX_BF16 ? launch_packed_chunks_bf16(p, C, grid, st) : launch_packed_chunks_f16(p, C, grid, st);
+    e = a->dtype == TRINIX_F32    ? launch_packed_chunks_f32(p, C, grid, st)
+        : a->dtype == TRINIX_BF16 ? launch_packed_chunks_bf16(p, C, grid, st)
+                                  : launch_packed_chunks_f16(p, C, grid, st);
+  } else if (a->dtype == TRINIX_F32) {
+    const int ks = fp32_wavefronts(a);
+    e = launch_packed_fwd_f32(p, C, ks, (int)(use_list(p, a, ks == 2 ? kRows64 : kRows128) * p.Hq), st);
   } else {
     const PackedShape shape = packed_shape(a);
     const int grid = (int)(use_list(p, a, kListOf[(int)shape]) * p.Hq);

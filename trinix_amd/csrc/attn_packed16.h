@@ -1,6 +1,7 @@
 // Packed-sequence attention forward of the 16-bit types on Tile16.
 #pragma once
 #include "attn_packed.h"
+#include "attn_packed_merge.h"
 #include "attn_tile16.h"
 
 namespace trinix {
@@ -21,7 +22,7 @@ __global__ __launch_bounds__(NW * 64, OCC) void packed_fwd16(const PackedParams 
   bwd_key_tiles(m0, BM, w.lq, w.lk, w.dlo, w.dhi, BN, kr.t_lo, kr.t_hi);
   packed_full_tiles(m0, mlast, w.lk, w.dlo, w.dhi, BN, kr.t_lo, kr.t_hi, kr.t_flo, kr.t_fhi);
   if constexpr (SPLIT) {
-    chunks = packed_chunks(kr.t_hi - kr.t_lo, BN, p.n_chunks, w.total, p.Hq, D == 256 ? 256 : 512);
+    chunks = packed_chunks(kr.t_hi - kr.t_lo, BN, p.n_chunks, w.total, p.Hq, C == 256 ? 256 : 512);
     if (chunk >= chunks.n) return;
     kr.t_lo += chunk * chunks.per;
     kr.t_hi = min(kr.t_hi, kr.t_lo + chunks.per);
@@ -115,68 +116,12 @@ hipError_t launch_packed_fwd16(const PackedParams& p, int C, PackedShape shape, 
   return hipErrorNotSupported;
 }
 
-// Joins the chunks' results: the blocks of the launch before, D / 4 threads a row, four
-// columns each; blocks that one workgroup did leave at once.
-template <class E, int D, int BM, int BN>
-__global__ __launch_bounds__(256) void packed_fwd_merge(const PackedParams p) {
-  constexpr int TPR = D / 4, UNR = 4;
-  const PackedBlock w(p, p.items, (int)blockIdx.x, p.Hkv, p.G);
-  if (w.blk < 0) return;
-  const int m0 = w.blk * BM, hq = w.h, c = (int)threadIdx.x % TPR;
-  int t_lo, t_hi;
-  bwd_key_tiles(m0, BM, w.lq, w.lk, w.dlo, w.dhi, BN, t_lo, t_hi);
-  const int n = packed_chunks(t_hi - t_lo, BN, p.n_chunks, w.total, p.Hq, D == 256 ? 256 : 512).n;
-  if (n <= 1) return;
-  const int64_t step = (int64_t)p.Hq * p.Tq;
-  for (int i = m0 + (int)threadIdx.x / TPR; i < min(m0 + BM, w.lq); i += 256 / TPR) {
-    const int64_t row = w.q0 + i, at = hq * (int64_t)p.Tq + row;
-    const float* pl = p.part_lse + at;
-    const float* po = p.part + at * D + c * 4;
-    float m = -INFINITY, L = 0.f;
-    f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-    for (int s0 = 0; s0 < n; s0 += UNR) {
-      float ls[UNR], mn = m;
-      f32x4_t ov[UNR];
-#pragma unroll
-      for (int u = 0; u < UNR; ++u) {
-        const int64_t s = min(s0 + u, n - 1) * step;
-        ls[u] = s0 + u < n ? pl[s] : -INFINITY;
-        ov[u] = *(const f32x4_t*)(po + s * D);
-        mn = fmaxf(mn, ls[u]);
-      }
-      const float m_use = mn == -INFINITY ? 0.f : mn, a = __builtin_amdgcn_exp2f(m - m_use);
-      L *= a;
-      o *= a;
-#pragma unroll
-      for (int u = 0; u < UNR; ++u) {
-        const float f = __builtin_amdgcn_exp2f(ls[u] - m_use);
-        L += f;
-        o += f * ov[u];
-      }
-      m = mn;
-    }
-    const float inv = L > 0.f ? 1.f / L : 0.f;  // a row that sees no key: 0
-    if (c * 4 < p.d) {
-      o *= inv;
-      const u32x2_t hi = {E::pack(o[0], o[1]), E::pack(o[2], o[3])};
-      const int64_t to = row * p.o_ss + hq * p.o_sh + c * 4;
-      *(u32x2_t*)((uint16_t*)p.o + to) = hi;
-      if (p.o_lo) {
-        constexpr float f = kLoScale<E>;
-        *(u32x2_t*)((uint16_t*)p.o_lo + to) = (u32x2_t){E::pack((o[0] - E::lo(hi[0])) * f, (o[1] - E::hi(hi[0])) * f),
-                                                        E::pack((o[2] - E::lo(hi[1])) * f, (o[3] - E::hi(hi[1])) * f)};
-      }
-    }
-    if (p.lse && c == 0) p.lse[at] = L > 0.f ? (m + __log2f(L)) * kLn2 : -INFINITY;
-  }
-}
-
 // grid: blocks times heads.
 template <class E, int C, int BN, int OCC, int KS>
 hipError_t launch_packed_chunks16(const PackedParams& p, int grid, hipStream_t st) {
   const hipError_t e = launch_packed_fwd16<E, C, BN, 4, OCC, KS, true>(p, grid * p.n_chunks, st);
   if (e != hipSuccess) return e;
-  return launch_kernel(&packed_fwd_merge<E, packed_lds_dim(C), 128 / KS, BN>, dim3((unsigned)grid), dim3(256), 0, st, p);
+  return launch_kernel(&packed_fwd_merge<E, packed_lds_dim(C), 128 / KS, BN, C == 256 ? 256 : 512>, dim3((unsigned)grid), dim3(256), 0, st, p);
 }
 template <class E>
 hipError_t launch_packed_chunks16(const PackedParams& p, int C, int grid, hipStream_t st) {

@@ -27,17 +27,29 @@
 
 namespace trinix {
 
-template <class O, int OCC, int KS>
+// SPLIT: p.n_chunks workgroups share the block's keys (see packed_fwd16).
+template <class O, int OCC, int KS, bool SPLIT>
 __global__ __launch_bounds__(256, OCC) void packed_fwd_f32(const PackedParams p) {
   using Store = typename O::Store;
   constexpr int NW = 4, BM = NW * 32 / KS, D = O::kD, DB = O::DB, TILE = kTileRows * D * (int)sizeof(Store);
   __shared__ __attribute__((aligned(1024))) char lds_k[2][KS * TILE];
   __shared__ __attribute__((aligned(1024))) char lds_v[2][KS * TILE];
-  const PackedBlock w(p, p.items, (int)blockIdx.x, p.Hkv, p.G);
+  const int per_chunk = SPLIT ? (int)gridDim.x / p.n_chunks : 1, chunk = SPLIT ? (int)blockIdx.x / per_chunk : 0;
+  const PackedBlock w(p, p.items, SPLIT ? packed_chunk_block((int)blockIdx.x, chunk, per_chunk) : (int)blockIdx.x, p.Hkv, p.G);
   if (w.blk < 0) return;
+  const int m0 = w.blk * BM;
+  int t_lo, t_hi;
+  bwd_key_tiles(m0, BM, w.lq, w.lk, w.dlo, w.dhi, kTileRows, t_lo, t_hi);
+  PackedChunks chunks{0, 1};
+  if constexpr (SPLIT) {
+    chunks = packed_chunks(t_hi - t_lo, kTileRows, p.n_chunks, w.total, p.Hq, kPackedF32Slots<D>);
+    if (chunk >= chunks.n) return;
+    t_lo += chunk * chunks.per;
+    t_hi = min(t_hi, t_lo + chunks.per);
+  }
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int hq = w.h, hkv = hq / p.G, m0 = w.blk * BM, kp = wave % KS, iw0 = m0 + wave / KS * 32, i = iw0 + r, ic = min(i, w.lq - 1);
+  const int hq = w.h, hkv = hq / p.G, kp = wave % KS, iw0 = m0 + wave / KS * 32, i = iw0 + r, ic = min(i, w.lq - 1);
   const PackedRange kseen = w.keys();
   const bool wide = p.rows16 != 0;
 
@@ -50,8 +62,6 @@ __global__ __launch_bounds__(256, OCC) void packed_fwd_f32(const PackedParams p)
   for (int db = 0; db < DB; ++db) acc[db] = (f32x16_t){};
   float m_run = -INFINITY, l_run = 0.f;
 
-  int t_lo, t_hi;
-  bwd_key_tiles(m0, BM, w.lq, w.lk, w.dlo, w.dhi, kTileRows, t_lo, t_hi);
   const Store* kbase = (const Store*)p.k + (int64_t)w.k0 * p.k_ss + hkv * p.k_sh;
   const Store* vbase = (const Store*)p.v + (int64_t)w.k0 * p.v_ss + hkv * p.v_sh;
   const PackedCopy<O, NW> copy_k(p.k_ss, wave, lane, p.d), copy_v(p.v_ss, wave, lane, p.d);
@@ -146,6 +156,17 @@ __global__ __launch_bounds__(256, OCC) void packed_fwd_f32(const PackedParams p)
   if (i >= w.lq) return;
   const float inv = l > 0.f ? 1.f / l : 0.f;  // a row that sees no key: 0
   const int64_t row = w.q0 + i;
+  if (SPLIT && chunks.n > 1) {
+    const int64_t at = ((int64_t)chunk * p.Hq + hq) * p.Tq + row;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int vq = 0; vq < 4; ++vq)
+        *(f32x4_t*)(p.part + at * D + db * 32 + vq * 8 + g * 4) =
+            (f32x4_t){acc[db][vq * 4] * inv, acc[db][vq * 4 + 1] * inv, acc[db][vq * 4 + 2] * inv, acc[db][vq * 4 + 3] * inv};
+    if (g == 0) p.part_lse[at] = l > 0.f ? m_run + log2f(l) : -INFINITY;
+    return;
+  }
   Store* orow = (Store*)p.o + row * p.o_ss + hq * p.o_sh;
 #pragma unroll
   for (int db = 0; db < DB; ++db)

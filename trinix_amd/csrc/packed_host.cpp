@@ -89,13 +89,14 @@ int64_t packed_partial_bytes(const trinix_packed_args* a) {
 // second launch joins them.  Measured, us whole | shared out: bf16 32/8 heads of 128, one
 // token behind 4000 keys 56 | 18, 4 behind 8000 106 | 44, 64 rows behind 8000 109 | 40, 512
 // 128 | 102; 12 chunks of 0 to 34 rows, two of them behind 5745 and 7929 keys, 16 heads 106 |
-// 31; 8 tokens behind 3000, 16/4 heads of 64 26 | 19, of 256 103 | 63.  It loses where the
+// 31; 8 tokens behind 3000, 16/4 heads of 64 26 | 19, of 256 103 | 63; fp32, one token behind
+// 4000, 32/8 heads of 128 299 | 53, 64 rows behind 8000, 16/4 605 | 98.  It loses where the
 // chains are short (30 x 30 rows behind 300 18.6 | 21) or fill the GPU (64 tokens of 32
 // heads behind 600 62 | 65), and gains little on prompts (8192 rows of 4 heads 124 | 108, 2048
 // of 8 33 | 35, 6 x 600 14 | 23), so those stay whole.
 constexpr int kPackedChunksMost = 8;
 int packed_key_chunks(const trinix_packed_args* a) {
-  if (a->dtype == TRINIX_F32 || a->total_q == 0) return 1;
+  if (a->total_q == 0) return 1;
   if (const char* env = getenv("TRINIX_PACKED_CHUNKS")) {  // (tuning and tests)
     const int64_t grids = INT32_MAX / (packed_list_cap(a->total_q, a->n_seqs, 64) * a->nheads_q);
     return (int)lmax(1, lmin(lmin(kPackedChunksMost, atoi(env)), grids));

@@ -26,7 +26,7 @@ int validate_packed(const trinix_packed_args* a, bool backward);
 int packed_head_splits(const trinix_packed_args* a);
 // Bytes of those partial sums.
 int64_t packed_partial_bytes(const trinix_packed_args* a);
-// Workgroups that share the keys of a block of rows in the 16-bit forward, at most (1:
+// Workgroups that share the keys of a block of rows in the forward, at most (1:
 // none), and the bytes of their fp32 partial results.
 int packed_key_chunks(const trinix_packed_args* a);
 int64_t packed_chunk_bytes(const trinix_packed_args* a);
